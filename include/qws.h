@@ -321,6 +321,61 @@ int qws_head_select_rescore(float* logits, const void* w_bf16, const void* x, in
 const int* qws_head_ws_cand(const void* ws);
 const float* qws_head_ws_exact(const void* ws);
 
+/* Log probabilities of given tokens, their ranks, the rows' entropies and their best alternatives, from rows of logits:
+ * what a request for log probabilities returns with its tokens, and what scores a text or a choice among labels.  Row r is
+ * logits[r * row_stride .. + V) (any V >= 1, any stride >= 0, any alignment of the element's size), as given: with
+ * z_i = x_i / temperature[r] (temperature NULL, 0 or NaN: 1),
+ *   log p_i = z_i - ln sum_j e^(z_j);  entropy = -sum_i p_i log p_i (0 for a row without a candidate);
+ *   rank of token i = the tokens before it in the order (larger logit, then lower index): 0 = the best;
+ *   alternatives = the first `top` tokens of that order, without those at -inf (id -1 and log probability -inf past the
+ *   last one).
+ * As in qws_sample, NaN logits count as -inf.  Several logits at +inf share the row's probability.  A given token at -inf,
+ * or in a row without a candidate, has log probability -inf; a token outside [0, V) (the -1 behind a verify call's
+ * accepted tokens) is skipped: log probability 0, rank -1.  Sums and statistics are fp32.
+ * Limits: V <= 524,288, M <= 64 and top <= 64 (else QWS_ERR_NOT_SUPPORTED).  out_logprobs is needed with M > 0,
+ * out_top_* with top > 0; the others are optional.  Zero-initialise the struct.  ws: qws_logprobs_ws_bytes(dtype, R, V, M,
+ * top) bytes of device memory, 256-byte aligned, no zeroing needed; calls that share one must be ordered.  Allocates
+ * nothing; two launches; deterministic.  No counterpart in the reference, whose server refuses `logprobs`
+ * (server/smk_core_client.py:37-72). */
+typedef struct qws_logprobs_batch {
+  const void* logits; /* device */
+  int dtype;          /* QWS_DTYPE_* */
+  int R, V;
+  long long row_stride; /* elements */
+  const int* tokens;    /* device [R][M], NULL with M = 0 */
+  int M, top;
+  const float* temperature; /* device [R] or NULL */
+  float* out_logprobs;      /* device [R][M] */
+  int* out_ranks;           /* device [R][M] or NULL */
+  float* out_entropy;       /* device [R] or NULL */
+  int* out_top_ids;         /* device [R][top] */
+  float* out_top_logprobs;  /* device [R][top] */
+} qws_logprobs_batch;
+size_t qws_logprobs_ws_bytes(int dtype, int R, int V, int M, int top);
+int qws_logprobs(const qws_logprobs_batch* b, void* ws, size_t ws_bytes, void* stream);
+
+/* A head held in 8 bits: the approximate logits that qws_head_select_rescore refines (the place of the reference's W4
+ * head product, engine/src/head_q.cu:15-100, in another format), and scoring.  Each block of 128 consecutive values of a row
+ * along K (the last may be shorter) is e4m3 values times 2^e, e the least whole number >= -127 with max|x| <= 448 * 2^e;
+ * values are rounded to nearest even; a value that is not finite makes its row's products NaN.  Weights are packed once,
+ * hidden states (bf16) within each call:  y[t][n] = sum over blocks of 2^(ex + ew) * sum_k qx qw, in fp32.
+ *   qws_fp8_pack:  w [N][K] (dtype QWS_DTYPE_*, rows row_stride elements apart) -> packed (device, qws_fp8_pack_bytes(N, K)
+ *                  bytes, 256-byte aligned): about N * K * 65 / 64 bytes, N and K padded to multiples of 256 and 128.
+ *   qws_fp8_head:  x [T][K] bf16 (rows x_stride elements apart) -> out [T][N] (fp32 or bf16, rows out_stride >= N apart).
+ *   qws_fp8_score: per hidden state the log probability of tokens[t] under softmax(y / temperature) and the entropy
+ *                  (optional), by qws_logprobs' rules (skipped tokens, temperatures, NaN); the logits are not stored.
+ * Any N <= 2^24, K <= 2^20, T <= 2^22 (else QWS_ERR_NOT_SUPPORTED), any stride and alignment of the element's size; T = 0
+ * does nothing.  ws: the queried bytes, 256-byte aligned, no zeroing needed; calls that share one must be ordered.
+ * Stream-ordered, allocate nothing, deterministic. */
+size_t qws_fp8_pack_bytes(int N, int K);
+int qws_fp8_pack(const void* w, int dtype, int N, int K, long long row_stride, void* packed, void* stream);
+size_t qws_fp8_head_ws_bytes(int T, int N, int K);
+int qws_fp8_head(const void* packed, int N, int K, const void* x, long long x_stride, int T, void* out, int out_dtype, long long out_stride, void* ws,
+                 size_t ws_bytes, void* stream);
+size_t qws_fp8_score_ws_bytes(int T, int N, int K);
+int qws_fp8_score(const void* packed, int N, int K, const void* x, long long x_stride, int T, const int* tokens, const float* temperature,
+                  float* out_logprobs, float* out_entropy, void* ws, size_t ws_bytes, void* stream);
+
 /* Argmax over fp32 logits [T][N] -> out_tok[t] (lowest index on ties, NaN never wins) and optional
  * out_val[t].  Same signature and contract as the reference's smk_argmax
  * (engine/include/engine.h:68-71, engine/src/misc.cu:133-137); ws of qws_argmax_ws_bytes() bytes. */

@@ -22,6 +22,9 @@ reference's sampling stage (tuan3w/qwen-warp):
       normalised residual max(0, p - q); bonus token from the last row when every draft is accepted
       engine/src/mtp_sample.cu:227-258 (accept_core).
 
+`oracle.logprobs` and `oracle.fp8` define the log probabilities and the 8-bit head in 64 bits (no counterpart in the
+reference).
+
 `oracle.pld` restates the reference's prompt-lookup tail proposer (engine/src/pld.cu, engine/include/pld.h);
 `oracle/build_ref.sh` builds the reference's own proposer from its sources into `oracle/_ref/` (checker only).
 

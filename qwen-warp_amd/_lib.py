@@ -74,10 +74,19 @@ class PldCfg(C.Structure):
     _fields_ = [(k, C.c_int) for k in ("n", "min_len", "max_tail", "cap", "back", "longest")]
 
 
+class LogprobsBatch(C.Structure):
+    """include/qws.h qws_logprobs_batch."""
+    _fields_ = [("logits", C.c_void_p), ("dtype", C.c_int), ("R", C.c_int), ("V", C.c_int), ("row_stride", C.c_longlong), ("tokens", C.c_void_p),
+                ("M", C.c_int), ("top", C.c_int), ("temperature", C.c_void_p), ("out_logprobs", C.c_void_p), ("out_ranks", C.c_void_p),
+                ("out_entropy", C.c_void_p), ("out_top_ids", C.c_void_p), ("out_top_logprobs", C.c_void_p)]
+
+
 EXPORTS = ("qws_sample_ws_bytes", "qws_sample", "qws_sample_noalloc", "qws_verify_ws_bytes", "qws_verify", "qws_verify_map", "qws_draft_pick",
            "qws_row_init_pick", "qws_argmax_ws_bytes", "qws_argmax",
            "qws_state_bytes", "qws_state_begin", "qws_state_note", "qws_state_read",
-           "qws_finish", "qws_finish_rows", "qws_finish_forced", "qws_head_ws_bytes", "qws_head_select_rescore", "qws_head_ws_cand", "qws_head_ws_exact", "qws_pld_default_cfg", "qws_pld_bytes", "qws_pld_reset", "qws_pld_append", "qws_pld_propose",
+           "qws_finish", "qws_finish_rows", "qws_finish_forced", "qws_head_ws_bytes", "qws_head_select_rescore", "qws_head_ws_cand", "qws_head_ws_exact",
+           "qws_logprobs_ws_bytes", "qws_logprobs", "qws_fp8_pack_bytes", "qws_fp8_pack", "qws_fp8_head_ws_bytes", "qws_fp8_head", "qws_fp8_score_ws_bytes",
+           "qws_fp8_score", "qws_pld_default_cfg", "qws_pld_bytes", "qws_pld_reset", "qws_pld_append", "qws_pld_propose",
            "qws_row_init", "qws_row_check", "qws_abi_sizes",
            "qws_timing", "qws_timing_read", "qws_timing_read_verify", "qws_test_philox", "qws_test_proc_logits", "qws_test_dist")
 
@@ -93,7 +102,7 @@ def load(path=None):
     if not p.exists():
         raise RuntimeError(f"libqws.so not built ({p}); run python qwen-warp_amd/build.py")
     lib = C.CDLL(str(p))
-    vp, ci, cu, sz = C.c_void_p, C.c_int, C.c_uint, C.c_size_t
+    vp, ci, cu, sz, ll = C.c_void_p, C.c_int, C.c_uint, C.c_size_t, C.c_longlong
     lib.qws_sample_ws_bytes.argtypes, lib.qws_sample_ws_bytes.restype = [ci, ci], sz
     lib.qws_sample.argtypes, lib.qws_sample.restype = [C.POINTER(Batch), vp, sz, vp], ci
     lib.qws_sample_noalloc.argtypes, lib.qws_sample_noalloc.restype = [C.POINTER(Batch), vp], ci
@@ -119,6 +128,14 @@ def load(path=None):
     lib.qws_head_select_rescore.restype = ci
     lib.qws_head_ws_cand.argtypes, lib.qws_head_ws_cand.restype = [vp], vp
     lib.qws_head_ws_exact.argtypes, lib.qws_head_ws_exact.restype = [vp], vp
+    lib.qws_logprobs_ws_bytes.argtypes, lib.qws_logprobs_ws_bytes.restype = [ci] * 5, sz
+    lib.qws_logprobs.argtypes, lib.qws_logprobs.restype = [C.POINTER(LogprobsBatch), vp, sz, vp], ci
+    lib.qws_fp8_pack_bytes.argtypes, lib.qws_fp8_pack_bytes.restype = [ci, ci], sz
+    lib.qws_fp8_pack.argtypes, lib.qws_fp8_pack.restype = [vp, ci, ci, ci, ll, vp, vp], ci
+    lib.qws_fp8_head_ws_bytes.argtypes, lib.qws_fp8_head_ws_bytes.restype = [ci] * 3, sz
+    lib.qws_fp8_head.argtypes, lib.qws_fp8_head.restype = [vp, ci, ci, vp, ll, ci, vp, ci, ll, vp, sz, vp], ci
+    lib.qws_fp8_score_ws_bytes.argtypes, lib.qws_fp8_score_ws_bytes.restype = [ci] * 3, sz
+    lib.qws_fp8_score.argtypes, lib.qws_fp8_score.restype = [vp, ci, ci, vp, ll, ci, vp, vp, vp, vp, vp, sz, vp], ci
     lib.qws_pld_default_cfg.argtypes, lib.qws_pld_default_cfg.restype = [C.POINTER(PldCfg)], None
     lib.qws_pld_bytes.argtypes, lib.qws_pld_bytes.restype = [ci, ci], sz
     lib.qws_pld_reset.argtypes, lib.qws_pld_reset.restype = [vp, ci, ci, ci, vp, ci, vp], ci

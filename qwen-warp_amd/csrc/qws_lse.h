@@ -1,0 +1,52 @@
+// Running log-sum-exp of a row of logits with its entropy: the statistics that the log-probability kernels
+// (qws_logprobs.hip) and the scoring head (qws_fp8.hip) keep per lane, join over lanes, waves and workgroups, and finish.
+//
+// With c = log2(e) / T and d_i = c (x_i - m), m the largest x so far:
+//   s = sum 2^d_i,   t = sum 2^d_i d_i    (fp32)
+// A larger maximum m' (delta = c (m' - m)) turns them into 2^-delta s and 2^-delta (t - delta s): one pass, any order.
+// Then, with both terms of H >= 0 (s >= 1, t <= 0: nothing cancels),
+//   log p_i = (x_i - m) / T - ln s,   H = ln s - ln 2 * t / s.
+// Differences to the maximum are taken before the scaling, so rows at the type's lowest value and rows mixing it with
+// -inf are exact; NaN counts as -inf (the sampling stage's rule), +inf as the largest finite value (so tokens at +inf share
+// the row); d is held above -D_MIN, where 2^d is 0 in fp32: no infinity meets a 0 in t.
+#pragma once
+#include "qws_device.h"
+
+namespace qws {
+
+constexpr float LSE_DMIN = 150.0f;
+constexpr float LN2 = 0.69314718055994531f;
+constexpr float F32_MAX = 3.402823466e+38f;
+
+struct Lse {
+  float m, s, t;
+};
+
+__device__ __forceinline__ float lse_exp2(float d) { return __builtin_amdgcn_exp2f(d); }
+// NaN -> -inf (the median of three with a NaN is the smaller of the others), +inf -> the largest finite value.  The -inf
+// comes from a register that the compiler does not see through: it would fold the median into min(x, F32_MAX), whose
+// answer for NaN is F32_MAX.
+__device__ __forceinline__ float lse_clean(float x) {
+  float lowest;
+  asm("s_mov_b32 %0, 0xff800000" : "=s"(lowest));
+  return __builtin_amdgcn_fmed3f(x, lowest, F32_MAX);
+}
+__device__ __forceinline__ float lse_temp(float T) { return T > 0.0f ? T : 1.0f; }  // 0 (a greedy row) and NaN: as T = 1
+__device__ __forceinline__ float lse_scale(float T) { return fminf((float)LOG2E / lse_temp(T), F32_MAX); }
+__device__ __forceinline__ float lse_d(float x, float m, float c) { return fmaxf((x - m) * c, -LSE_DMIN); }  // NaN (-inf - -inf): -D_MIN
+
+__device__ __forceinline__ Lse lse_join(Lse a, Lse b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  const float da = lse_d(a.m, m, c), db = lse_d(b.m, m, c), ea = lse_exp2(da), eb = lse_exp2(db);
+  return {m, fmaf(ea, a.s, eb * b.s), fmaf(ea, fmaf(da, a.s, a.t), eb * fmaf(db, b.s, b.t))};
+}
+__device__ inline Lse lse_join_lanes(Lse v, float c, int from, int to) {  // butterfly over lane bits `from` .. `to` (powers of two)
+  for (int i = from; i <= to; i <<= 1) v = lse_join(v, {__shfl_xor(v.m, i), __shfl_xor(v.s, i), __shfl_xor(v.t, i)}, c);
+  return v;
+}
+__device__ __forceinline__ float lse_log(Lse v) { return logf(v.s); }
+// log p of a (clean) logit; -inf for a masked one and in a row without a candidate
+__device__ __forceinline__ float lse_logprob(Lse v, float x, float T) { return x == -INFINITY ? -INFINITY : (x - v.m) / lse_temp(T) - lse_log(v); }
+__device__ __forceinline__ float lse_entropy(Lse v) { return v.m == -INFINITY ? 0.0f : lse_log(v) - LN2 * (v.t / v.s); }
+
+}  // namespace qws

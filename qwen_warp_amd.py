@@ -9,3 +9,5 @@ from qwen_warp_amd.sampling import (TF_BROKEN, TF_RESCAN, TF_SPLIT_SELECT, TF_ST
 from qwen_warp_amd.pld import DevicePld  # noqa: E402,F401
 from qwen_warp_amd.finish import StepBook  # noqa: E402,F401
 from qwen_warp_amd.head import HeadSelect  # noqa: E402,F401
+from qwen_warp_amd.logprobs import LogProbs, LogProbsResult  # noqa: E402,F401
+from qwen_warp_amd.fp8 import Fp8Head  # noqa: E402,F401

@@ -1,0 +1,217 @@
+"""Fp8Head (qws_fp8_* through the Python wrapper) against the 64-bit definition (oracle/fp8.py, oracle/logprobs.py).
+
+The packed weights are read back exactly (products with unit vectors).  A logit is a sum of K exact products in fp32, in
+blocks of 128: it is within (128 + K / 128) 2^-23 of sum |qx qw| (a rounding, or a truncation, of each partial sum).  A
+logit's error moves ln sum e^z by as much at most, and a log probability or an entropy by the bounds of
+tests/test_gpu_logprobs.py beside it."""
+import numpy as np
+import pytest
+import torch
+
+import qwen_warp_amd as q
+from oracle import fp8 as F
+from oracle import logprobs as L
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+
+
+def data(T, N, K, seed, wdtype=torch.bfloat16):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(N, K, generator=g) * (0.01 + 0.05 * torch.rand(N, 1, generator=g))
+    x = torch.randn(T, K, generator=g) * (0.1 + 3 * torch.rand(T, 1, generator=g))
+    w[:, ::61] *= 5
+    x[:, ::37] *= 8
+    return w.to(wdtype), x.to(torch.bfloat16)
+
+
+def product(w, x):
+    """(logits, their bound) in 64 bits"""
+    a, b = F.values(x.double().numpy()), F.values(w.double().numpy())
+    return a @ b.T, (128 + x.shape[1] / 128) * 2.0 ** -23 * (np.abs(a) @ np.abs(b).T)
+
+
+@pytest.mark.parametrize("wdtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,K", [(1, 1), (5, 127), (16, 128), (300, 129), (257, 300), (64, 640)])
+def test_weights_read_back(N, K, wdtype):
+    w, _ = data(1, N, K, N + K, wdtype)
+    w[0] = 0.0
+    w[-1, 0] = 2.0 ** -100
+    eye = torch.eye(K, dtype=torch.bfloat16, device="cuda")
+    for pad in (0, 1):
+        v = torch.zeros(N, K + pad, dtype=wdtype, device="cuda")[:, :K]
+        v.copy_(w)
+        got = q.Fp8Head(v)(eye).t().double().cpu().numpy()
+        assert (got == F.values(w.double().numpy())).all()
+
+
+def test_scales_at_their_ends():
+    """Blocks whose largest value is just at, below and above a scale's range; powers over the whole exponent range."""
+    K = 128
+    p = 2.0 ** torch.arange(-60, 60, dtype=torch.float64)
+    w = torch.zeros(360, K, dtype=torch.float64)
+    w[:120, 5], w[120:240, 5], w[240:, 5] = 1.75 * p, 1.75 * p * (1 + 2.0 ** -20), p
+    w[:, 6] = w[:, 5] / 3
+    w = w.float()
+    eye = torch.eye(K, dtype=torch.bfloat16, device="cuda")
+    got = q.Fp8Head(w.cuda())(eye).t().double().cpu().numpy()
+    assert (got == F.values(w.double().numpy())).all()
+
+
+@pytest.mark.parametrize("T,N,K", [(1, 1, 1), (1, 1000, 100), (2, 15, 128), (3, 8191, 1000), (7, 129, 5120), (16, 4096, 640), (17, 1000, 257), (33, 700, 512),
+                                   (64, 513, 385), (65, 300, 1024), (100, 2001, 130), (128, 256, 128), (129, 255, 2000), (200, 1300, 768), (257, 257, 384), (600, 900, 640)])
+def test_logits(T, N, K):
+    w, x = data(T, N, K, T + N + K)
+    want, tol = product(w, x)
+    head = q.Fp8Head(w.cuda())
+    for pad in (0, 3):
+        y = torch.full((T, K + pad), float("nan"), dtype=torch.bfloat16, device="cuda")[:, :K]
+        y.copy_(x)
+        got = head(y)
+        assert got.shape == (T, N) and got.dtype == torch.float32
+        err = np.abs(got.double().cpu().numpy() - want)
+        assert (err <= tol).all(), f"off by {(err / tol).max()} of the bound"
+        half = head(y, dtype=torch.bfloat16)
+        assert torch.equal(half.view(torch.int16), got.to(torch.bfloat16).view(torch.int16))
+        # into a wider buffer, at any alignment; nothing around it is touched
+        for dtype in (torch.float32, torch.bfloat16):
+            buf = torch.full((T, N + 9), 7.0, dtype=dtype, device="cuda")
+            head(y, out=buf[:, 5:5 + N])
+            assert torch.equal(buf[:, 5:5 + N], got.to(dtype)) and (buf[:, :5] == 7).all() and (buf[:, 5 + N:] == 7).all()
+
+
+def test_rows_do_not_depend_on_the_batch():
+    """A hidden state's logits in batches of other sizes stay within the bound; the same call gives the same bits."""
+    w, x = data(300, 3000, 1280, 5)
+    head = q.Fp8Head(w.cuda())
+    want, tol = product(w, x)
+    x = x.cuda()
+    for T in (1, 15, 31, 64, 96, 150, 300):
+        got = head(x[:T])
+        assert (np.abs(got.double().cpu().numpy() - want[:T]) <= tol[:T]).all(), T
+        assert torch.equal(got, head(x[:T]))
+
+
+def test_special_values():
+    """Zeros give zeros; a row with NaN or an infinity is NaN, the others are not touched by it."""
+    w, x = data(20, 500, 300, 6)
+    want, tol = product(w, x)
+    x[3] = 0
+    x[5, 17], x[6, 299], x[7, 0] = float("nan"), INF, -INF
+    wn = w.clone()
+    wn[11, 4], wn[12, 299] = INF, float("nan")
+    got = q.Fp8Head(wn.cuda())(x.cuda()).double().cpu().numpy()
+    nan = np.zeros((20, 500), bool)
+    nan[5:8] = True
+    nan[:, 11:13] = True
+    want[3] = 0
+    assert (np.isnan(got) == nan).all()
+    assert (np.abs(got - want)[~nan] <= tol[~nan]).all()
+    lp, h = q.Fp8Head(wn.cuda()).score(x.cuda(), torch.full((20,), 12, dtype=torch.int32, device="cuda"))
+    assert (lp == -INF).all() and (h[5:8] == 0).all() and torch.isfinite(h).all()  # NaN logits count as -inf
+
+
+@pytest.mark.parametrize("T,N,K", [(1, 1, 1), (1, 5000, 256), (5, 129, 128), (16, 8191, 640), (17, 500, 130), (77, 3001, 384), (130, 1000, 512), (300, 257, 100), (520, 1025, 256)])
+@pytest.mark.parametrize("temperature", [False, True])
+def test_score(T, N, K, temperature):
+    w, x = data(T, N, K, T * N + K)
+    y, tol = product(w, x)
+    g = torch.Generator().manual_seed(T)
+    tokens = torch.randint(0, N, (T,), generator=g).to(torch.int32)
+    t = 0.3 + 2 * torch.rand(T, generator=g) if temperature else None
+    if T > 4:
+        tokens[2], tokens[3] = -1, N
+        if temperature:
+            t[1] = 0.0
+    head = q.Fp8Head(w.cuda())
+    lp, h = head.score(x.cuda(), tokens.cuda(), temperature=t.cuda() if temperature else None)
+    lp, h = lp.double().cpu().numpy(), h.double().cpu().numpy()
+    for r in range(T):
+        temp = 1.0 if t is None or t[r] == 0 else float(t[r])
+        want, _, wh, _, _ = L.row(y[r], [int(tokens[r])], 0, temp)
+        off = tol[r].max() / temp
+        sums = (256 + 30) * 2.0 ** -24
+        assert abs(lp[r] - want[0]) <= 2 * off + sums + 8 * abs(want[0]) * 2.0 ** -24, f"row {r}: {lp[r]} {want[0]}"
+        # dH = -cov(z, log p): a change of off in z moves H by at most off * sd(log p), sd <= ln N + 1 + |mean|
+        assert abs(h[r] - wh) <= off * (2 * np.log(N) + 2) + sums * (1 + 2 * wh), f"row {r}: entropy {h[r]} {wh}"
+    again = head.score(x.cuda(), tokens.cuda(), temperature=t.cuda() if temperature else None)
+    assert (again[0].double().cpu().numpy() == lp).all() and (again[1].double().cpu().numpy() == h).all()
+
+
+def test_score_agrees_with_the_logits():
+    """score() against LogProbs over the same head's logits, through the package."""
+    w, x = data(90, 6000, 512, 9)
+    head = q.Fp8Head(w.cuda())
+    tokens = torch.randint(0, 6000, (90,), generator=torch.Generator().manual_seed(1)).to(torch.int32).cuda()
+    lp, h = head.score(x.cuda(), tokens)
+    want = q.LogProbs("cuda")(head(x.cuda()), tokens)
+    assert torch.allclose(lp, want.logprobs, atol=5e-5, rtol=1e-5) and torch.allclose(h, want.entropy, atol=5e-5, rtol=1e-5)
+
+
+def test_no_rows_streams_and_graph():
+    w, x = data(40, 2000, 256, 10)
+    head = q.Fp8Head(w.cuda())
+    x = x.cuda()
+    assert head(x[:0]).shape == (0, 2000) and head.score(x[:0], torch.empty(0, dtype=torch.int32, device="cuda"))[0].shape == (0,)
+    first = head(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        head(x[:7])
+        with torch.cuda.stream(side):
+            other = head(x)
+        side.synchronize()
+        assert torch.equal(first, other)
+    buf, tokens = x.clone(), torch.arange(40, dtype=torch.int32, device="cuda")
+    for n in (1, 40):
+        head(buf[:n]), head.score(buf[:n], tokens[:n])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y, (lp, h) = head(buf[:n]), head.score(buf[:n], tokens[:n])
+        for i in range(4):
+            buf.copy_(data(40, 1, 256, 50 + i)[1])
+            want = [head(buf[:n]).clone(), *(t.clone() for t in head.score(buf[:n], tokens[:n]))]
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip((y, lp, h), want)), f"replay {i}"
+
+
+def test_offsets_past_32_bits():
+    """Hidden states and logits whose rows lie 2^31 + 8 elements apart."""
+    w, x = data(2, 700, 200, 11)
+    stride = (1 << 31) + 8
+    xs = torch.zeros(stride + 700, dtype=torch.bfloat16, device="cuda")
+    far = xs.as_strided((2, 200), (stride, 1))
+    far.copy_(x)
+    head = q.Fp8Head(w.cuda())
+    want = head(x.cuda(), dtype=torch.bfloat16)
+    assert torch.equal(head(far, dtype=torch.bfloat16), want)
+    out = xs.as_strided((2, 700), (stride, 1))
+    xin = x.cuda()
+    head(xin, out=out)
+    assert torch.equal(out, want)
+
+
+def test_behind_the_candidate_select():
+    """The head's logits refined by HeadSelect: the argmax is the bf16 head's."""
+    w, x = data(8, 4096, 512, 12)
+    x[:] = (x.float() + 60 * w[torch.arange(8) * 500].float()).to(torch.bfloat16)
+    head, select = q.Fp8Head(w.cuda()), q.HeadSelect("cuda")
+    tok, val, _, _ = select(head(x.cuda()), w.cuda(), x.cuda(), 32)
+    exact = x.double() @ w.double().t()
+    assert tok.tolist() == exact.argmax(1).tolist()
+
+
+def test_refusals():
+    w, x = data(4, 100, 64, 13)
+    w, x = w.cuda(), x.cuda()
+    head = q.Fp8Head(w)
+    i32 = torch.zeros(4, dtype=torch.int32, device="cuda")
+    for call in (lambda: q.Fp8Head(w.half()), lambda: q.Fp8Head(w.t()), lambda: q.Fp8Head(w[0]), lambda: q.Fp8Head(w[:0]), lambda: head(x.float()), lambda: head(x[:, :63]),
+                 lambda: head(x.cpu()), lambda: head(x[0]), lambda: head(x, dtype=torch.float16), lambda: head(x, out=torch.zeros(4, 99, device="cuda")),
+                 lambda: head(x, out=torch.zeros(1, 100, device="cuda").expand(4, 100)), lambda: head.score(x, i32[:3]), lambda: head.score(x, i32.long()),
+                 lambda: head.score(x, i32, temperature=torch.ones(4))):
+        with pytest.raises(q.ValidationError):
+            call()

@@ -1,0 +1,256 @@
+"""LogProbs (qws_logprobs through the Python wrapper) against the 64-bit definition (oracle/logprobs.py): ranks and
+alternatives bit-exact, log probabilities and entropies within the bound of their fp32 sums.
+
+The bound, in units of u = 2^-24.  A lane adds a chain of elements, parts are joined over 6 lane levels, the waves and the
+row's workgroups (at most 9 levels of ours, 3 roundings each), every weight 2^d has the error of its exponential (2 u) and of
+d (2 u |d| ln 2, and 2^d |d| ln 2 < 1 / e): under (chain + 64) u relative in s, and as much again in t.  So ln s is off by
+(chain + 66) u + u ln s, a log probability by that and 4 u |log p|, the entropy by (chain + 66) (1 + 2 H) u + 4 u H."""
+import numpy as np
+import pytest
+import torch
+
+import qwen_warp_amd as q
+from oracle import logprobs as L
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+INF = float("inf")
+
+
+def chain(R, V):
+    return 64 + (R * V) // (2048 * 256) * 2
+
+
+def layout(x, pad=0, offset=0):
+    """x [R, V] on the GPU in rows of V + pad elements that start `offset` elements behind an aligned address; NaN around."""
+    R, V = x.shape
+    buf = torch.full((R * (V + pad) + offset + 16,), float("nan"), dtype=x.dtype, device="cuda")
+    y = buf[offset:offset + R * (V + pad)].view(R, V + pad)[:, :V]
+    y.copy_(x)
+    return y
+
+
+def compare(x, tokens, top, temperature, out, label):
+    """x [R, V] as the kernel reads it, tokens [R, M]; out: a result with those shapes."""
+    R, V = x.shape
+    xs = x.double().cpu().numpy()
+    n = chain(R, V) + 66
+    for r in range(R):
+        lp, rank, h, ids, tlp = L.row(xs[r], tokens[r].tolist(), top, 1.0 if temperature is None else float(temperature[r]))
+        at = f"{label} row {r}"
+        assert out.ranks[r].tolist() == rank.tolist(), at
+        assert out.top_ids[r].tolist() == ids.tolist(), at
+        ln_s = 30.0
+        for got, want, what in ((out.logprobs[r], lp, "log p"), (out.top_logprobs[r], tlp, "alternatives")):
+            got = got.double().cpu().numpy()
+            with np.errstate(over="ignore"):
+                want = want.astype(np.float32).astype(np.float64)
+            fine = np.isfinite(want)
+            assert (got[~fine] == want[~fine]).all(), f"{at}: {what}"
+            assert (np.abs(got - want)[fine] <= (n + ln_s + 6 * np.abs(want[fine])) * U).all(), f"{at}: {what} off by {np.abs(got - want)[fine].max()}"
+        assert abs(float(out.entropy[r]) - h) <= (n * (1 + 2 * h) + 6 * h) * U, f"{at}: entropy {float(out.entropy[r])} {h}"
+
+
+def check(x, tokens, top=0, temperature=None, label="", pad=0, offset=0):
+    y = layout(x.cuda(), pad, offset)
+    out = q.LogProbs("cuda")(y, tokens.cuda(), top=top, temperature=temperature.cuda() if temperature is not None else None)
+    torch.cuda.synchronize()
+    compare(x, tokens.view(x.shape[0], -1), top, temperature, out._replace(logprobs=out.logprobs.view(x.shape[0], -1), ranks=out.ranks.view(x.shape[0], -1)), label)
+    return out
+
+
+def rows(R, V, dtype, seed, scale=3.0):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(R, V, generator=g) * scale).to(dtype)
+    return x, g
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,V,pad,offset", [(1, 1, 0, 0), (3, 2, 0, 1), (2, 63, 1, 0), (2, 64, 0, 3), (5, 65, 6, 5), (1, 1023, 0, 7), (3, 2049, 2, 1), (2, 8192, 0, 0),
+                                            (4, 12345, 3, 2), (1, 70001, 0, 1)])
+def test_shapes(dtype, R, V, pad, offset):
+    x, g = rows(R, V, dtype, R * V + pad)
+    for M, top in ((1, 0), (1, 1), (3, 5), (64, 64)):
+        tokens = torch.randint(0, V, (R, M), generator=g).to(torch.int32)
+        check(x, tokens, top, None, f"M={M} top={top}", pad, offset)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_full_vocabulary(dtype):
+    x, g = rows(3, 248320, dtype, 7)
+    x[0, 1000:1032] += 12
+    tokens = torch.tensor([1005, 77, 248319], dtype=torch.int32)
+    check(x, tokens, 20, torch.tensor([0.3, 1.0, 2.5]), "full", 0, 0)
+    check(x, tokens, 64, None, "full, misaligned", 5, 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_rows(dtype):
+    """Rows enough that a workgroup takes several stripes of one (the parts of a row are then fewer and longer)."""
+    x, g = rows(700, 30011, dtype, 8)
+    tokens = torch.randint(-1, 30011, (700, 2), generator=g).to(torch.int32)
+    check(x, tokens, 6, None, "many rows", 1, 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_orders(dtype):
+    """Ascending, descending, flat and blockwise rows: the alternatives are exact whatever the order in memory."""
+    V = 9001
+    up = torch.arange(V, dtype=torch.float32) / 16
+    block = torch.zeros(V)
+    block[64 * 5:64 * 6] = 3.0  # one group holds every alternative
+    stride = torch.zeros(V)
+    stride[::64] = 5.0  # every group has the same maximum
+    x = torch.stack([up, up.flip(0), torch.zeros(V), block, stride, torch.full((V,), -7.5)]).to(dtype)
+    tokens = torch.tensor([[0, V - 1, 320, 4000]] * 6, dtype=torch.int32)
+    for top in (1, 20, 64):
+        check(x, tokens, top, None, f"orders top={top}", 3, 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [None, 0.4, 1.7])
+def test_masks(dtype, temperature):
+    """Rows of nothing, of one token, with NaN, infinities and the type's lowest value, alone and mixed."""
+    V = 5003
+    low, nan = torch.finfo(dtype).min, float("nan")
+    x, g = rows(14, V, dtype, 9)
+    x[0] = -INF
+    x[1] = nan
+    x[2] = -INF
+    x[2, 4321] = -3.0
+    x[3] = low
+    x[4] = low
+    x[4, [7, 4000]] = 2.0
+    x[5, :] = -INF
+    x[5, ::1000] = low
+    x[6, ::2] = nan
+    x[7, 1::3] = -INF
+    x[8, 17] = INF
+    x[9, [3, 5000]] = INF
+    x[10] = -INF
+    x[10, :3] = torch.tensor([1.0, 3.0, 2.0])
+    x[11] = torch.finfo(dtype).max
+    x[12] = -INF
+    x[12, 9] = INF
+    x[13, 0], x[13, 1], x[13, 2:] = 0.0, -0.0, -1.0
+    tokens = torch.tensor([[0, 4321, 17, 3, 5000, 7, 1, -1, V, 2 ** 31 - 1]] * 14, dtype=torch.int32)
+    t = torch.full((14,), temperature) if temperature else None
+    for pad, offset in ((0, 0), (1, 3)):
+        check(x, tokens, 5, t, f"masks {pad}", pad, offset)
+        check(x, tokens[:, 0].contiguous(), 0, t, f"masks, one token {pad}", pad, offset)
+
+
+def test_temperatures():
+    """0 and NaN read as 1; tiny, huge and infinite ones give the limits (a point mass, a uniform row)."""
+    V = 3000
+    x, _ = rows(6, V, torch.float32, 10)
+    x[:, 11] = 40.0
+    t = torch.tensor([0.0, float("nan"), 1e-40, 1e-6, 1e30, INF])
+    tokens = torch.full((6,), 11, dtype=torch.int32)
+    out = q.LogProbs("cuda")(x.cuda(), tokens.cuda(), top=2, temperature=t.cuda())
+    one = q.LogProbs("cuda")(x.cuda(), tokens.cuda(), top=2)
+    assert torch.equal(out.logprobs[:2], one.logprobs[:2]) and torch.equal(out.entropy[:2], one.entropy[:2])
+    assert (out.logprobs[2:4] == 0).all() and (out.entropy[2:4] == 0).all()
+    assert torch.allclose(out.logprobs[4:].cpu(), torch.full((2,), -np.log(V), dtype=torch.float32), atol=1e-4)
+    assert torch.allclose(out.entropy[4:].cpu(), torch.full((2,), np.log(V), dtype=torch.float32), atol=1e-4)
+    assert torch.equal(out.top_ids, one.top_ids) and torch.equal(out.ranks, one.ranks)
+
+
+def test_large_logits_and_values():
+    """Logits of 1e4 and 1e30: differences to the maximum are taken first."""
+    for scale in (1e4, 1e30):
+        x, g = rows(3, 4097, torch.float32, 11)
+        x = x * scale
+        x[1, 5] = x[1].max()
+        check(x, torch.tensor([[5, 9], [5, 9], [5, 9]], dtype=torch.int32), 4, None, f"scale {scale}")
+
+
+def test_leading_dimensions_strides_and_outputs():
+    """[B, K + 1, V] logits with a verify call's tokens; rows shared by a stride of 0; nothing but the entropy."""
+    x, g = rows(12, 777, torch.float32, 12)
+    tokens = torch.randint(0, 777, (4, 3), generator=g).to(torch.int32)
+    tokens[1, 2] = -1
+    op = q.LogProbs("cuda")
+    out = op(x.view(4, 3, 777).cuda(), tokens.cuda(), top=3)
+    assert out.logprobs.shape == (4, 3) and out.ranks.shape == (4, 3) and out.entropy.shape == (4, 3) and out.top_ids.shape == (4, 3, 3)
+    flat = op(x.cuda(), tokens.view(12).cuda(), top=3)
+    assert all(torch.equal(a.flatten(), b.flatten()) for a, b in zip(out, flat))
+    assert out.logprobs[1, 2] == 0 and out.ranks[1, 2] == -1
+    labels = op(x.view(4, 3, 777).cuda(), tokens.view(4, 3, 1).expand(4, 3, 5).contiguous().cuda())
+    assert labels.logprobs.shape == (4, 3, 5) and torch.equal(labels.logprobs[..., 4], out.logprobs) and torch.equal(labels.ranks[..., 2], out.ranks)
+    shared = op(x[:1].cuda().expand(6, 777), torch.arange(6, dtype=torch.int32, device="cuda"), top=2)
+    assert (shared.entropy == shared.entropy[0]).all() and shared.ranks.unique().numel() == 6
+    bare = op(x.cuda())
+    assert bare.logprobs is None and bare.ranks is None and torch.equal(bare.entropy.view(4, 3), out.entropy) and bare.top_ids.shape == (12, 0)
+    no_ranks = op(x.cuda(), tokens.view(12).cuda(), ranks=False)
+    assert no_ranks.ranks is None and torch.equal(no_ranks.logprobs.view(4, 3), out.logprobs)
+    empty = op(torch.empty(0, 777, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda"), top=3)
+    assert empty.logprobs.shape == (0,) and empty.top_ids.shape == (0, 3)
+
+
+def test_widest_vocabulary():
+    V = 1 << 19
+    for dtype in (torch.float32, torch.bfloat16):
+        x, g = rows(2, V, dtype, 13)
+        check(x, torch.tensor([[V - 1], [0]], dtype=torch.int32), 64, None, "widest", 1, 1)
+    with pytest.raises(RuntimeError):
+        q.LogProbs("cuda")(torch.zeros(1, V + 1, device="cuda"))
+
+
+def test_offsets_past_32_bits():
+    """Rows 2^31 + 8 elements apart."""
+    stride, V = (1 << 31) + 8, 5000
+    buf = torch.zeros(stride + V, dtype=torch.bfloat16, device="cuda")
+    x, _ = rows(2, V, torch.bfloat16, 14)
+    y = buf.as_strided((2, V), (stride, 1))
+    y.copy_(x)
+    tokens = torch.tensor([[3], [4999]], dtype=torch.int32)
+    out = q.LogProbs("cuda")(y, tokens.cuda(), top=8)
+    compare(x, tokens, 8, None, out, "far rows")
+
+
+def test_streams_and_repeats():
+    """The same bits on every run and on another stream, also with calls of other shapes in between."""
+    x, g = rows(40, 20000, torch.float32, 15)
+    x, tokens = x.cuda(), torch.randint(0, 20000, (40,), generator=g).to(torch.int32).cuda()
+    op = q.LogProbs("cuda")
+    first = op(x, tokens, top=20)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for i in range(5):
+        op(x[: 1 + i], tokens[: 1 + i], top=1)
+        with torch.cuda.stream(side):
+            other = op(x, tokens, top=20)
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(first, other))
+        assert all(torch.equal(a, b) for a, b in zip(first, op(x, tokens, top=20)))
+
+
+def test_graph():
+    """A captured call, replayed with new logits in place and eager work in between."""
+    x, g = rows(8, 30000, torch.bfloat16, 16)
+    buf, tokens = x.cuda(), torch.randint(0, 30000, (8,), generator=g).to(torch.int32).cuda()
+    op = q.LogProbs("cuda")
+    op(buf, tokens, top=5)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = op(buf, tokens, top=5)
+    for i in range(4):
+        buf.copy_(rows(8, 30000, torch.bfloat16, 100 + i)[0])
+        want = [t.clone() for t in op(buf, tokens, top=5)]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), f"replay {i}"
+
+
+def test_refusals():
+    op = q.LogProbs("cuda")
+    x = torch.zeros(4, 100, device="cuda")
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    for call in (lambda: op(x.half()), lambda: op(x.t()), lambda: op(x[0]), lambda: op(x, i32(3)), lambda: op(x, i32(4).long()), lambda: op(x, i32(4).cpu()),
+                 lambda: op(x, i32(4, 65)), lambda: op(x, i32(4, 0)), lambda: op(x, i32(8)[::2]), lambda: op(x, top=65), lambda: op(x, top=-1),
+                 lambda: op(x, temperature=torch.ones(3, device="cuda")), lambda: op(x, temperature=torch.ones(4)), lambda: op(x.double())):
+        with pytest.raises(q.ValidationError):
+            call()
