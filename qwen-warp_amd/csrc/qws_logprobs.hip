@@ -11,20 +11,27 @@
 //               pass over the logits does nothing more for 64 alternatives than for none, whatever their order in memory.
 #include "qws_lse.h"
 
+#include <type_traits>
+
 namespace qws {
 
 constexpr int LP_NT = 256;      // threads
 constexpr int LP_NW = LP_NT / 64;
 constexpr int LP_GRP = 64;      // consecutive logits of a group
 constexpr int LP_NMAX = 64;     // alternatives and given tokens of a row at most
-constexpr int LP_U = 4;         // 16-byte vectors of a thread in flight together
 constexpr int LP_VMAX = 1 << 19;
-constexpr int LP_WGS = 2048;    // workgroups that fill the card: 8 of 256 threads on each of 256 CUs
+constexpr int LP_CUS = 256;
+constexpr int LP_U = 4;         // vectors of a thread loaded together, where it has more than one
 
 template <typename T>
 constexpr int lp_e() { return 16 / (int)sizeof(T); }  // elements of a vector
 template <typename T>
+constexpr int lp_waves(int u) { return u * lp_e<T>() > 16 ? 5 : 8; }  // waves of a SIMD that the block's registers allow
+template <typename T>
 constexpr int lp_stripe() { return LP_NT * lp_e<T>(); }  // elements that a workgroup's threads load at once
+
+template <typename T>
+using lp_bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
 
 struct LpArgs {
   const void* x;
@@ -51,29 +58,127 @@ __device__ __forceinline__ float lp_one(const T* p) {
   else
     return lse_clean(__uint_as_float((uint32_t)*gmem((const uint16_t*)p) << 16));
 }
-// the vector at virtual position v (elements [lead, end) of `base` exist; base is 16-byte aligned)
 template <typename T>
 __device__ __forceinline__ void lp_unpack(vu4 r, float* x) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) x[j] = lse_clean(__uint_as_float(r[j]));
+    for (int j = 0; j < 4; j++) x[j] = __uint_as_float(r[j]);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      x[2 * j] = lse_clean(__uint_as_float(r[j] << 16));
-      x[2 * j + 1] = lse_clean(__uint_as_float(r[j] & 0xFFFF0000u));
+      x[2 * j] = __uint_as_float(r[j] << 16);
+      x[2 * j + 1] = __uint_as_float(r[j] & 0xFFFF0000u);
     }
   }
 }
+// the vector at position v of `base` (16-byte aligned), of which [lead, end) exist: the rest reads -inf
 template <typename T>
-__device__ inline void lp_load_edge(const T* base, int v, int lead, int end, float* x) {
+__device__ __forceinline__ vu4 lp_load_edge(const T* base, int v, int lead, int end) {
+  constexpr int E = lp_e<T>();
+  vu4 r;
+  if (v >= lead && v + E <= end) {
+    r = *gmem((const vu4*)(base + v));
+  } else {
+    uint32_t y[E];
 #pragma unroll
-  for (int j = 0; j < lp_e<T>(); j++) x[j] = v + j >= lead && v + j < end ? lp_one(base + v + j) : -INFINITY;
+    for (int j = 0; j < E; j++) y[j] = *gmem((const lp_bits<T>*)base + min(max(v + j, lead), end - 1));
+#pragma unroll
+    for (int j = 0; j < E; j++)
+      if (v + j < lead || v + j >= end) y[j] = 0xFF800000u >> (sizeof(T) == 4 ? 0 : 16);
+#pragma unroll
+    for (int j = 0; j < 4; j++) r[j] = sizeof(T) == 4 ? y[j] : y[j * (E / 4)] | y[(j * (E / 4) + 1) % E] << 16;
+  }
+  return r;
 }
 
-// RANK: 0 no given tokens' ranks, 1 one token per row (held in registers), 2 several (in LDS)
-template <typename T, int RANK, bool TOP>
-__global__ void __launch_bounds__(LP_NT, 8) k_lp_scan(LpArgs a) {
+// The largest of the block's values; a NaN shows in the sums (lp_fast), not here.  One instruction for two values, where
+// fmaxf on loaded values also has to quiet them.
+__device__ __forceinline__ float lp_max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+template <int E>
+__device__ __forceinline__ float lp_max(const float* x) {
+  float m = lp_max3(x[0], x[1], x[2]);
+#pragma unroll
+  for (int j = 3; j + 1 < E; j += 2) m = lp_max3(m, x[j], x[j + 1]);
+  return lp_max3(m, x[E - 1], x[E - 1]);
+}
+
+// The largest of each group's lanes (8 or 16), in every lane: one instruction a step, where fmaxf of a moved value takes four.
+// A lane's value is written at least two instructions before another lane's step reads it (the hardware does not wait).
+template <int U, int E>
+__device__ __forceinline__ void lp_group_max(float (&m)[U]) {
+#define QWS_DPP(n, ctrl) "v_max_f32_dpp %" #n ", %" #n ", %" #n " " ctrl " row_mask:0xf bank_mask:0xf\n\t"
+#define QWS_STEP(ctrl)                                                                                                                \
+  if constexpr (U == 4)                                                                                                               \
+    asm("s_nop 1\n\t" QWS_DPP(0, ctrl) QWS_DPP(1, ctrl) QWS_DPP(2, ctrl) QWS_DPP(3, ctrl) : "+v"(m[0]), "+v"(m[U / 4]), "+v"(m[U / 2]), "+v"(m[U - 1])); \
+  else                                                                                                                                \
+    asm("s_nop 1\n\t" QWS_DPP(0, ctrl) : "+v"(m[0]))
+  static_assert(U == 1 || U == 4, "vectors of a block");
+  QWS_STEP("quad_perm:[1,0,3,2]");
+  QWS_STEP("quad_perm:[2,3,0,1]");
+  QWS_STEP("row_half_mirror");
+  if constexpr (E == 4) { QWS_STEP("row_mirror"); }
+#undef QWS_STEP
+#undef QWS_DPP
+}
+
+// A lane's sums over blocks of logits of moderate size (below LP_MOST in magnitude at their largest, no -inf, no NaN),
+// relative to any reference M = fl(c m) within LP_SLACK of the largest, so that M rarely moves: a multiply-add, an
+// exponential and two sums per logit.  Blocks with anything else go to Lse's general form (lp_slow).
+constexpr float LP_MOST = 0x1p60f;  // and c <= 2^60: products stay finite
+constexpr float LP_SLACK = 8.0f;    // in log2 units: d <= 8, so the entropy's two terms cancel by 8 units at most
+struct LpFast {
+  float m, M, limit, s, t;
+};
+template <int U, int E>
+__device__ __forceinline__ bool lp_fast(LpFast& f, const float (&x)[U][E], float best, float c) {
+  if (__any(best > f.limit)) {
+    if (best > f.limit) {
+      const float M = c * best, d = f.M - M, e = lse_exp2(d);
+      f = {best, M, best + LP_SLACK / c, f.s * e, e * fmaf(d, f.s, f.t)};
+    }
+  }
+  float s = f.s, t = f.t;
+#pragma unroll
+  for (int u = 0; u < U; u++)
+#pragma unroll
+    for (int j = 0; j < E; j++) {
+      const float d = fmaf(x[u][j], c, -f.M), e = lse_exp2(d);
+      s += e;
+      t = fmaf(e, d, t);
+    }
+  if (__any(!(fabsf(t) < INFINITY))) return false;  // -inf or NaN among them
+  f.s = s;
+  f.t = t;
+  return true;
+}
+// the fast sums relative to c m: r = c m - M is what rounding M took
+__device__ __forceinline__ Lse lp_fast_end(const LpFast& f, float c) {
+  if (f.m == -INFINITY) return {-INFINITY, 0.0f, 0.0f};
+  const float r = fmaf(c, f.m, -f.M), e = lse_exp2(-r);
+  return {f.m, f.s * e, e * fmaf(-r, f.s, f.t)};
+}
+template <int U, int E>
+__device__ __forceinline__ void lp_slow(Lse& v, const float (&x)[U][E], float best, float c) {
+  const float m = fmaxf(v.m, best), d = lse_d(v.m, m, c), e = lse_exp2(d);
+  v = {m, v.s * e, e * fmaf(d, v.s, v.t)};
+#pragma unroll
+  for (int u = 0; u < U; u++)
+#pragma unroll
+    for (int j = 0; j < E; j++) {
+      const float dj = lse_d(x[u][j], m, c), ej = lse_exp2(dj);
+      v.s += ej;
+      v.t = fmaf(ej, dj, v.t);
+    }
+}
+
+// RANK: 0 no given tokens' ranks, 1 one token per row (held in registers), 2 several (in LDS).  U vectors of a thread make a
+// block: loaded together, one step of the running maximum.
+template <typename T, int RANK, bool TOP, int U>
+__global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
   constexpr int E = lp_e<T>(), SE = lp_stripe<T>();
   __shared__ float s_xt[LP_NMAX];
   __shared__ int s_tv[LP_NMAX], s_cnt[LP_NMAX];
@@ -87,11 +192,13 @@ __global__ void __launch_bounds__(LP_NT, 8) k_lp_scan(LpArgs a) {
   const int nstripes = (end + SE - 1) / SE, s_end = min((ch + 1) * a.per, nstripes);
   float xt = 0.0f;
   int tv = -1, cnt = 0;  // virtual position of the token (-1: skipped), logits before it
+  bool moderate = c <= LP_MOST;  // no given token's logit is extreme
   if constexpr (RANK == 1) {
     const int t = a.tok[row];
     if (t >= 0 && t < a.V) {
       tv = t + lead;
       xt = lp_one(p + t);
+      moderate = moderate && fabsf(xt) < LP_MOST;
     }
   }
   if constexpr (RANK == 2) {
@@ -103,57 +210,59 @@ __global__ void __launch_bounds__(LP_NT, 8) k_lp_scan(LpArgs a) {
       s_cnt[tid] = 0;
     }
     bar();
+    for (int k = 0; k < a.M; k += 64) moderate = moderate && !__any(k + lane < a.M && !(fabsf(s_xt[min(k + lane, a.M - 1)]) < LP_MOST));
   }
   Lse v = {-INFINITY, 0.0f, 0.0f};
-  for (int s = ch * a.per; s < s_end; s += LP_U) {
-    float x[LP_U][E];
+  LpFast f = {-INFINITY, -1e30f, -INFINITY, 0.0f, 0.0f};
+  char* gmax = (char*)(a.gmax + (long long)row * a.groups);
+  for (int s = ch * a.per; s < s_end; s += U) {
+    float top[U];
+    vu4 r[U];
     const int first = s * SE;
-    if (first >= lead && first + LP_U * SE <= end && s + LP_U <= s_end) {
-      vu4 r[LP_U];
+    if (first >= lead && first + U * SE <= end && s + U <= s_end) {
 #pragma unroll
-      for (int u = 0; u < LP_U; u++) r[u] = *gmem((const vu4*)(base + first + u * SE + tid * E));
+      for (int u = 0; u < U; u++) r[u] = __builtin_nontemporal_load((const QWS_G vu4*)(base + first + u * SE + tid * E));  // read once
+    } else {  // past the row's end, or into the next workgroup's stripes: nothing
 #pragma unroll
-      for (int u = 0; u < LP_U; u++) lp_unpack<T>(r[u], x[u]);
-    } else {
-#pragma unroll
-      for (int u = 0; u < LP_U; u++) lp_load_edge(base, first + u * SE + tid * E, lead, s + u < s_end ? end : 0, x[u]);
+      for (int u = 0; u < U; u++) r[u] = lp_load_edge(base, first + u * SE + tid * E, s + u < s_end ? lead : end, end);
     }
-    float best = -INFINITY;
+    float x[U][E], best = -INFINITY, least = INFINITY;
 #pragma unroll
-    for (int u = 0; u < LP_U; u++) {
-      float m = x[u][0];
+    for (int u = 0; u < U; u++) {
+      lp_unpack<T>(r[u], x[u]);
+      top[u] = lp_max<E>(x[u]);
+      best = fmaxf(best, top[u]);
+      least = fminf(least, top[u]);
+    }
+    if (!(moderate && __all(best < LP_MOST && least > -LP_MOST)) || !lp_fast(f, x, best, c)) {
+      best = -INFINITY;
 #pragma unroll
-      for (int j = 1; j < E; j++) m = fmaxf(m, x[u][j]);
-      best = fmaxf(best, m);
-      if constexpr (TOP) {
-        constexpr int L = LP_GRP / E;  // lanes of a group: 8 or 16
-        m = fmaxf(m, dpp_perm<0xB1>(m));
-        m = fmaxf(m, dpp_perm<0x4E>(m));
-        m = fmaxf(m, dpp_perm<0x141>(m));
-        if constexpr (L == 16) m = fmaxf(m, dpp_perm<0x140>(m));
-        if ((lane & (L - 1)) == 0 && s + u < s_end) a.gmax[(long long)row * a.groups + (first + u * SE + tid * E) / LP_GRP] = m;
+      for (int u = 0; u < U; u++) {
+        top[u] = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+          x[u][j] = lse_clean(x[u][j]);
+          top[u] = fmaxf(top[u], x[u][j]);
+        }
+        best = fmaxf(best, top[u]);
       }
+      lp_slow(v, x, best, c);
     }
-    {  // the new maximum, then the elements
-      const float m = fmaxf(v.m, best), d = lse_d(v.m, m, c), e = lse_exp2(d);
-      v = {m, v.s * e, e * fmaf(d, v.s, v.t)};
+    if constexpr (TOP) {
+      lp_group_max<U, E>(top);
+#pragma unroll
+      for (int u = 0; u < U; u++)  // byte offsets in 32 bits: one address register for all
+        if ((lane & (LP_GRP / E - 1)) == 0 && s + u < s_end) *(float*)(gmax + (unsigned)((first + u * SE + tid * E) / LP_GRP * 4)) = top[u];
     }
-#pragma unroll
-    for (int u = 0; u < LP_U; u++)
-#pragma unroll
-      for (int j = 0; j < E; j++) {
-        const float d = lse_d(x[u][j], v.m, c), e = lse_exp2(d);
-        v.s += e;
-        v.t = fmaf(e, d, v.t);
-      }
     if constexpr (RANK != 0) {
       const int n = RANK == 1 ? 1 : a.M;
       for (int k = 0; k < n; k++) {
         const float xk = RANK == 1 ? xt : s_xt[k];
         const int tk = RANK == 1 ? tv : s_tv[k];
         int add = 0;
+        if (!__any(best >= xk)) continue;  // a likely token: nothing here is before it
 #pragma unroll
-        for (int u = 0; u < LP_U; u++) {
+        for (int u = 0; u < U; u++) {
           // this wave's elements: [lo, lo + 64 E); a stripe of the next workgroup lies behind every token
           const int lo = s + u < s_end ? first + u * SE + wave * 64 * E : 0x7FFFFFFF - 64 * E;
           if (lo + 64 * E <= tk) {
@@ -174,7 +283,7 @@ __global__ void __launch_bounds__(LP_NT, 8) k_lp_scan(LpArgs a) {
       }
     }
   }
-  v = lse_join_lanes(v, c, 1, 32);
+  v = lse_join_lanes(lse_join(v, lp_fast_end(f, c), c), c, 1, 32);
   if constexpr (RANK == 1) {
     if (tid == 0) s_cnt[0] = 0;
     bar();
@@ -221,27 +330,47 @@ __device__ inline uint64_t lp_threshold(uint64_t mine, int n, LpSel& s) {
 __device__ __forceinline__ void lp_take(uint64_t k, uint64_t thr, LpSel& s, uint64_t* list) {
   if (k && k >= thr) list[atomicAdd(&s.n, 1)] = k;
 }
-// calls put(rank, key) for every key of the list that is among its n best
+// calls put(rank, key) for every key of the list that is among its n best (after a barrier behind lp_take)
 template <typename F>
-__device__ __forceinline__ void lp_ranked(const LpSel& s, const uint64_t* list, int n, F put) {
-  const int c = s.n;
+__device__ __forceinline__ void lp_ranked(LpSel& s, const uint64_t* list, int n, F put) {
+  const int c = s.n, lane = lane_id(), wave = wave_id();
+  if (c <= 64) {  // each wave compares the lanes' keys with a quarter of the list
+    if (wave == 0) s.rank[lane] = 0;
+    bar();
+    const uint64_t k = lane < c ? list[lane] : 0;
+    const int q = (c + LP_NW - 1) / LP_NW, hi = min((wave + 1) * q, c);
+    int r = 0;
+#pragma unroll 4
+    for (int j = wave * q; j < hi; j++) r += list[j] > k;
+    atomicAdd(&s.rank[lane], r);
+    bar();
+    if (wave == 0 && lane < c && s.rank[lane] < n) put(s.rank[lane], k);
+    return;
+  }
   for (int i = threadIdx.x; i < c; i += LP_NT) {
     const uint64_t k = list[i];
     int r = 0;
+#pragma unroll 4
     for (int j = 0; j < c; j++) r += list[j] > k;
     if (r < n) put(r, k);
   }
 }
 
-template <typename T>
+// KPT: groups of a thread at most (0: no alternatives), all loaded at once
+template <typename T, int KPT>
 __global__ void __launch_bounds__(LP_NT) k_lp_row(LpArgs a) {
   constexpr int E = lp_e<T>();
-  extern __shared__ uint64_t list[];  // as many keys as a selection can keep: max(groups, 64 top)
+  extern __shared__ uint64_t list[];  // lp_list(groups, top) keys
   __shared__ LpSel s;
   __shared__ Lse s_lse[LP_NW];
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), row = blockIdx.x;
   const T* p = (const T*)a.x + (long long)row * a.stride;
   const int lead = (int)((uintptr_t)p / sizeof(T)) & (E - 1), end = lead + a.V;
+  const int ng = (end + LP_GRP - 1) / LP_GRP;
+  const float* gm = a.gmax + (long long)row * a.groups;
+  float gv[KPT ? KPT : 1];
+#pragma unroll
+  for (int i = 0; i < KPT; i++) gv[i] = *gmem(gm + min(i * LP_NT + tid, ng - 1));
   const float temp = a.temp ? a.temp[row] : 1.0f, c = lse_scale(temp);
   Lse v = {-INFINITY, 0.0f, 0.0f};
   for (int g = tid; g < a.G; g += LP_NT) {
@@ -260,7 +389,7 @@ __global__ void __launch_bounds__(LP_NT) k_lp_row(LpArgs a) {
     const int t = a.tok[o];
     const bool ok = t >= 0 && t < a.V;
     const float x = ok ? lp_one(p + t) : 0.0f;
-    if (a.out_lp && lane == 0) a.out_lp[o] = ok ? lse_logprob(v, x, temp) : 0.0f;
+    if (lane == 0) a.out_lp[o] = ok ? lse_logprob(v, x, temp) : 0.0f;
     if (a.out_rank) {
       int n = 0;
       for (int g = lane; g < a.G; g += 64) n += a.cnt[((long long)row * a.G + g) * a.M + m];
@@ -269,67 +398,75 @@ __global__ void __launch_bounds__(LP_NT) k_lp_row(LpArgs a) {
       if (lane == 0) a.out_rank[o] = ok ? n : -1;
     }
   }
-  if (a.top == 0) return;
-  const float* gm = a.gmax + (long long)row * a.groups;
-  uint64_t best = 0;
-  for (int g = tid; g < a.groups; g += LP_NT) {
-    const float x = gm[g];
-    if (x > -INFINITY) best = max(best, comp(okey(x), (uint32_t)g));
-  }
-  uint64_t thr = lp_threshold(best, a.top, s);
-  for (int g = tid; g < a.groups; g += LP_NT) {
-    const float x = gm[g];
-    if (x > -INFINITY) lp_take(comp(okey(x), (uint32_t)g), thr, s, list);
-  }
-  bar();
-  lp_ranked(s, list, a.top, [&](int r, uint64_t k) { s.win[r] = (int)comp_idx(k); });
-  const int nw = min(s.n, a.top);
-  bar();
-  uint64_t key[LP_NMAX / LP_NW];
-  best = 0;
+  if constexpr (KPT != 0) {
+    auto group = [&](int i) {
+      const int g = i * LP_NT + tid;
+      return g < ng && gv[i] > -INFINITY ? comp(okey(gv[i]), (uint32_t)g) : 0;
+    };
+    uint64_t best = 0;
 #pragma unroll
-  for (int i = 0; i < LP_NMAX / LP_NW; i++) {
-    const int k = i * LP_NW + wave;
-    key[i] = 0;
-    if (k < nw) {
-      const int e = s.win[k] * LP_GRP + lane;
-      if (e >= lead && e < end) {
-        const float x = lp_one(p + (e - lead));
-        if (x > -INFINITY) key[i] = comp(okey(x), (uint32_t)(e - lead));
+    for (int i = 0; i < KPT; i++) best = max(best, group(i));
+    uint64_t thr = lp_threshold(best, a.top, s);
+#pragma unroll
+    for (int i = 0; i < KPT; i++) lp_take(group(i), thr, s, list);
+    bar();
+    lp_ranked(s, list, a.top, [&](int r, uint64_t k) { s.win[r] = (int)comp_idx(k); });
+    const int nw = min(s.n, a.top);
+    bar();
+    constexpr int PER = LP_NMAX / LP_NW;  // winning groups of a wave at most
+    float x[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+      if (i * LP_NW < nw) x[i] = lp_one(p + (min(max(s.win[min(i * LP_NW + wave, nw - 1)] * LP_GRP + lane, lead), end - 1) - lead));
+    uint64_t key[PER];
+    best = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int k = i * LP_NW + wave;
+      key[i] = 0;
+      if (k < nw) {
+        const int e = s.win[k] * LP_GRP + lane;
+        if (e >= lead && e < end && x[i] > -INFINITY) key[i] = comp(okey(x[i]), (uint32_t)(e - lead));
       }
+      best = max(best, key[i]);
     }
-    best = max(best, key[i]);
-  }
-  thr = lp_threshold(best, a.top, s);
+    thr = lp_threshold(best, a.top, s);
 #pragma unroll
-  for (int i = 0; i < LP_NMAX / LP_NW; i++) lp_take(key[i], thr, s, list);
-  bar();
-  int* ids = a.out_ids + (long long)row * a.top;
-  float* lps = a.out_top + (long long)row * a.top;
-  lp_ranked(s, list, a.top, [&](int r, uint64_t k) {
-    ids[r] = (int)comp_idx(k);
-    lps[r] = lse_logprob(v, okey_val(comp_key(k)), temp);
-  });
-  for (int r = s.n + tid; r < a.top; r += LP_NT) {
-    ids[r] = -1;
-    lps[r] = -INFINITY;
+    for (int i = 0; i < PER; i++) lp_take(key[i], thr, s, list);
+    bar();
+    int* ids = a.out_ids + (long long)row * a.top;
+    float* lps = a.out_top + (long long)row * a.top;
+    lp_ranked(s, list, a.top, [&](int r, uint64_t k) {
+      ids[r] = (int)comp_idx(k);
+      lps[r] = lse_logprob(v, okey_val(comp_key(k)), temp);
+    });
+    for (int r = s.n + tid; r < a.top; r += LP_NT) {
+      ids[r] = -1;
+      lps[r] = -INFINITY;
+    }
   }
+}
+// Keys that a selection of the n best can list: those of the n lanes whose best are the n largest
+inline size_t lp_list(int groups, int n) {
+  const int a = n * ((groups + 63) / 64) < groups ? n * ((groups + 63) / 64) : groups, b = n < 64 ? n * n : n * 64;
+  return (size_t)(a > b ? a : b);
 }
 
 struct LpPlan {
   int G, per, groups;
   size_t part, cnt, gmax, total;  // byte offsets
 };
-// Workgroups of a row: all of its stripes' while the card is not full, else as many as fill it (more would add parts to
-// join and no bandwidth).
+// Stripes of a workgroup: one while the card holds them all at once; then four (a block), eight, and as many as leave eight
+// rounds of workgroups, so that the last round is a small part (2,048 bf16 rows of 248,320: 257 us with one round of whole
+// rows, 229 with eight; 256 fp32 rows: 60 and 57; 36 rows, one stripe each: 35, eight: 25).
 template <typename T>
 LpPlan lp_plan(int R, int V, int M, int top) {
   LpPlan q;
   const int stripes = (V + lp_e<T>() - 1 + lp_stripe<T>() - 1) / lp_stripe<T>();
-  const long long all = (long long)R * stripes;
-  q.per = (int)((all + LP_WGS - 1) / LP_WGS);
-  if (q.per > stripes) q.per = stripes;
-  if (q.per > LP_U) q.per = (q.per + LP_U - 1) / LP_U * LP_U;
+  const long long all = (long long)R * stripes, fill = LP_CUS * lp_waves<T>(LP_U);  // fill: workgroups of four waves held at once
+  const long long rounds = (all + 8 * fill - 1) / (8 * fill), few = (stripes + LP_U - 1) / LP_U * LP_U;
+  const long long per = all <= fill || stripes == 1 ? 1 : all <= 4 * fill ? LP_U : rounds <= 2 * LP_U ? 2 * LP_U : (rounds + LP_U - 1) / LP_U * LP_U;
+  q.per = (int)(per > few ? few : per);
   q.G = (stripes + q.per - 1) / q.per;
   q.groups = top ? stripes * (lp_stripe<T>() / LP_GRP) : 0;
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
@@ -340,12 +477,21 @@ LpPlan lp_plan(int R, int V, int M, int top) {
   return q;
 }
 
-template <typename T, int RANK>
+template <typename T, int RANK, bool TOP>
 void lp_launch_scan(const LpArgs& a, int R, hipStream_t st) {
-  if (a.top)
-    hipLaunchKernelGGL((k_lp_scan<T, RANK, true>), dim3((unsigned)R * a.G), dim3(LP_NT), 0, st, a);
+  if (a.per == 1)
+    hipLaunchKernelGGL((k_lp_scan<T, RANK, TOP, 1>), dim3((unsigned)R * a.G), dim3(LP_NT), 0, st, a);
   else
-    hipLaunchKernelGGL((k_lp_scan<T, RANK, false>), dim3((unsigned)R * a.G), dim3(LP_NT), 0, st, a);
+    hipLaunchKernelGGL((k_lp_scan<T, RANK, TOP, LP_U>), dim3((unsigned)R * a.G), dim3(LP_NT), 0, st, a);
+}
+template <typename T, bool TOP>
+void lp_launch_scan(const LpArgs& a, int R, hipStream_t st) {
+  if (!a.M || !a.out_rank)
+    lp_launch_scan<T, 0, TOP>(a, R, st);
+  else if (a.M == 1)
+    lp_launch_scan<T, 1, TOP>(a, R, st);
+  else
+    lp_launch_scan<T, 2, TOP>(a, R, st);
 }
 template <typename T>
 int lp_launch(LpArgs a, int R, char* ws, size_t ws_bytes, hipStream_t st) {
@@ -357,16 +503,19 @@ int lp_launch(LpArgs a, int R, char* ws, size_t ws_bytes, hipStream_t st) {
   a.part = (float4*)(ws + q.part);
   a.cnt = (int*)(ws + q.cnt);
   a.gmax = (float*)(ws + q.gmax);
-  if (!a.M || !a.out_rank)
-    lp_launch_scan<T, 0>(a, R, st);
-  else if (a.M == 1)
-    lp_launch_scan<T, 1>(a, R, st);
+  if (a.top)
+    lp_launch_scan<T, true>(a, R, st);
   else
-    lp_launch_scan<T, 2>(a, R, st);
+    lp_launch_scan<T, false>(a, R, st);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  const size_t lds = a.top ? sizeof(uint64_t) * (size_t)(q.groups > LP_GRP * a.top ? q.groups : LP_GRP * a.top) : 0;
-  hipLaunchKernelGGL((k_lp_row<T>), dim3(R), dim3(LP_NT), lds, st, a);
+  const size_t lds = a.top ? sizeof(uint64_t) * lp_list(q.groups, a.top) : 0;
+  if (!a.top)
+    hipLaunchKernelGGL((k_lp_row<T, 0>), dim3(R), dim3(LP_NT), 0, st, a);
+  else if (q.groups <= 16 * LP_NT)
+    hipLaunchKernelGGL((k_lp_row<T, 16>), dim3(R), dim3(LP_NT), lds, st, a);
+  else
+    hipLaunchKernelGGL((k_lp_row<T, 33>), dim3(R), dim3(LP_NT), lds, st, a);
   return (int)hipGetLastError();
 }
 
