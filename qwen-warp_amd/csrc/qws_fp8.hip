@@ -12,12 +12,14 @@
 //
 // Layout.  16 rows x 64 values are a fragment of 1 KB: lane l's 16 bytes are row l % 16, values 16 (l / 16) .. + 15, the
 // operands of two 16x16x32 products.  (Which 32 of the values share a product does not matter, as long as both operands
-// take the same.)  Every load of a wave is 1 KB of consecutive bytes, in memory and in LDS.  The fragments of a group of 16
-// rows lie along K; the exponents (biased by 127) of four consecutive blocks are the bytes of one word per row.  Rows and
-// values beyond N, T and K are 0.
+// take the same.)  Every load of a wave is 1 KB of consecutive bytes, in memory and in LDS.  A tile's fragments (256 weight
+// rows; the hidden states of a workgroup) lie together for each 64 values of K, so that a workgroup copies runs of several
+// KB.  The exponents (biased by 127) of four consecutive blocks are the bytes of one word per row, a tile's words together.
+// Rows and values beyond N, T and K are 0.
 #include "qws_lse.h"
 
 #include <type_traits>
+#include <utility>
 
 namespace qws {
 
@@ -26,27 +28,46 @@ typedef __bf16 f8_b8 __attribute__((ext_vector_type(8)));
 
 constexpr int F8_KB = 128;       // values of a block
 constexpr int F8_FRAG = 1024;    // bytes of a fragment; two along K are a block
-constexpr int F8_ROWS = 256;     // packed rows are a multiple of this
+constexpr int F8_ROWS = 256;     // weight rows of a tile
 constexpr int F8_NMAX = 1 << 24, F8_KMAX = 1 << 20;
 
 __host__ __device__ inline int f8_up(int n, int m) { return (n + m - 1) / m * m; }
 struct F8Layout {
   int rows, kb, kb4;      // padded rows, blocks, words of exponents per row
+  int groups;             // groups of 16 rows of a tile
   size_t scales, total;   // byte offsets
 };
-__host__ __device__ inline F8Layout f8_layout(int rows, int K) {
+// rows: in whole tiles; bytes: of a value
+__host__ __device__ inline F8Layout f8_layout(int rows, int K, int groups, int bytes) {
   F8Layout l;
-  l.rows = f8_up(rows, F8_ROWS);
+  l.groups = groups;
+  l.rows = f8_up(rows, 16 * groups);
   l.kb = f8_up(K, F8_KB) / F8_KB;
   l.kb4 = (l.kb + 3) / 4;
-  l.scales = (size_t)l.rows * l.kb * F8_KB;
-  l.total = (l.scales + (size_t)l.rows * l.kb4 * 4 + 255) & ~(size_t)255;
+  l.scales = (size_t)l.rows * l.kb * F8_KB * bytes;
+  l.total = (l.scales + (bytes == 1 ? (size_t)l.rows * l.kb4 * 4 : 0) + 255) & ~(size_t)255;
   return l;
+}
+__host__ __device__ inline F8Layout f8_weights(int N, int K) { return f8_layout(N, K, F8_ROWS / 16, 1); }
+
+// bf16 operand of product h (0, 1) of a fragment's 16 bytes, times the block's scale
+template <int H>
+__device__ __forceinline__ f8_b8 f8_wide(vu4 r, float scale) {
+  union {
+    f8_b2 p[4];
+    f8_b8 v;
+  } u;
+  u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r[2 * H], scale, false);
+  u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r[2 * H], scale, true);
+  u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r[2 * H + 1], scale, false);
+  u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r[2 * H + 1], scale, true);
+  return u.v;
 }
 
 // One wave per block of 16 rows: lane l takes row l % 16, values 16 (l / 16) .. + 15 of both fragments.  A value that is not
 // finite becomes NaN, the one such value that e4m3 has.
-template <typename T>
+//   WIDE: the values as bf16 instead (exact), as k_f8_tile takes hidden states: product h of fragment c is 1 KB of its own.
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) k_f8_pack(const T* x, long long stride, int rows, int K, F8Layout l, char* out) {
   const int lane = lane_id(), kb = blockIdx.y * 4 + wave_id(), group = blockIdx.x;
   if (kb >= l.kb4 * 4) return;
@@ -87,8 +108,7 @@ __global__ void __launch_bounds__(256) k_f8_pack(const T* x, long long stride, i
   most = max(most, (uint32_t)__shfl_xor((int)most, 32));
   // 448 = 1.75 * 2^8: biased exponent of the block, one more where the fraction is above .75; at least 0 (2^-127)
   const int e = max((int)(most >> 23) - 8 + ((most & 0x7FFFFFu) > 0x600000u ? 1 : 0), 0);
-  if ((lane >> 4) == 0) *((uint8_t*)(out + l.scales) + (((size_t)group * l.kb4 + kb / 4) * 16 + lane) * 4 + (kb & 3)) = (uint8_t)(kb < l.kb ? e : 0);
-  if (kb >= l.kb) return;
+  if (WIDE && kb >= l.kb) return;
   const float up = __uint_as_float((uint32_t)(254 - e) << 23);  // 2^(127 - e)
   uint32_t q[8];
 #pragma unroll
@@ -98,9 +118,26 @@ __global__ void __launch_bounds__(256) k_f8_pack(const T* x, long long stride, i
     for (int i = 0; i < 4; i++) f[i] = fabsf(v[4 * j + i]) <= F32_MAX ? v[4 * j + i] * up : NAN;
     q[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false), true);
   }
-  vu4* d = (vu4*)(out + ((size_t)group * l.kb + kb) * 2 * F8_FRAG);
-  d[lane] = (vu4){q[0], q[1], q[2], q[3]};
-  d[64 + lane] = (vu4){q[4], q[5], q[6], q[7]};
+  const size_t place = ((size_t)(group / l.groups) * l.kb + kb) * 2 * l.groups + group % l.groups;  // fragment 0 of the block; fragment 1: + l.groups
+  if constexpr (WIDE) {
+    const float scale = __uint_as_float((uint32_t)e << 23);
+    vu4* d = (vu4*)(out + place * 2 * F8_FRAG);
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      const vu4 w = {q[4 * c], q[4 * c + 1], q[4 * c + 2], q[4 * c + 3]};
+      d[c * l.groups * 128 + lane] = __builtin_bit_cast(vu4, f8_wide<0>(w, scale));
+      d[c * l.groups * 128 + 64 + lane] = __builtin_bit_cast(vu4, f8_wide<1>(w, scale));
+    }
+  } else {
+    if ((lane >> 4) == 0) {
+      const size_t word = ((size_t)(group / l.groups) * l.kb4 + kb / 4) * l.groups * 16 + group % l.groups * 16 + lane;
+      *((uint8_t*)(out + l.scales) + word * 4 + (kb & 3)) = (uint8_t)(kb < l.kb ? e : 0);
+    }
+    if (kb >= l.kb) return;
+    vu4* d = (vu4*)(out + place * F8_FRAG);
+    d[lane] = (vu4){q[0], q[1], q[2], q[3]};
+    d[l.groups * 64 + lane] = (vu4){q[4], q[5], q[6], q[7]};
+  }
 }
 
 struct F8Args {
@@ -117,19 +154,6 @@ struct F8Args {
   int parts;
 };
 
-// bf16 operand of product h (0, 1) of a fragment's 16 bytes, times the block's scale
-template <int H>
-__device__ __forceinline__ f8_b8 f8_wide(vu4 r, float scale) {
-  union {
-    f8_b2 p[4];
-    f8_b8 v;
-  } u;
-  u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r[2 * H], scale, false);
-  u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r[2 * H], scale, true);
-  u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r[2 * H + 1], scale, false);
-  u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r[2 * H + 1], scale, true);
-  return u.v;
-}
 __device__ __forceinline__ vf4 f8_mfma(f8_b8 a, f8_b8 b, vf4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 // the scale of block k from its word of four exponents
 __device__ __forceinline__ float f8_scale(uint32_t word, int k) { return __uint_as_float(((word >> (8 * (k & 3))) & 255u) << 23); }
@@ -161,32 +185,54 @@ __device__ __forceinline__ void f8_put(O* out, long long stride, int t, int n, i
     }
 }
 
-// A wave's logits of hidden state `t` (one of the lane's 16-lane column) at rows n0 + 16 i + 4 (lane / 16) + r, joined over the
-// column's four lanes; the given token's logit goes to a.given.
+// Logits y of hidden state `t` at rows n0 + 16 i + 4 (lane / 16) + r, joined over the four lanes that hold t; the logit of its
+// given token `tok` goes to a.given.  c: the temperature's scale.
 template <int F>
-__device__ __forceinline__ Lse f8_stats(const F8Args& a, const vf4* y, int t, int n0) {
-  const int tok = t < a.T ? a.tok[t] : -1;
-  const float c = lse_scale(a.temp && t < a.T ? a.temp[t] : 1.0f);
+__device__ __forceinline__ Lse f8_stats(const F8Args& a, const vf4* y, int t, int n0, int tok, float c) {
   const int nq = n0 + 4 * (lane_id() >> 4);
-  Lse v = {-INFINITY, 0.0f, 0.0f};
+  if (__any(tok >= n0 && tok < n0 + 16 * F)) {
 #pragma unroll
-  for (int i = 0; i < F; i++)
+    for (int i = 0; i < F; i++)
 #pragma unroll
-    for (int r = 0; r < 4; r++)
-      if (nq + 16 * i + r < a.N) v.m = fmaxf(v.m, lse_clean(y[i][r]));
+      for (int r = 0; r < 4; r++)
+        if (nq + 16 * i + r == tok) a.given[t] = lse_clean(y[i][r]);
+  }
+  Lse v;
+  float m = lse_max3(y[0][0], y[0][1], y[0][2]);
+#pragma unroll
+  for (int i = 0; i < F; i++) m = i == 0 ? lse_max3(m, y[0][3], y[0][3]) : lse_max3(lse_max3(m, y[i][0], y[i][1]), y[i][2], y[i][3]);
+  const float M = c * m;
+  float s = 0.0f, q = 0.0f;
 #pragma unroll
   for (int i = 0; i < F; i++)
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-      const int n = nq + 16 * i + r;
-      const float x = n < a.N ? lse_clean(y[i][r]) : -INFINITY;
-      const float d = lse_d(x, v.m, c), e = lse_exp2(d);
-      v.s += e;
-      v.t = fmaf(e, d, v.t);
-      if (n == tok) a.given[t] = x;
+      const float d = fmaf(y[i][r], c, -M), e = lse_exp2(d);
+      s += e;
+      q = fmaf(e, d, q);
     }
+  if (n0 + 16 * F <= a.N && __all(fabsf(m) < LSE_MOST && c <= LSE_MOST && fabsf(q) < INFINITY)) {
+    v = lse_exact(m, M, s, q, c);
+  } else {  // rows behind the last, NaN or extreme logits
+    v = {-INFINITY, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < F; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        if (nq + 16 * i + r < a.N) v.m = fmaxf(v.m, lse_clean(y[i][r]));
+#pragma unroll
+    for (int i = 0; i < F; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const float d = lse_d(nq + 16 * i + r < a.N ? lse_clean(y[i][r]) : -INFINITY, v.m, c), e = lse_exp2(d);
+        v.s += e;
+        v.t = fmaf(e, d, v.t);
+      }
+  }
   return lse_join_lanes(v, c, 16, 32);
 }
+__device__ __forceinline__ int f8_token(const F8Args& a, int t) { return t < a.T ? a.tok[t] : -1; }
+__device__ __forceinline__ float f8_temp_scale(const F8Args& a, int t) { return lse_scale(a.temp && t < a.T ? a.temp[t] : 1.0f); }
 __device__ __forceinline__ void f8_put_part(const F8Args& a, int t, int part, Lse v) { a.part[(size_t)t * a.parts + part] = make_float4(v.m, v.s, v.t, 0.0f); }
 template <typename O>
 __device__ __forceinline__ bool f8_can_be_wide(const F8Args& a) {
@@ -203,9 +249,10 @@ __global__ void __launch_bounds__(256) k_f8_few(F8Args a) {
   __shared__ Lse s_lse[G][16 * TF];
   const int lane = lane_id(), wave = wave_id(), g0 = blockIdx.x * G;
   const int kb = a.lw.kb, kb4 = a.lw.kb4, per = (kb + 3) / 4, lo = wave * per, hi = min(lo + per, kb);
-  const char* pw = a.w + (size_t)g0 * kb * (2 * F8_FRAG) + 16 * lane;
+  constexpr int WG = F8_ROWS / 16;  // groups of a tile; G divides it
+  const char* pw = a.w + ((size_t)(g0 / WG) * kb * 2 * WG + g0 % WG) * F8_FRAG + 16 * lane;
   const char* px = a.x + 16 * lane;
-  const uint32_t* qw = (const uint32_t*)(a.w + a.lw.scales) + (size_t)g0 * kb4 * 16 + (lane & 15);
+  const uint32_t* qw = (const uint32_t*)(a.w + a.lw.scales) + ((size_t)(g0 / WG) * kb4 * WG + g0 % WG) * 16 + (lane & 15);
   const uint32_t* qx = (const uint32_t*)(a.x + a.lx.scales) + (lane & 15);
   vf4 acc[G][TF] = {};
   vu4 w[G][2], x[TF][2];
@@ -214,15 +261,15 @@ __global__ void __launch_bounds__(256) k_f8_few(F8Args a) {
 #pragma unroll
     for (int g = 0; g < G; g++)
 #pragma unroll
-      for (int h = 0; h < 2; h++) w[g][h] = *gmem((const vu4*)(pw + ((size_t)g * kb + k) * (2 * F8_FRAG) + h * F8_FRAG));
+      for (int h = 0; h < 2; h++) w[g][h] = *gmem((const vu4*)(pw + ((size_t)(2 * k + h) * WG + g) * F8_FRAG));
 #pragma unroll
     for (int j = 0; j < TF; j++)
 #pragma unroll
-      for (int h = 0; h < 2; h++) x[j][h] = *gmem((const vu4*)(px + ((size_t)j * kb + k) * (2 * F8_FRAG) + h * F8_FRAG));
+      for (int h = 0; h < 2; h++) x[j][h] = *gmem((const vu4*)(px + ((size_t)(2 * k + h) * TF + j) * F8_FRAG));
 #pragma unroll
-    for (int g = 0; g < G; g++) ew[g] = *gmem(qw + ((size_t)g * kb4 + k / 4) * 16);
+    for (int g = 0; g < G; g++) ew[g] = *gmem(qw + ((size_t)(k / 4) * WG + g) * 16);
 #pragma unroll
-    for (int j = 0; j < TF; j++) ex[j] = *gmem(qx + ((size_t)j * kb4 + k / 4) * 16);
+    for (int j = 0; j < TF; j++) ex[j] = *gmem(qx + ((size_t)(k / 4) * TF + j) * 16);
   };
   if (lo < hi) load(lo);
   for (int k = lo; k < hi; k++) {
@@ -267,7 +314,7 @@ __global__ void __launch_bounds__(256) k_f8_few(F8Args a) {
     const int g = i / TF, t = 16 * (i % TF) + (lane & 15), n0 = 16 * (g0 + g);
     const vf4 y = (s_acc[0][i][lane] + s_acc[1][i][lane]) + (s_acc[2][i][lane] + s_acc[3][i][lane]);
     if constexpr (std::is_void_v<O>) {
-      const Lse v = f8_stats<1>(a, &y, t, n0);
+      const Lse v = f8_stats<1>(a, &y, t, n0, f8_token(a, t), f8_temp_scale(a, t));
       if (lane < 16) s_lse[g][t] = v;
     } else {
       f8_put<O>((O*)a.out, a.out_stride, t, n0 + 4 * (lane >> 4), a.T, a.N, y, wide);
@@ -278,7 +325,7 @@ __global__ void __launch_bounds__(256) k_f8_few(F8Args a) {
     const int t = threadIdx.x;
     if (t < 16 * TF && t < a.T) {
       Lse v = s_lse[0][t];
-      const float c = lse_scale(a.temp ? a.temp[t] : 1.0f);
+      const float c = f8_temp_scale(a, t);
 #pragma unroll
       for (int g = 1; g < G; g++) v = lse_join(v, s_lse[g][t], c);
       f8_put_part(a, t, blockIdx.x, v);
@@ -286,107 +333,194 @@ __global__ void __launch_bounds__(256) k_f8_few(F8Args a) {
   }
 }
 
-// Tiles of BN weight rows x BT hidden states, WN x WT waves.  A block of 128 along K is a stage: in registers while the one
-// before is computed, then in one of two LDS buffers.
-template <typename O, int BN, int BT, int WN, int WT>
-__global__ void __launch_bounds__(64 * WN * WT, 2) k_f8_tile(F8Args a, int tiles_n, int tiles_t) {
-  constexpr int NT = 64 * WN * WT, GN = BN / 16, GT = BT / 16, FN = GN / WN, FT = GT / WT, GB = 2 * F8_FRAG;
-  constexpr int LN = GN * GB / (16 * NT), LT = GT * GB / (16 * NT), STEP = 16 * NT / GB;  // loads of a thread; groups of one load
-  static_assert(LN * 16 * NT == GN * GB && LT * 16 * NT == GT * GB && STEP * GB == 16 * NT, "whole loads");
-  static_assert(BN + BT <= NT, "a thread per row for the scales");
-  __shared__ vu4 s_buf[2][(GN + GT) * GB / 16];
-  __shared__ uint32_t s_sc[2][BN + BT];
+typedef __attribute__((address_space(3))) void f8_lds;
+// 1 KB of consecutive bytes of memory into LDS, 16 bytes a lane, past the registers; OFFSET (below 4 KB) moves both places.
+// The instruction is written out because the compiler, where it knows of such a copy, waits for all of them before a read of
+// LDS; what has arrived is f8_meet's to say.
+template <int OFFSET>
+__device__ __forceinline__ void f8_copy(const char* from, uint32_t lane_offset, const void* to) {
+  const uint32_t at = (uint32_t)(uintptr_t)(f8_lds*)to;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(at), "v"(lane_offset), "s"(from), "n"(OFFSET) : "memory", "m0");
+}
+__device__ __forceinline__ void f8_copy_words(const char* from, uint32_t lane_offset, const void* to) {  // 64 words
+  const uint32_t at = (uint32_t)(uintptr_t)(f8_lds*)to;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(at), "v"(lane_offset), "s"(from) : "memory", "m0");
+}
+// Waits until at most N of the wave's newest loads are in flight and its LDS reads are done, then for the workgroup.  One
+// statement that no memory access moves across.
+template <int N>
+__device__ __forceinline__ void f8_meet() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// Tiles of 256 weight rows x 32 FT hidden states: 4 waves of 128 x 16 FT, one to a SIMD.  A stage is 64 values along K, 16 KB
+// of weights and 4 FT KB of hidden states (already bf16: k_f8_pack), copied by the memory system straight into one of three
+// LDS buffers, three stages ahead.  A stage has two halves of 32 values: the first half's products run while the second
+// half's hidden states are read, then everybody meets (a wave first waits for its own copies of the next stage; the newest
+// stage's stay in flight), and the second half's products run while the next stage's operands are read.  A half has a step
+// for each fragment of weights: its FT products, and beside them the next fragment's widening to bf16, a few reads and one
+// copy (into the buffer that the last meeting freed: over the second half and the next first one), little enough for the
+// time of as many products.  A workgroup takes every 256th tile; the first stages of its next one are copied while it
+// finishes the last.
+template <int FT>
+struct F8Buf {
+  vu4 w[F8_ROWS / 16 * 64];
+  vu4 x[2 * FT * 128];
+  uint32_t e[F8_ROWS];  // exponents
+};
+constexpr int F8_CUS = 256;
+template <typename O, int FT>
+__global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int tiles_t) {
+  constexpr int BN = F8_ROWS, BT = 32 * FT, WN = 2, WT = 2, FN = 8, GN = BN / 16, GT = BT / 16;
+  constexpr int NEW = GN / 4 + FT + 1;  // copies of a wave per stage: 4 KB of weights, FT of hidden states, 64 exponents
+  static_assert(NEW <= 2 * FN, "one a step");
+  __shared__ F8Buf<FT> b0, b1, b2;
   __shared__ Lse s_lse[std::is_void_v<O> ? WN : 1][std::is_void_v<O> ? BT : 1];
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), wn = wave / WT, wt = wave % WT;
+  const int kb4 = a.lw.kb4, stages = 2 * a.lw.kb;
+  const uint32_t o16 = 16 * lane, o4 = 4 * lane;
+  const char *pw, *px, *pe;  // the wave's copies of the tile
   // XCD x (workgroups x, x + 8, ..) takes the tiles of weight rows x, x + 8, .., all of their hidden states in a row: the
   // weights of a tile come into one L2 once
-  const int seq = blockIdx.x >> 3, tn = (seq / tiles_t) * 8 + (blockIdx.x & 7), tt = seq % tiles_t;
-  if (tn >= tiles_n) return;
-  const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), wn = wave / WT, wt = wave % WT;
-  const int n0 = tn * BN, t0 = tt * BT, kb = a.lw.kb, kb4 = a.lw.kb4;
-  const size_t run = (size_t)kb * GB;  // bytes of a group
-  const char* pw = a.w + (size_t)(n0 / 16) * run + (size_t)(tid * 16 / GB) * run + tid * 16 % GB;
-  const char* px = a.x + (size_t)(t0 / 16) * run + (size_t)(tid * 16 / GB) * run + tid * 16 % GB;
-  const int row = tid < BN ? n0 + tid : t0 + tid - BN;
-  const uint32_t* ps = (const uint32_t*)(tid < BN ? a.w + a.lw.scales : a.x + a.lx.scales) + (size_t)(row / 16) * kb4 * 16 + row % 16;
-  const bool has_scale = tid < BN + BT;
-  vu4 r[LN + LT];
-  auto load = [&](int k) {
-#pragma unroll
-    for (int i = 0; i < LN; i++) r[i] = *gmem((const vu4*)(pw + i * STEP * run + (size_t)k * GB));
-#pragma unroll
-    for (int i = 0; i < LT; i++) r[LN + i] = *gmem((const vu4*)(px + i * STEP * run + (size_t)k * GB));
+  auto row_tile = [&](int id) { return (id >> 3) / tiles_t * 8 + (id & 7); };
+  auto point = [&](int id) {
+    const int tn = row_tile(id), tt = (id >> 3) % tiles_t;
+    pw = a.w + ((size_t)tn * stages * GN + 4 * wave) * F8_FRAG;
+    px = a.x + ((size_t)tt * stages * 4 * FT + FT * wave) * 1024;
+    pe = a.w + a.lw.scales + (size_t)tn * kb4 * 4 * BN + 256 * wave;
   };
-  auto store = [&](int b) {
-#pragma unroll
-    for (int i = 0; i < LN + LT; i++) s_buf[b][i * NT + tid] = r[i];
+  auto copy = [&](int k, F8Buf<FT>& b, auto D) {  // copy D of stage k
+    constexpr int d = decltype(D)::value, xd = d - GN / 4;
+    k = min(k, stages - 1);  // past the end: the last stage again, into a buffer that is not read any more
+    if constexpr (d < GN / 4)
+      f8_copy<d * 1024>(pw + (size_t)k * (GN * F8_FRAG), o16, b.w + GN / 4 * wave * 64);
+    else if constexpr (d < NEW - 1)
+      f8_copy<xd % 4 * 1024>(px + (size_t)k * (4 * FT * 1024) + xd / 4 * 4096, o16, b.x + (FT * wave + xd / 4 * 4) * 64);
+    else if constexpr (d == NEW - 1)
+      f8_copy_words(pe + (size_t)(k / 8) * (4 * BN), o4, b.e + 64 * wave);
   };
-  uint32_t word = 0;
-  if (has_scale) s_sc[0][tid] = *gmem(ps);
-  load(0);
-  store(0);
-  load(min(1, kb - 1));
-  bar();
-  vf4 acc[FN][FT] = {};
-  for (int k = 0; k < kb; k++) {
-    if (k + 1 < kb) store((k + 1) & 1);
-    if ((k & 3) == 0 && has_scale) word = *gmem(ps + (size_t)min(k / 4 + 1, kb4 - 1) * 16);
-    if ((k & 3) == 3 && has_scale) s_sc[(k / 4 + 1) & 1][tid] = word;
-    load(min(k + 2, kb - 1));
-    const uint32_t* sc = s_sc[(k / 4) & 1];
-    const vu4* buf = s_buf[k & 1] + lane;
-    float sw[FN], sx[FT];
+  auto each = [&](auto f) {  // f(0) .. f(FN - 1), as constants
+    [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>()), ...); }(std::make_integer_sequence<int, FN>());
+  };
+  auto copy_all = [&](int k, F8Buf<FT>& b) {
+    each([&](auto I) {
+      copy(k, b, std::integral_constant<int, decltype(I)::value>());
+      copy(k, b, std::integral_constant<int, decltype(I)::value + FN>());
+    });
+  };
+  vu4 w[FN];
+  uint32_t word[FN];
+  f8_b8 x0[FT], x1[FT], q;
+  vf4 acc[FN][FT];
+  auto read_x = [&](const F8Buf<FT>& b, int h, int j) { return __builtin_bit_cast(f8_b8, b.x[((wt * FT + j) * 2 + h) * 64 + lane]); };
+  auto read_w = [&](const F8Buf<FT>& b, int i) {
+    w[i] = b.w[(wn * FN + i) * 64 + lane];
+    word[i] = b.e[16 * (wn * FN + i) + (lane & 15)];
+  };
+  // stage k in b; `next` holds the next one, `last` the one before (free; the copies of stage k + 2 go on into it)
+  auto stage = [&](int k, F8Buf<FT>& b, const F8Buf<FT>& next, F8Buf<FT>& last) {
+    const int kb = k >> 1, kn = (k + 1) >> 1;
+    each([&](auto I) {
+      constexpr int i = decltype(I)::value;
 #pragma unroll
-    for (int i = 0; i < FN; i++) sw[i] = f8_scale(sc[(wn * FN + i) * 16 + (lane & 15)], k);
+      for (int j = 0; j < FT; j++)
+        if (j / 2 == i) x1[j] = read_x(b, 1, j);
+      const f8_b8 qn = i + 1 < FN ? f8_wide<0>(w[(i + 1) % FN], f8_scale(word[(i + 1) % FN], kb)) : f8_wide<1>(w[0], f8_scale(word[0], kb));
 #pragma unroll
-    for (int j = 0; j < FT; j++) sx[j] = f8_scale(sc[BN + (wt * FT + j) * 16 + (lane & 15)], k);
+      for (int j = 0; j < FT; j++) acc[i][j] = f8_mfma(q, x0[j], acc[i][j]);
+      copy(k + 2, last, std::integral_constant<int, i + FN>());
+      q = qn;
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    f8_meet<NEW>();
+    each([&](auto I) {
+      constexpr int i = decltype(I)::value;
+      f8_b8 qn;
+      if (i + 1 < FN) qn = f8_wide<1>(w[(i + 1) % FN], f8_scale(word[(i + 1) % FN], kb));
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      f8_b8 b0[FT], b1[FT];
+      for (int j = 0; j < FT; j++)
+        if (j / 2 == i) x0[j] = read_x(next, 0, j);
+      read_w(next, i);
+      if (i + 1 == FN) qn = f8_wide<0>(w[0], f8_scale(word[0], kn));
+#pragma unroll
+      for (int j = 0; j < FT; j++) acc[i][j] = f8_mfma(q, x1[j], acc[i][j]);
+      copy(k + 3, b, I);
+      q = qn;
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  const int total = (tiles_n + 7) / 8 * 8 * tiles_t;
+  int id = blockIdx.x;
+  while (id < total && row_tile(id) >= tiles_n) id += gridDim.x;
+  if (id >= total) return;
+  point(id);
+  copy_all(0, b0);
+  copy_all(1, b1);
+  for (;;) {
+    const int tn = row_tile(id), n0 = tn * BN, t0 = (id >> 3) % tiles_t * BT;
+    each([&](auto I) { copy(2, b2, I); });  // the others follow in the first half
+    f8_meet<NEW + FN>();
+#pragma unroll
+    for (int i = 0; i < FN; i++) read_w(b0, i);
+#pragma unroll
+    for (int j = 0; j < FT; j++) x0[j] = read_x(b0, 0, j);
+    q = f8_wide<0>(w[0], f8_scale(word[0], 0));
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+#pragma unroll
+      for (int j = 0; j < FT; j++) acc[i][j] = (vf4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < stages; k += 3) {
+      stage(k, b0, b1, b2);
+      if (k + 1 < stages) stage(k + 1, b1, b2, b0);
+      if (k + 2 < stages) stage(k + 2, b2, b0, b1);
+    }
+    f8_meet<0>();  // the copies past the end
+    do id += gridDim.x;
+    while (id < total && row_tile(id) >= tiles_n);
+    if (id < total) {
+      point(id);
+      copy_all(0, b0);
+      copy_all(1, b1);
+    }
+    if constexpr (std::is_void_v<O>) {
+      int tok[FT];
+      float c[FT];
 #pragma unroll
       for (int j = 0; j < FT; j++) {
-        const vu4 x = buf[(GN + wt * FT + j) * (GB / 16) + h * 64];
-        b0[j] = f8_wide<0>(x, sx[j]);
-        b1[j] = f8_wide<1>(x, sx[j]);
+        const int t = t0 + (wt * FT + j) * 16 + (lane & 15);
+        tok[j] = f8_token(a, t);
+        c[j] = f8_temp_scale(a, t);
       }
 #pragma unroll
-      for (int i = 0; i < FN; i++) {
-        const vu4 w = buf[(wn * FN + i) * (GB / 16) + h * 64];
-        const f8_b8 a0 = f8_wide<0>(w, sw[i]), a1 = f8_wide<1>(w, sw[i]);
+      for (int j = 0; j < FT; j++) {
+        const int tl = (wt * FT + j) * 16 + (lane & 15);
+        vf4 y[FN];
 #pragma unroll
-        for (int j = 0; j < FT; j++) acc[i][j] = f8_mfma(a0, b0[j], acc[i][j]);
-#pragma unroll
-        for (int j = 0; j < FT; j++) acc[i][j] = f8_mfma(a1, b1[j], acc[i][j]);
+        for (int i = 0; i < FN; i++) y[i] = acc[i][j];
+        const Lse v = f8_stats<FN>(a, y, t0 + tl, n0 + wn * FN * 16, tok[j], c[j]);
+        if (lane < 16) s_lse[wn][tl] = v;
       }
-    }
-    bar();
-  }
-  const bool wide = f8_can_be_wide<f8_out<O>>(a);
+      bar();
+      const int t = t0 + tid;
+      if (tid < BT && t < a.T) {  // BT <= 256 threads
+        Lse v = s_lse[0][tid];
 #pragma unroll
-  for (int j = 0; j < FT; j++) {
-    const int tl = (wt * FT + j) * 16 + (lane & 15), n = n0 + wn * FN * 16;
-    vf4 y[FN];
-#pragma unroll
-    for (int i = 0; i < FN; i++) y[i] = acc[i][j];
-    if constexpr (std::is_void_v<O>) {
-      const Lse v = f8_stats<FN>(a, y, t0 + tl, n);
-      if (lane < 16) s_lse[wn][tl] = v;
+        for (int i = 1; i < WN; i++) v = lse_join(v, s_lse[i][tid], f8_temp_scale(a, t));
+        f8_put_part(a, t, tn, v);
+      }
+      bar();  // before the next tile's statistics
     } else {
+      const bool wide = f8_can_be_wide<O>(a);
 #pragma unroll
-      for (int i = 0; i < FN; i++) f8_put<O>((O*)a.out, a.out_stride, t0 + tl, n + 16 * i + 4 * (lane >> 4), a.T, a.N, y[i], wide);
-    }
-  }
-  if constexpr (std::is_void_v<O>) {
-    bar();
-    const int t = t0 + tid;
-    if (tid < BT && t < a.T) {
-      Lse v = s_lse[0][tid];
-      const float c = lse_scale(a.temp ? a.temp[t] : 1.0f);
+      for (int j = 0; j < FT; j++)
 #pragma unroll
-      for (int i = 1; i < WN; i++) v = lse_join(v, s_lse[i][tid], c);
-      f8_put_part(a, t, tn, v);
+        for (int i = 0; i < FN; i++)
+          f8_put<O>((O*)a.out, a.out_stride, t0 + (wt * FT + j) * 16 + (lane & 15), n0 + (wn * FN + i) * 16 + 4 * (lane >> 4), a.T, a.N, acc[i][j], wide);
     }
+    if (id >= total) return;
   }
 }
+
 // One wave per hidden state: its parts joined
 __global__ void __launch_bounds__(256) k_f8_score(F8Args a, float* out_lp, float* out_h) {
   const int lane = lane_id(), t = blockIdx.x * 4 + wave_id();
@@ -404,19 +538,17 @@ __global__ void __launch_bounds__(256) k_f8_score(F8Args a, float* out_lp, float
   if (out_h) out_h[t] = lse_entropy(v);
 }
 
-template <typename T>
-int f8_pack(const void* x, long long stride, int rows, int K, char* out, hipStream_t st) {
-  const F8Layout l = f8_layout(rows, K);
-  hipLaunchKernelGGL((k_f8_pack<T>), dim3(l.rows / 16, l.kb4), dim3(256), 0, st, (const T*)x, stride, rows, K, l, out);
+template <typename T, bool WIDE>
+int f8_pack(const void* x, long long stride, int rows, int K, F8Layout l, char* out, hipStream_t st) {
+  hipLaunchKernelGGL((k_f8_pack<T, WIDE>), dim3(l.rows / 16, l.kb4), dim3(256), 0, st, (const T*)x, stride, rows, K, l, out);
   return (int)hipGetLastError();
 }
 
-// What runs T hidden states against N weight rows: row groups of a workgroup of k_f8_few (0: k_f8_tile), the tile, and the
-// parts that scoring joins per hidden state.
+// What runs T hidden states against N weight rows: k_f8_few with `groups` row groups to a workgroup and `frags` fragments of
+// hidden states, or (groups = 0) k_f8_tile with `frags` fragments to a wave; the parts that scoring joins per hidden state.
 struct F8Plan {
-  int groups, frags, bt, parts;
+  int groups, frags, parts;
 };
-constexpr int F8_BN = 256;
 inline F8Plan f8_plan(int T, int N) {
   F8Plan p = {};
   if (T <= 64) {
@@ -425,17 +557,23 @@ inline F8Plan f8_plan(int T, int N) {
     p.groups = f8_up(N, 64) / 64 < 512 ? 1 : p.frags == 4 ? 2 : 4;
     p.parts = f8_up(N, 16 * p.groups) / (16 * p.groups);
   } else {
-    p.bt = T <= 128 ? 128 : 256;
-    p.parts = f8_up(N, F8_BN) / F8_BN;
+    const int tiles = (T + 255) / 256;
+    p.frags = ((T + tiles - 1) / tiles + 31) / 32;
+    p.parts = f8_up(N, F8_ROWS) / F8_ROWS;
   }
   return p;
+}
+// the packed hidden states: a workgroup's are a tile, 8-bit or (k_f8_tile) bf16
+inline F8Layout f8_states(int T, int N, int K) {
+  const F8Plan p = f8_plan(T, N);
+  return p.groups ? f8_layout(T, K, p.frags, 1) : f8_layout(T, K, 2 * p.frags, 2);
 }
 struct F8Ws {
   size_t part, given, total;
 };
 inline F8Ws f8_ws(int T, int N, int K, bool score) {
   F8Ws w;
-  w.part = f8_layout(T, K).total;
+  w.part = f8_states(T, N, K).total;
   w.given = w.part + (score ? (size_t)T * f8_plan(T, N).parts * sizeof(float4) : 0);
   w.total = (w.given + (score ? (size_t)T * 4 : 0) + 255) & ~(size_t)255;
   return w;
@@ -446,15 +584,16 @@ inline bool f8_aligned(const void* p) { return p && ((uintptr_t)p & 255) == 0; }
 
 }  // namespace qws
 
-extern "C" size_t qws_fp8_pack_bytes(int N, int K) { return qws::f8_shape(1, N, K) && qws::f8_fits(1, N, K) ? qws::f8_layout(N, K).total : 0; }
+extern "C" size_t qws_fp8_pack_bytes(int N, int K) { return qws::f8_shape(1, N, K) && qws::f8_fits(1, N, K) ? qws::f8_weights(N, K).total : 0; }
 
 extern "C" int qws_fp8_pack(const void* w, int dtype, int N, int K, long long row_stride, void* packed, void* stream) {
   using namespace qws;
   if (!f8_shape(1, N, K) || (dtype != QWS_DTYPE_F32 && dtype != QWS_DTYPE_BF16) || !w || row_stride < 0 || !f8_aligned(packed)) return QWS_ERR_INVALID;
   if ((uintptr_t)w & (dtype == QWS_DTYPE_F32 ? 3 : 1)) return QWS_ERR_INVALID;
   if (!f8_fits(1, N, K)) return QWS_ERR_NOT_SUPPORTED;
-  return dtype == QWS_DTYPE_F32 ? f8_pack<float>(w, row_stride, N, K, (char*)packed, (hipStream_t)stream)
-                                : f8_pack<uint16_t>(w, row_stride, N, K, (char*)packed, (hipStream_t)stream);
+  const F8Layout l = f8_weights(N, K);
+  return dtype == QWS_DTYPE_F32 ? f8_pack<float, false>(w, row_stride, N, K, l, (char*)packed, (hipStream_t)stream)
+                                : f8_pack<uint16_t, false>(w, row_stride, N, K, l, (char*)packed, (hipStream_t)stream);
 }
 
 extern "C" size_t qws_fp8_head_ws_bytes(int T, int N, int K) {
@@ -477,8 +616,8 @@ static F8Args f8_args(const void* packed, int N, int K, int T, const void* ws) {
   F8Args a = {};
   a.w = (const char*)packed;
   a.x = (const char*)ws;
-  a.lw = f8_layout(N, K);
-  a.lx = f8_layout(T, K);
+  a.lw = f8_weights(N, K);
+  a.lx = f8_states(T, N, K);
   a.N = N;
   a.T = T;
   return a;
@@ -487,18 +626,29 @@ template <typename O, int G, int TF>
 static void f8_few(const F8Args& a, hipStream_t st) {
   hipLaunchKernelGGL((k_f8_few<O, G, TF>), dim3((a.N + 16 * G - 1) / (16 * G)), dim3(256), 0, st, a);
 }
-template <typename O, int BT, int WN, int WT>
+template <typename O, int FT>
 static void f8_tile(const F8Args& a, hipStream_t st) {
-  const int tn = (a.N + F8_BN - 1) / F8_BN, tt = (a.T + BT - 1) / BT;
-  hipLaunchKernelGGL((k_f8_tile<O, F8_BN, BT, WN, WT>), dim3((tn + 7) / 8 * 8 * tt), dim3(64 * WN * WT), 0, st, a, tn, tt);
+  const int tn = (a.N + F8_ROWS - 1) / F8_ROWS, tt = (a.T + 32 * FT - 1) / (32 * FT);
+  const int total = (tn + 7) / 8 * 8 * tt;
+  hipLaunchKernelGGL((k_f8_tile<O, FT>), dim3(total < F8_CUS ? total : F8_CUS), dim3(256), 0, st, a, tn, tt);
 }
+// packs the hidden states and runs the product
 template <typename O>
-static int f8_product(F8Args a, hipStream_t st) {
+static int f8_product(F8Args a, int K, const void* x, long long x_stride, char* ws, hipStream_t st) {
   const F8Plan p = f8_plan(a.T, a.N);
   a.parts = p.parts;
-  if (p.groups == 0)
-    p.bt == 128 ? f8_tile<O, 128, 4, 2>(a, st) : f8_tile<O, 256, 2, 4>(a, st);
-  else if (p.frags == 1)
+  const int e = p.groups ? f8_pack<uint16_t, false>(x, x_stride, a.T, K, a.lx, ws, st) : f8_pack<uint16_t, true>(x, x_stride, a.T, K, a.lx, ws, st);
+  if (e) return e;
+  if (p.groups == 0) {
+    switch (p.frags) {
+      case 3: f8_tile<O, 3>(a, st); break;
+      case 4: f8_tile<O, 4>(a, st); break;
+      case 5: f8_tile<O, 5>(a, st); break;
+      case 6: f8_tile<O, 6>(a, st); break;
+      case 7: f8_tile<O, 7>(a, st); break;
+      default: f8_tile<O, 8>(a, st);
+    }
+  } else if (p.frags == 1)
     p.groups == 1 ? f8_few<O, 1, 1>(a, st) : f8_few<O, 4, 1>(a, st);
   else if (p.frags == 2)
     p.groups == 1 ? f8_few<O, 1, 2>(a, st) : f8_few<O, 4, 2>(a, st);
@@ -516,12 +666,11 @@ extern "C" int qws_fp8_head(const void* packed, int N, int K, const void* x, lon
   if (out_dtype != QWS_DTYPE_F32 && out_dtype != QWS_DTYPE_BF16) return QWS_ERR_INVALID;
   if (T == 0) return QWS_OK;
   if (!out || ((uintptr_t)out & (out_dtype == QWS_DTYPE_F32 ? 3 : 1)) || (T > 1 && out_stride < N) || ws_bytes < f8_ws(T, N, K, false).total) return QWS_ERR_INVALID;
-  const int e = f8_pack<uint16_t>(x, x_stride, T, K, (char*)ws, (hipStream_t)stream);
-  if (e) return e;
   F8Args a = f8_args(packed, N, K, T, ws);
   a.out = out;
   a.out_stride = out_stride;
-  return out_dtype == QWS_DTYPE_F32 ? f8_product<float>(a, (hipStream_t)stream) : f8_product<uint16_t>(a, (hipStream_t)stream);
+  return out_dtype == QWS_DTYPE_F32 ? f8_product<float>(a, K, x, x_stride, (char*)ws, (hipStream_t)stream)
+                                    : f8_product<uint16_t>(a, K, x, x_stride, (char*)ws, (hipStream_t)stream);
 }
 
 extern "C" int qws_fp8_score(const void* packed, int N, int K, const void* x, long long x_stride, int T, const int* tokens, const float* temperature,
@@ -531,15 +680,13 @@ extern "C" int qws_fp8_score(const void* packed, int N, int K, const void* x, lo
   if (c != QWS_OK || T == 0) return c;
   const F8Ws w = f8_ws(T, N, K, true);
   if (!tokens || !out_logprobs || ws_bytes < w.total) return QWS_ERR_INVALID;
-  int e = f8_pack<uint16_t>(x, x_stride, T, K, (char*)ws, (hipStream_t)stream);
-  if (e) return e;
   F8Args a = f8_args(packed, N, K, T, ws);
   a.tok = tokens;
   a.temp = temperature;
   a.part = (float4*)((char*)ws + w.part);
   a.given = (float*)((char*)ws + w.given);
   a.parts = f8_plan(T, N).parts;
-  e = f8_product<void>(a, (hipStream_t)stream);
+  const int e = f8_product<void>(a, K, x, x_stride, (char*)ws, (hipStream_t)stream);
   if (e) return e;
   hipLaunchKernelGGL(k_f8_score, dim3((T + 3) / 4), dim3(256), 0, (hipStream_t)stream, a, out_logprobs, out_entropy);
   return (int)hipGetLastError();

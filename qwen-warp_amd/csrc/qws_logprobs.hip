@@ -91,19 +91,13 @@ __device__ __forceinline__ vu4 lp_load_edge(const T* base, int v, int lead, int 
   return r;
 }
 
-// The largest of the block's values; a NaN shows in the sums (lp_fast), not here.  One instruction for two values, where
-// fmaxf on loaded values also has to quiet them.
-__device__ __forceinline__ float lp_max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
+// The largest of a vector; a NaN shows in the sums (lp_fast), not here
 template <int E>
 __device__ __forceinline__ float lp_max(const float* x) {
-  float m = lp_max3(x[0], x[1], x[2]);
+  float m = lse_max3(x[0], x[1], x[2]);
 #pragma unroll
-  for (int j = 3; j + 1 < E; j += 2) m = lp_max3(m, x[j], x[j + 1]);
-  return lp_max3(m, x[E - 1], x[E - 1]);
+  for (int j = 3; j + 1 < E; j += 2) m = lse_max3(m, x[j], x[j + 1]);
+  return lse_max3(m, x[E - 1], x[E - 1]);
 }
 
 // The largest of each group's lanes (8 or 16), in every lane: one instruction a step, where fmaxf of a moved value takes four.
@@ -125,10 +119,9 @@ __device__ __forceinline__ void lp_group_max(float (&m)[U]) {
 #undef QWS_DPP
 }
 
-// A lane's sums over blocks of logits of moderate size (below LP_MOST in magnitude at their largest, no -inf, no NaN),
+// A lane's sums over blocks of logits of moderate size (below LSE_MOST in magnitude at their largest, no -inf, no NaN),
 // relative to any reference M = fl(c m) within LP_SLACK of the largest, so that M rarely moves: a multiply-add, an
 // exponential and two sums per logit.  Blocks with anything else go to Lse's general form (lp_slow).
-constexpr float LP_MOST = 0x1p60f;  // and c <= 2^60: products stay finite
 constexpr float LP_SLACK = 8.0f;    // in log2 units: d <= 8, so the entropy's two terms cancel by 8 units at most
 struct LpFast {
   float m, M, limit, s, t;
@@ -155,11 +148,9 @@ __device__ __forceinline__ bool lp_fast(LpFast& f, const float (&x)[U][E], float
   f.t = t;
   return true;
 }
-// the fast sums relative to c m: r = c m - M is what rounding M took
 __device__ __forceinline__ Lse lp_fast_end(const LpFast& f, float c) {
   if (f.m == -INFINITY) return {-INFINITY, 0.0f, 0.0f};
-  const float r = fmaf(c, f.m, -f.M), e = lse_exp2(-r);
-  return {f.m, f.s * e, e * fmaf(-r, f.s, f.t)};
+  return lse_exact(f.m, f.M, f.s, f.t, c);
 }
 template <int U, int E>
 __device__ __forceinline__ void lp_slow(Lse& v, const float (&x)[U][E], float best, float c) {
@@ -192,13 +183,13 @@ __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
   const int nstripes = (end + SE - 1) / SE, s_end = min((ch + 1) * a.per, nstripes);
   float xt = 0.0f;
   int tv = -1, cnt = 0;  // virtual position of the token (-1: skipped), logits before it
-  bool moderate = c <= LP_MOST;  // no given token's logit is extreme
+  bool moderate = c <= LSE_MOST;  // no given token's logit is extreme
   if constexpr (RANK == 1) {
     const int t = a.tok[row];
     if (t >= 0 && t < a.V) {
       tv = t + lead;
       xt = lp_one(p + t);
-      moderate = moderate && fabsf(xt) < LP_MOST;
+      moderate = moderate && fabsf(xt) < LSE_MOST;
     }
   }
   if constexpr (RANK == 2) {
@@ -210,7 +201,7 @@ __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
       s_cnt[tid] = 0;
     }
     bar();
-    for (int k = 0; k < a.M; k += 64) moderate = moderate && !__any(k + lane < a.M && !(fabsf(s_xt[min(k + lane, a.M - 1)]) < LP_MOST));
+    for (int k = 0; k < a.M; k += 64) moderate = moderate && !__any(k + lane < a.M && !(fabsf(s_xt[min(k + lane, a.M - 1)]) < LSE_MOST));
   }
   Lse v = {-INFINITY, 0.0f, 0.0f};
   LpFast f = {-INFINITY, -1e30f, -INFINITY, 0.0f, 0.0f};
@@ -234,7 +225,7 @@ __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
       best = fmaxf(best, top[u]);
       least = fminf(least, top[u]);
     }
-    if (!(moderate && __all(best < LP_MOST && least > -LP_MOST)) || !lp_fast(f, x, best, c)) {
+    if (!(moderate && __all(best < LSE_MOST && least > -LSE_MOST)) || !lp_fast(f, x, best, c)) {
       best = -INFINITY;
 #pragma unroll
       for (int u = 0; u < U; u++) {

@@ -35,6 +35,21 @@ __device__ __forceinline__ float lse_temp(float T) { return T > 0.0f ? T : 1.0f;
 __device__ __forceinline__ float lse_scale(float T) { return fminf((float)LOG2E / lse_temp(T), F32_MAX); }
 __device__ __forceinline__ float lse_d(float x, float m, float c) { return fmaxf((x - m) * c, -LSE_DMIN); }  // NaN (-inf - -inf): -D_MIN
 
+// The largest of three; a NaN does not show in it.  One instruction, where fmaxf on values that may be signalling NaNs also
+// has to quiet them.
+__device__ __forceinline__ float lse_max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// Sums of moderate values (below LSE_MOST in magnitude, c as well) relative to M = fl(c m) take one multiply-add for d; what
+// rounding M took, r = c m - M, is given back at the end.
+constexpr float LSE_MOST = 0x1p60f;
+__device__ __forceinline__ Lse lse_exact(float m, float M, float s, float t, float c) {
+  const float r = fmaf(c, m, -M), e = lse_exp2(-r);
+  return {m, s * e, e * fmaf(-r, s, t)};
+}
+
 __device__ __forceinline__ Lse lse_join(Lse a, Lse b, float c) {
   const float m = fmaxf(a.m, b.m);
   const float da = lse_d(a.m, m, c), db = lse_d(b.m, m, c), ea = lse_exp2(da), eb = lse_exp2(db);
