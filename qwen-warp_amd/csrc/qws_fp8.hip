@@ -29,6 +29,7 @@ typedef __bf16 f8_b8 __attribute__((ext_vector_type(8)));
 constexpr int F8_KB = 128;       // values of a block
 constexpr int F8_FRAG = 1024;    // bytes of a fragment; two along K are a block
 constexpr int F8_ROWS = 256;     // weight rows of a tile
+constexpr int F8_CUS = 256;
 constexpr int F8_NMAX = 1 << 24, F8_KMAX = 1 << 20;
 
 __host__ __device__ inline int f8_up(int n, int m) { return (n + m - 1) / m * m; }
@@ -353,8 +354,8 @@ __device__ __forceinline__ void f8_meet() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// Tiles of 256 weight rows x 32 FT hidden states: 4 waves of 128 x 16 FT, one to a SIMD.  A stage is 64 values along K, 16 KB
-// of weights and 4 FT KB of hidden states (already bf16: k_f8_pack), copied by the memory system straight into one of three
+// Tiles of 32 FN weight rows (128 or 256) x 32 FT hidden states: 4 waves of 16 FN x 16 FT, one to a SIMD.  A stage is 64
+// values along K, 2 FN KB of weights and 4 FT KB of hidden states (already bf16: k_f8_pack), copied by the memory system straight into one of three
 // LDS buffers, three stages ahead.  A stage has two halves of 32 values: the first half's products run while the second
 // half's hidden states are read, then everybody meets (a wave first waits for its own copies of the next stage; the newest
 // stage's stay in flight), and the second half's products run while the next stage's operands are read.  A half has a step
@@ -362,19 +363,19 @@ __device__ __forceinline__ void f8_meet() {
 // copy (into the buffer that the last meeting freed: over the second half and the next first one), little enough for the
 // time of as many products.  A workgroup takes every 256th tile; the first stages of its next one are copied while it
 // finishes the last.
-template <int FT>
+template <int FN, int FT>
 struct F8Buf {
-  vu4 w[F8_ROWS / 16 * 64];
+  vu4 w[2 * FN * 64];
   vu4 x[2 * FT * 128];
-  uint32_t e[F8_ROWS];  // exponents
+  uint32_t e[256];  // exponents of the 32 FN rows
 };
-constexpr int F8_CUS = 256;
-template <typename O, int FT>
+template <typename O, int FN, int FT>
 __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int tiles_t) {
-  constexpr int BN = F8_ROWS, BT = 32 * FT, WN = 2, WT = 2, FN = 8, GN = BN / 16, GT = BT / 16;
-  constexpr int NEW = GN / 4 + FT + 1;  // copies of a wave per stage: 4 KB of weights, FT of hidden states, 64 exponents
-  static_assert(NEW <= 2 * FN, "one a step");
-  __shared__ F8Buf<FT> b0, b1, b2;
+  constexpr int WN = 2, WT = 2, GN = WN * FN, BN = 16 * GN, BT = 16 * WT * FT;
+  constexpr int SUB = F8_ROWS / BN;  // workgroups' tiles of a tile as it is packed
+  constexpr int NEW = GN / 4 + FT + 1;  // copies of a wave per stage: FN / 2 KB of weights, FT of hidden states, 64 exponents
+  constexpr int CP = (NEW + 2 * FN - 1) / (2 * FN);  // copies of a step
+  __shared__ F8Buf<FN, FT> b0, b1, b2;
   __shared__ Lse s_lse[std::is_void_v<O> ? WN : 1][std::is_void_v<O> ? BT : 1];
   const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), wn = wave / WT, wt = wave % WT;
   const int kb4 = a.lw.kb4, stages = 2 * a.lw.kb;
@@ -385,40 +386,44 @@ __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int t
   auto row_tile = [&](int id) { return (id >> 3) / tiles_t * 8 + (id & 7); };
   auto point = [&](int id) {
     const int tn = row_tile(id), tt = (id >> 3) % tiles_t;
-    pw = a.w + ((size_t)tn * stages * GN + 4 * wave) * F8_FRAG;
+    pw = a.w + ((size_t)(tn / SUB) * stages * GN * SUB + tn % SUB * GN + GN / 4 * wave) * F8_FRAG;
     px = a.x + ((size_t)tt * stages * 4 * FT + FT * wave) * 1024;
-    pe = a.w + a.lw.scales + (size_t)tn * kb4 * 4 * BN + 256 * wave;
+    pe = a.w + a.lw.scales + (size_t)(tn / SUB) * kb4 * 4 * F8_ROWS + (tn % SUB * BN + 64 * wave % BN) * 4;  // where BN is 128, twice
   };
-  auto copy = [&](int k, F8Buf<FT>& b, auto D) {  // copy D of stage k
+  auto copy = [&](int k, F8Buf<FN, FT>& b, auto D) {  // copy D of stage k
     constexpr int d = decltype(D)::value, xd = d - GN / 4;
     k = min(k, stages - 1);  // past the end: the last stage again, into a buffer that is not read any more
     if constexpr (d < GN / 4)
-      f8_copy<d * 1024>(pw + (size_t)k * (GN * F8_FRAG), o16, b.w + GN / 4 * wave * 64);
+      f8_copy<d * 1024>(pw + (size_t)k * (F8_ROWS / 16 * F8_FRAG), o16, b.w + GN / 4 * wave * 64);
     else if constexpr (d < NEW - 1)
       f8_copy<xd % 4 * 1024>(px + (size_t)k * (4 * FT * 1024) + xd / 4 * 4096, o16, b.x + (FT * wave + xd / 4 * 4) * 64);
     else if constexpr (d == NEW - 1)
-      f8_copy_words(pe + (size_t)(k / 8) * (4 * BN), o4, b.e + 64 * wave);
+      f8_copy_words(pe + (size_t)(k / 8) * (4 * F8_ROWS), o4, b.e + 64 * wave);
   };
   auto each = [&](auto f) {  // f(0) .. f(FN - 1), as constants
     [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>()), ...); }(std::make_integer_sequence<int, FN>());
   };
-  auto copy_all = [&](int k, F8Buf<FT>& b) {
-    each([&](auto I) {
-      copy(k, b, std::integral_constant<int, decltype(I)::value>());
-      copy(k, b, std::integral_constant<int, decltype(I)::value + FN>());
-    });
+  // step i of the first FN steps of a stage's copies, and of the others
+  auto copy_first = [&](int k, F8Buf<FN, FT>& b, auto I) {
+    copy(k, b, std::integral_constant<int, decltype(I)::value * CP>());
+    if constexpr (CP > 1) copy(k, b, std::integral_constant<int, decltype(I)::value * CP + 1>());
+  };
+  auto copy_others = [&](int k, F8Buf<FN, FT>& b, auto I) { copy_first(k, b, std::integral_constant<int, decltype(I)::value + FN>()); };
+  auto copy_all = [&](int k, F8Buf<FN, FT>& b) {
+    each([&](auto I) { copy_first(k, b, I); });
+    each([&](auto I) { copy_others(k, b, I); });
   };
   vu4 w[FN];
   uint32_t word[FN];
   f8_b8 x0[FT], x1[FT], q;
   vf4 acc[FN][FT];
-  auto read_x = [&](const F8Buf<FT>& b, int h, int j) { return __builtin_bit_cast(f8_b8, b.x[((wt * FT + j) * 2 + h) * 64 + lane]); };
-  auto read_w = [&](const F8Buf<FT>& b, int i) {
+  auto read_x = [&](const F8Buf<FN, FT>& b, int h, int j) { return __builtin_bit_cast(f8_b8, b.x[((wt * FT + j) * 2 + h) * 64 + lane]); };
+  auto read_w = [&](const F8Buf<FN, FT>& b, int i) {
     w[i] = b.w[(wn * FN + i) * 64 + lane];
     word[i] = b.e[16 * (wn * FN + i) + (lane & 15)];
   };
   // stage k in b; `next` holds the next one, `last` the one before (free; the copies of stage k + 2 go on into it)
-  auto stage = [&](int k, F8Buf<FT>& b, const F8Buf<FT>& next, F8Buf<FT>& last) {
+  auto stage = [&](int k, F8Buf<FN, FT>& b, const F8Buf<FN, FT>& next, F8Buf<FN, FT>& last) {
     const int kb = k >> 1, kn = (k + 1) >> 1;
     each([&](auto I) {
       constexpr int i = decltype(I)::value;
@@ -428,7 +433,7 @@ __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int t
       const f8_b8 qn = i + 1 < FN ? f8_wide<0>(w[(i + 1) % FN], f8_scale(word[(i + 1) % FN], kb)) : f8_wide<1>(w[0], f8_scale(word[0], kb));
 #pragma unroll
       for (int j = 0; j < FT; j++) acc[i][j] = f8_mfma(q, x0[j], acc[i][j]);
-      copy(k + 2, last, std::integral_constant<int, i + FN>());
+      copy_others(k + 2, last, I);
       q = qn;
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int t
       if (i + 1 == FN) qn = f8_wide<0>(w[0], f8_scale(word[0], kn));
 #pragma unroll
       for (int j = 0; j < FT; j++) acc[i][j] = f8_mfma(q, x1[j], acc[i][j]);
-      copy(k + 3, b, I);
+      copy_first(k + 3, b, I);
       q = qn;
       __builtin_amdgcn_sched_barrier(0);
     });
@@ -458,8 +463,8 @@ __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int t
   copy_all(1, b1);
   for (;;) {
     const int tn = row_tile(id), n0 = tn * BN, t0 = (id >> 3) % tiles_t * BT;
-    each([&](auto I) { copy(2, b2, I); });  // the others follow in the first half
-    f8_meet<NEW + FN>();
+    each([&](auto I) { copy_first(2, b2, I); });  // the others follow in the first half
+    f8_meet<NEW + (FN * CP < NEW ? FN * CP : NEW)>();
 #pragma unroll
     for (int i = 0; i < FN; i++) read_w(b0, i);
 #pragma unroll
@@ -545,22 +550,35 @@ int f8_pack(const void* x, long long stride, int rows, int K, F8Layout l, char* 
 }
 
 // What runs T hidden states against N weight rows: k_f8_few with `groups` row groups to a workgroup and `frags` fragments of
-// hidden states, or (groups = 0) k_f8_tile with `frags` fragments to a wave; the parts that scoring joins per hidden state.
+// hidden states, or (groups = 0) k_f8_tile with tiles of 32 fn x 32 frags; the parts that scoring joins per hidden state.
+// Measured (us of a scoring call at K = 5,120, N = 248,320, k_f8_few / k_f8_tile): 24 states 262 / 256, 64 states 382 / 267;
+// but where the tiles are fewer than half the CUs (N = 8,191, K = 1,000) 64 states 19 / 24.
 struct F8Plan {
-  int groups, frags, parts;
+  int groups, frags, fn, parts;
 };
 inline F8Plan f8_plan(int T, int N) {
   F8Plan p = {};
-  if (T <= 64) {
+  if (T <= 32 || (T <= 64 && N < 128 * F8_CUS / 2)) {
     p.frags = T <= 16 ? 1 : T <= 32 ? 2 : 4;
-    // one group to a workgroup where the card would not be full of four
-    p.groups = f8_up(N, 64) / 64 < 512 ? 1 : p.frags == 4 ? 2 : 4;
+    p.groups = p.frags == 4 ? 2 : 4;
     p.parts = f8_up(N, 16 * p.groups) / (16 * p.groups);
-  } else {
-    const int tiles = (T + 255) / 256;
-    p.frags = ((T + tiles - 1) / tiles + 31) / 32;
-    p.parts = f8_up(N, F8_ROWS) / F8_ROWS;
+    return p;
   }
+  // The least rounds of workgroups times a tile's time: its products, per fragment of weights their widening, and a constant
+  // (512 states: tiles of 256 x 256 965 us, 128 x 256 1,080, 256 x 128 1,063; 300: 256 x 160 654, 256 x 128 796; 77 states
+  // at N = 32,001, K = 1,280: 128 x 96 27, 256 x 96 33).
+  long long best = 0;
+  for (int fn = 8; fn >= 4; fn -= 4)
+    for (int frags = 8; frags >= 3; frags--) {
+      const long long tiles = (long long)(f8_up(N, 32 * fn) / (32 * fn)) * (f8_up(T, 32 * frags) / (32 * frags));
+      const long long cost = (tiles + F8_CUS - 1) / F8_CUS * (fn * (4 * frags + 3) + 38);
+      if (p.fn == 0 || cost < best) {
+        best = cost;
+        p.fn = fn;
+        p.frags = frags;
+      }
+    }
+  p.parts = f8_up(N, 32 * p.fn) / (32 * p.fn);
   return p;
 }
 // the packed hidden states: a workgroup's are a tile, 8-bit or (k_f8_tile) bf16
@@ -626,34 +644,39 @@ template <typename O, int G, int TF>
 static void f8_few(const F8Args& a, hipStream_t st) {
   hipLaunchKernelGGL((k_f8_few<O, G, TF>), dim3((a.N + 16 * G - 1) / (16 * G)), dim3(256), 0, st, a);
 }
-template <typename O, int FT>
+template <typename O, int FN, int FT>
 static void f8_tile(const F8Args& a, hipStream_t st) {
-  const int tn = (a.N + F8_ROWS - 1) / F8_ROWS, tt = (a.T + 32 * FT - 1) / (32 * FT);
-  const int total = (tn + 7) / 8 * 8 * tt;
-  hipLaunchKernelGGL((k_f8_tile<O, FT>), dim3(total < F8_CUS ? total : F8_CUS), dim3(256), 0, st, a, tn, tt);
+  const int tn = f8_up(a.N, 32 * FN) / (32 * FN), tt = f8_up(a.T, 32 * FT) / (32 * FT);
+  const long long total = (long long)((tn + 7) / 8 * 8) * tt;
+  hipLaunchKernelGGL((k_f8_tile<O, FN, FT>), dim3(total < F8_CUS ? (int)total : F8_CUS), dim3(256), 0, st, a, tn, tt);
+}
+template <typename O, int FN>
+static void f8_tiles(const F8Args& a, int frags, hipStream_t st) {
+  switch (frags) {
+    case 3: return f8_tile<O, FN, 3>(a, st);
+    case 4: return f8_tile<O, FN, 4>(a, st);
+    case 5: return f8_tile<O, FN, 5>(a, st);
+    case 6: return f8_tile<O, FN, 6>(a, st);
+    case 7: return f8_tile<O, FN, 7>(a, st);
+    default: return f8_tile<O, FN, 8>(a, st);
+  }
 }
 // packs the hidden states and runs the product
 template <typename O>
 static int f8_product(F8Args a, int K, const void* x, long long x_stride, char* ws, hipStream_t st) {
   const F8Plan p = f8_plan(a.T, a.N);
   a.parts = p.parts;
+  if (p.groups == 0 && (long long)(p.parts + 7) * (f8_up(a.T, 32 * p.frags) / (32 * p.frags)) > 0x7FFF0000) return QWS_ERR_NOT_SUPPORTED;
   const int e = p.groups ? f8_pack<uint16_t, false>(x, x_stride, a.T, K, a.lx, ws, st) : f8_pack<uint16_t, true>(x, x_stride, a.T, K, a.lx, ws, st);
   if (e) return e;
-  if (p.groups == 0) {
-    switch (p.frags) {
-      case 3: f8_tile<O, 3>(a, st); break;
-      case 4: f8_tile<O, 4>(a, st); break;
-      case 5: f8_tile<O, 5>(a, st); break;
-      case 6: f8_tile<O, 6>(a, st); break;
-      case 7: f8_tile<O, 7>(a, st); break;
-      default: f8_tile<O, 8>(a, st);
-    }
-  } else if (p.frags == 1)
-    p.groups == 1 ? f8_few<O, 1, 1>(a, st) : f8_few<O, 4, 1>(a, st);
+  if (p.groups == 0)
+    p.fn == 8 ? f8_tiles<O, 8>(a, p.frags, st) : f8_tiles<O, 4>(a, p.frags, st);
+  else if (p.frags == 1)
+    f8_few<O, 4, 1>(a, st);
   else if (p.frags == 2)
-    p.groups == 1 ? f8_few<O, 1, 2>(a, st) : f8_few<O, 4, 2>(a, st);
+    f8_few<O, 4, 2>(a, st);
   else
-    p.groups == 1 ? f8_few<O, 1, 4>(a, st) : f8_few<O, 2, 4>(a, st);
+    f8_few<O, 2, 4>(a, st);
   return (int)hipGetLastError();
 }
 }  // namespace qws

@@ -2,6 +2,7 @@
 qws_logprobs) on torch tensors."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import NamedTuple, Optional
 
@@ -24,10 +25,13 @@ class LogProbsResult(NamedTuple):
 
 def rows_of(x: torch.Tensor, name: str):
     """(rows, stride) of a tensor [..., n] read as rows of n contiguous elements at one stride."""
-    if x.dim() < 2 or (x.shape[-1] > 1 and x.stride(-1) != 1):
+    shape, strides = x.shape, x.stride()
+    if len(shape) < 2 or (shape[-1] > 1 and strides[-1] != 1):
         raise ValidationError(f"{name} must be [..., n] with contiguous rows", name)
+    if len(shape) == 2:
+        return shape[0], strides[0] if shape[0] > 1 else 0
     rows, stride = 1, 0
-    for size, step in zip(reversed(x.shape[:-1]), reversed(x.stride()[:-1])):
+    for size, step in zip(reversed(shape[:-1]), reversed(strides[:-1])):
         if size == 1:
             continue
         if rows == 1:
@@ -39,8 +43,19 @@ def rows_of(x: torch.Tensor, name: str):
 
 
 def given(t: torch.Tensor, shape, dtype, device, name: str):
-    if t.dtype != dtype or t.device != device or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.dtype != dtype or t.device != device or t.shape != shape or not t.is_contiguous():
         raise ValidationError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}", name)
+
+
+def on_stream(index: int):
+    """(a context that makes GPU `index` the current one, its current stream's handle).  These calls are small next to the
+    kernels they start only if the host is quick: the context is left out where nothing changes, and the handle comes without
+    a stream object (2 us)."""
+    same = torch._C._cuda_getDevice() == index
+    return NOTHING if same else torch.cuda.device(index), torch._C._cuda_getCurrentRawStream(index)
+
+
+NOTHING = contextlib.nullcontext()
 
 
 class LogProbs:
@@ -57,34 +72,49 @@ class LogProbs:
     def __init__(self, device="cuda"):
         self.lib = _lib.load()
         self.device = torch.device(device)
+        self._ws_bytes = {}
 
     def __call__(self, logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0, temperature: Optional[torch.Tensor] = None,
                  ranks: bool = True) -> LogProbsResult:
-        if logits.device.type != "cuda" or logits.dtype not in (torch.float32, torch.bfloat16):
+        dtype, dev = logits.dtype, logits.device
+        if not logits.is_cuda or (dtype != torch.float32 and dtype != torch.bfloat16):
             raise ValidationError("logits must be a CUDA fp32 / bf16 tensor", "logits")
         R, stride = rows_of(logits, "logits")
-        lead, V, dev = logits.shape[:-1], logits.shape[-1], logits.device
-        top = int(top)
+        lead, V, top = logits.shape[:-1], logits.shape[-1], int(top)
         if V < 1 or not 0 <= top <= LOGPROBS_MAX:
             raise ValidationError(f"top must be in [0, {LOGPROBS_MAX}]", "top", top)
-        M = 0
+        M, lp, rk = 0, None, None
         if tokens is not None:
-            M = 1 if tokens.dim() < logits.dim() else tokens.shape[-1]
-            if not 1 <= M <= LOGPROBS_MAX:
-                raise ValidationError(f"at most {LOGPROBS_MAX} tokens a row", "tokens", M)
-            given(tokens, lead if tokens.dim() < logits.dim() else (*lead, M), torch.int32, dev, "tokens")
+            shape = lead
+            M = 1
+            if tokens.dim() > len(lead):
+                M = tokens.shape[-1]
+                shape = (*lead, M)
+                if not 1 <= M <= LOGPROBS_MAX:
+                    raise ValidationError(f"at most {LOGPROBS_MAX} tokens a row", "tokens", M)
+            given(tokens, shape, torch.int32, dev, "tokens")
         if temperature is not None:
             given(temperature, lead, torch.float32, dev, "temperature")
-        with torch.cuda.device(dev):
-            lp = torch.empty(tokens.shape, dtype=torch.float32, device=dev) if M else None
-            rk = torch.empty(tokens.shape, dtype=torch.int32, device=dev) if M and ranks else None
+        where, stream = on_stream(dev.index)
+        with where:
+            if M:
+                lp = torch.empty(shape, dtype=torch.float32, device=dev)
+                if ranks:
+                    rk = torch.empty_like(tokens)
             h = torch.empty(lead, dtype=torch.float32, device=dev)
             ids = torch.empty((*lead, top), dtype=torch.int32, device=dev)
             tlp = torch.empty((*lead, top), dtype=torch.float32, device=dev)
             if R:
-                dt = _lib.DTYPE_F32 if logits.dtype == torch.float32 else _lib.DTYPE_BF16
-                ptr = lambda t: t.data_ptr() if t is not None and t.numel() else None  # noqa: E731
-                b = _lib.LogprobsBatch(logits.data_ptr(), dt, R, V, stride, ptr(tokens), M, top, ptr(temperature), ptr(lp), ptr(rk), ptr(h), ptr(ids), ptr(tlp))
-                ws = torch.empty(self.lib.qws_logprobs_ws_bytes(dt, R, V, M, top), dtype=torch.uint8, device=dev)
-                check(self.lib.qws_logprobs(C.byref(b), ws.data_ptr(), ws.numel(), C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)), "qws_logprobs")
+                dt = _lib.DTYPE_F32 if dtype == torch.float32 else _lib.DTYPE_BF16
+                key = (dt, R, V, M, top)
+                n = self._ws_bytes.get(key)
+                if n is None:
+                    n = self._ws_bytes[key] = self.lib.qws_logprobs_ws_bytes(*key)
+                ws = torch.empty(n, dtype=torch.uint8, device=dev)
+                b = _lib.LogprobsBatch(logits.data_ptr(), dt, R, V, stride, tokens.data_ptr() if M else None, M, top,
+                                       temperature.data_ptr() if temperature is not None else None, lp.data_ptr() if M else None,
+                                       rk.data_ptr() if rk is not None else None, h.data_ptr(), ids.data_ptr() if top else None, tlp.data_ptr() if top else None)
+                err = self.lib.qws_logprobs(C.byref(b), ws.data_ptr(), n, stream)
+                if err:
+                    check(err, "qws_logprobs")
         return LogProbsResult(lp, rk, h, ids, tlp)
