@@ -65,8 +65,19 @@ __device__ __forceinline__ f8_b8 f8_wide(vu4 r, float scale) {
   return u.v;
 }
 
-// One wave per block of 16 rows: lane l takes row l % 16, values 16 (l / 16) .. + 15 of both fragments.  A value that is not
-// finite becomes NaN, the one such value that e4m3 has.
+// The biased exponent of a block whose largest magnitude is `most` (as bits): 448 = 1.75 * 2^8, so the value's own less 8, one
+// more where its fraction is above .75; at least 0 (2^-127)
+__device__ __forceinline__ int f8_exponent(uint32_t most) { return max((int)(most >> 23) - 8 + ((most & 0x7FFFFFu) > 0x600000u ? 1 : 0), 0); }
+// four values over the block's scale, rounded to e4m3; one that is not finite becomes NaN, the only such value it has
+__device__ __forceinline__ uint32_t f8_four(const float* v, int e) {
+  const float up = __uint_as_float((uint32_t)(254 - e) << 23);  // 2^(127 - e)
+  float f[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) f[i] = fabsf(v[i]) <= F32_MAX ? v[i] * up : NAN;
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false), true);
+}
+
+// One wave per block of 16 rows: lane l takes row l % 16, values 16 (l / 16) .. + 15 of both fragments.
 //   WIDE: the values as bf16 instead (exact), as k_f8_tile takes hidden states: product h of fragment c is 1 KB of its own.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) k_f8_pack(const T* x, long long stride, int rows, int K, F8Layout l, char* out) {
@@ -107,18 +118,11 @@ __global__ void __launch_bounds__(256) k_f8_pack(const T* x, long long stride, i
   for (int j = 0; j < 32; j++) most = max(most, __float_as_uint(v[j]) & 0x7FFFFFFFu);
   most = max(most, (uint32_t)__shfl_xor((int)most, 16));
   most = max(most, (uint32_t)__shfl_xor((int)most, 32));
-  // 448 = 1.75 * 2^8: biased exponent of the block, one more where the fraction is above .75; at least 0 (2^-127)
-  const int e = max((int)(most >> 23) - 8 + ((most & 0x7FFFFFu) > 0x600000u ? 1 : 0), 0);
+  const int e = f8_exponent(most);
   if (WIDE && kb >= l.kb) return;
-  const float up = __uint_as_float((uint32_t)(254 - e) << 23);  // 2^(127 - e)
   uint32_t q[8];
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    float f[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) f[i] = fabsf(v[4 * j + i]) <= F32_MAX ? v[4 * j + i] * up : NAN;
-    q[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false), true);
-  }
+  for (int j = 0; j < 8; j++) q[j] = f8_four(v + 4 * j, e);
   const size_t place = ((size_t)(group / l.groups) * l.kb + kb) * 2 * l.groups + group % l.groups;  // fragment 0 of the block; fragment 1: + l.groups
   if constexpr (WIDE) {
     const float scale = __uint_as_float((uint32_t)e << 23);
@@ -143,9 +147,10 @@ __global__ void __launch_bounds__(256) k_f8_pack(const T* x, long long stride, i
 
 struct F8Args {
   const char* w;   // packed weights
-  const char* x;   // packed hidden states
+  const char* x;   // packed hidden states, or the hidden states themselves
   F8Layout lw, lx;
-  int N, T;
+  int N, T, K;
+  long long x_stride;  // hidden states as they came: elements
   void* out;       // logits: fp32 or bf16 [T][out_stride], or null
   long long out_stride;
   const int* tok;  // scoring
@@ -244,10 +249,17 @@ using f8_out = std::conditional_t<std::is_void_v<O>, float, O>;
 
 // Few hidden states (T <= 16 TF): the weights' bytes bound it.  A workgroup takes G groups of 16 weight rows, its 4 waves a
 // quarter of K each, straight from memory into registers, one block ahead; their sums meet in LDS.
-template <typename O, int G, int TF>
-__global__ void __launch_bounds__(256) k_f8_few(F8Args a) {
-  __shared__ vf4 s_acc[4][G * TF][64];
-  __shared__ Lse s_lse[G][16 * TF];
+//   RAW (TF = 1): the hidden states as they came, 16-byte aligned vectors of 8; each workgroup rounds them into LDS itself,
+//   under its first loads of weights, which for a few KB takes less than a launch of k_f8_pack.
+template <int G, int TF>
+constexpr int f8_sums() { return 4 * G * TF * 64 * (int)sizeof(vf4); }
+__host__ __device__ inline int f8_raw_row(int kb) { return kb * F8_KB + 16; }  // bytes of a row in LDS: rows start in other banks
+__host__ __device__ inline int f8_raw_bytes(int T, int kb) { return T * (f8_raw_row(kb) + kb * 4); }
+template <typename O, int G, int TF, bool RAW>
+__global__ void __launch_bounds__(256, RAW ? 4 : 1) k_f8_few(F8Args a) {
+  extern __shared__ __attribute__((aligned(16))) char s_mem[];  // the rounded hidden states, then the sums
+  vf4(*s_acc)[G * TF][64] = (vf4(*)[G * TF][64])s_mem;
+  __shared__ Lse s_lse[std::is_void_v<O> ? G : 1][16 * TF];
   const int lane = lane_id(), wave = wave_id(), g0 = blockIdx.x * G;
   const int kb = a.lw.kb, kb4 = a.lw.kb4, per = (kb + 3) / 4, lo = wave * per, hi = min(lo + per, kb);
   constexpr int WG = F8_ROWS / 16;  // groups of a tile; G divides it
@@ -255,24 +267,67 @@ __global__ void __launch_bounds__(256) k_f8_few(F8Args a) {
   const char* px = a.x + 16 * lane;
   const uint32_t* qw = (const uint32_t*)(a.w + a.lw.scales) + ((size_t)(g0 / WG) * kb4 * WG + g0 % WG) * 16 + (lane & 15);
   const uint32_t* qx = (const uint32_t*)(a.x + a.lx.scales) + (lane & 15);
+  const int rs = f8_raw_row(kb), mine = min(lane & 15, a.T - 1);  // RAW: a lane without a row reads the last one, as zeros
+  const char* rx = s_mem + mine * rs + 16 * (lane >> 4);
+  float* rscale = (float*)(s_mem + a.T * rs);
   vf4 acc[G][TF] = {};
   vu4 w[G][2], x[TF][2];
   uint32_t ew[G], ex[TF];
-  auto load = [&](int k) {
+  auto load_w = [&](int k) {
 #pragma unroll
     for (int g = 0; g < G; g++)
 #pragma unroll
       for (int h = 0; h < 2; h++) w[g][h] = *gmem((const vu4*)(pw + ((size_t)(2 * k + h) * WG + g) * F8_FRAG));
 #pragma unroll
-    for (int j = 0; j < TF; j++)
-#pragma unroll
-      for (int h = 0; h < 2; h++) x[j][h] = *gmem((const vu4*)(px + ((size_t)(2 * k + h) * TF + j) * F8_FRAG));
-#pragma unroll
     for (int g = 0; g < G; g++) ew[g] = *gmem(qw + ((size_t)(k / 4) * WG + g) * 16);
-#pragma unroll
-    for (int j = 0; j < TF; j++) ex[j] = *gmem(qx + ((size_t)(k / 4) * TF + j) * 16);
   };
-  if (lo < hi) load(lo);
+  auto load_x = [&](int k) {
+    if constexpr (RAW) {
+      const bool row = (lane & 15) < a.T;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        x[0][h] = *(const vu4*)(rx + k * F8_KB + h * 64);
+        if (!row) x[0][h] = (vu4){0, 0, 0, 0};
+      }
+      ex[0] = __float_as_uint(rscale[mine * kb + k]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < TF; j++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) x[j][h] = *gmem((const vu4*)(px + ((size_t)(2 * k + h) * TF + j) * F8_FRAG));
+#pragma unroll
+      for (int j = 0; j < TF; j++) ex[j] = *gmem(qx + ((size_t)(k / 4) * TF + j) * 16);
+    }
+  };
+  auto load = [&](int k) {
+    load_w(k);
+    load_x(k);
+  };
+  if constexpr (RAW) {
+    if (lo < hi) load_w(lo);
+    // 16 lanes take a block, 8 values each
+    for (int u = threadIdx.x; u < a.T * kb * 16; u += 256) {
+      const int row = u / (kb * 16), k0 = u % (kb * 16) * 8;
+      vu4 r = {};
+      if (k0 < a.K) r = *gmem((const vu4*)((const uint16_t*)a.x + (long long)row * a.x_stride + k0));
+      float v[8];
+      uint32_t most = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        v[i] = __uint_as_float(i & 1 ? r[i / 2] & 0xFFFF0000u : r[i / 2] << 16);
+        most = max(most, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+      }
+      most = max8(most);
+      most = max(most, dpp_perm<0x140>(most));  // row_mirror: the other eight lanes
+      const int e = f8_exponent(most);
+      *(uint2*)(s_mem + row * rs + k0) = make_uint2(f8_four(v, e), f8_four(v + 4, e));
+      if ((lane & 15) == 0) rscale[row * kb + k0 / F8_KB] = __uint_as_float((uint32_t)e << 23);
+    }
+    bar();
+    if (lo < hi) load_x(lo);
+  } else {
+    if (lo < hi) load(lo);
+  }
   for (int k = lo; k < hi; k++) {
     vu4 cw[G][2], cx[TF][2];
     float sw[G], sx[TF];
@@ -286,7 +341,7 @@ __global__ void __launch_bounds__(256) k_f8_few(F8Args a) {
     for (int j = 0; j < TF; j++) {
       cx[j][0] = x[j][0];
       cx[j][1] = x[j][1];
-      sx[j] = f8_scale(ex[j], k);
+      sx[j] = RAW ? __uint_as_float(ex[j]) : f8_scale(ex[j], k);
     }
     load(min(k + 1, hi - 1));
 #pragma unroll
@@ -305,6 +360,7 @@ __global__ void __launch_bounds__(256) k_f8_few(F8Args a) {
       }
     }
   }
+  if constexpr (RAW) bar();  // the sums take the hidden states' place
 #pragma unroll
   for (int g = 0; g < G; g++)
 #pragma unroll
@@ -581,6 +637,12 @@ inline F8Plan f8_plan(int T, int N) {
   p.parts = f8_up(N, 32 * p.fn) / (32 * p.fn);
   return p;
 }
+// Whether each workgroup of k_f8_few rounds the hidden states itself: up to 20,480 values (us with / without, K = 5,120:
+// one state at N = 248,320 222 / 226, at N = 64,000 59 / 62, four 65 / 66, five 66.2 / 65.8; sixteen 552 / 241).
+constexpr int F8_RAW = 20480;
+inline bool f8_raw(int T, int K, const void* x, long long stride) {
+  return T <= 16 && K % 8 == 0 && ((uintptr_t)x & 15) == 0 && (T == 1 || stride % 8 == 0) && T * f8_up(K, F8_KB) <= F8_RAW;
+}
 // the packed hidden states: a workgroup's are a tile, 8-bit or (k_f8_tile) bf16
 inline F8Layout f8_states(int T, int N, int K) {
   const F8Plan p = f8_plan(T, N);
@@ -638,11 +700,13 @@ static F8Args f8_args(const void* packed, int N, int K, int T, const void* ws) {
   a.lx = f8_states(T, N, K);
   a.N = N;
   a.T = T;
+  a.K = K;
   return a;
 }
-template <typename O, int G, int TF>
+template <typename O, int G, int TF, bool RAW>
 static void f8_few(const F8Args& a, hipStream_t st) {
-  hipLaunchKernelGGL((k_f8_few<O, G, TF>), dim3((a.N + 16 * G - 1) / (16 * G)), dim3(256), 0, st, a);
+  const int raw = RAW ? f8_raw_bytes(a.T, a.lw.kb) : 0, sums = f8_sums<G, TF>();
+  hipLaunchKernelGGL((k_f8_few<O, G, TF, RAW>), dim3((a.N + 16 * G - 1) / (16 * G)), dim3(256), raw > sums ? raw : sums, st, a);
 }
 template <typename O, int FN, int FT>
 static void f8_tile(const F8Args& a, hipStream_t st) {
@@ -667,16 +731,22 @@ static int f8_product(F8Args a, int K, const void* x, long long x_stride, char* 
   const F8Plan p = f8_plan(a.T, a.N);
   a.parts = p.parts;
   if (p.groups == 0 && (long long)(p.parts + 7) * (f8_up(a.T, 32 * p.frags) / (32 * p.frags)) > 0x7FFF0000) return QWS_ERR_NOT_SUPPORTED;
+  if (f8_raw(a.T, K, x, x_stride)) {
+    a.x = (const char*)x;
+    a.x_stride = x_stride;
+    f8_few<O, 4, 1, true>(a, st);
+    return (int)hipGetLastError();
+  }
   const int e = p.groups ? f8_pack<uint16_t, false>(x, x_stride, a.T, K, a.lx, ws, st) : f8_pack<uint16_t, true>(x, x_stride, a.T, K, a.lx, ws, st);
   if (e) return e;
   if (p.groups == 0)
     p.fn == 8 ? f8_tiles<O, 8>(a, p.frags, st) : f8_tiles<O, 4>(a, p.frags, st);
   else if (p.frags == 1)
-    f8_few<O, 4, 1>(a, st);
+    f8_few<O, 4, 1, false>(a, st);
   else if (p.frags == 2)
-    f8_few<O, 4, 2>(a, st);
+    f8_few<O, 4, 2, false>(a, st);
   else
-    f8_few<O, 2, 4>(a, st);
+    f8_few<O, 2, 4, false>(a, st);
   return (int)hipGetLastError();
 }
 }  // namespace qws

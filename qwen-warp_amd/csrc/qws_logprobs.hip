@@ -166,6 +166,85 @@ __device__ __forceinline__ void lp_slow(Lse& v, const float (&x)[U][E], float be
     }
 }
 
+// The selections of a row's workgroup.  A key is a value's order and its place (comp): larger = earlier.
+struct LpSel {
+  uint64_t col[LP_NW][64], best[64], thr;
+  int rank[64], n;
+  int win[64];
+};
+// The n-th largest (n <= 64) of the 64 lanes' best values (order keys, 0 = none), each over the lane of every wave; 0 when
+// fewer lanes have one: a lower bound of the workgroup's n-th largest value.  Clears s.n; every wave gets it without a second
+// barrier, by bisection over the key's bits.  Ends with a barrier before lp_take's first use of s.n.
+__device__ __forceinline__ uint32_t lp_bound(uint32_t mine, int n, LpSel& s) {
+  uint32_t* col = (uint32_t*)s.col;
+  bar();
+  col[threadIdx.x] = mine;
+  if (threadIdx.x == 0) s.n = 0;
+  bar();
+#pragma unroll
+  for (int w = 0; w < LP_NW; w++) mine = max(mine, col[64 * w + lane_id()]);
+  uint32_t t = 0;
+#pragma unroll 1
+  for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
+    if (__popcll(__ballot(mine >= (t | bit))) >= n) t |= bit;
+  return t;
+}
+// The same over whole keys (distinct, 0 = none): no more of them than lp_list are at or above it, however many values tie.
+__device__ inline uint64_t lp_threshold(uint64_t mine, int n, LpSel& s) {
+  const int lane = lane_id(), wave = wave_id();
+  bar();
+  s.col[wave][lane] = mine;
+  if (wave == 0) s.rank[lane] = 0;
+  if (threadIdx.x == 0) s.thr = 0, s.n = 0;
+  bar();
+#pragma unroll
+  for (int w = 0; w < LP_NW; w++) mine = max(mine, s.col[w][lane]);
+  if (wave == 0) s.best[lane] = mine;
+  bar();
+  int above = 0;
+#pragma unroll
+  for (int j = 0; j < 64 / LP_NW; j++) above += s.best[wave * (64 / LP_NW) + j] > mine;
+  atomicAdd(&s.rank[lane], above);
+  bar();
+  if (wave == 0 && mine && s.rank[lane] == n - 1) s.thr = mine;
+  bar();
+  return s.thr;
+}
+__device__ __forceinline__ void lp_take(uint64_t k, uint64_t thr, LpSel& s, uint64_t* list) {
+  if (k && k >= thr) list[atomicAdd(&s.n, 1)] = k;
+}
+// calls put(rank, key) for every key of the list that is among its n best (after a barrier behind the list's last write)
+template <typename F>
+__device__ __forceinline__ void lp_ranked(LpSel& s, const uint64_t* list, int n, F put) {
+  const int c = s.n, lane = lane_id(), wave = wave_id();
+  if (c <= 64) {  // each wave compares the lanes' keys with a quarter of the list
+    if (wave == 0) s.rank[lane] = 0;
+    bar();
+    const uint64_t k = lane < c ? list[lane] : 0;
+    const int q = (c + LP_NW - 1) / LP_NW, hi = min((wave + 1) * q, c);
+    int r = 0;
+#pragma unroll 4
+    for (int j = wave * q; j < hi; j++) r += list[j] > k;
+    atomicAdd(&s.rank[lane], r);
+    bar();
+    if (wave == 0 && lane < c && s.rank[lane] < n) put(s.rank[lane], k);
+    return;
+  }
+  for (int i = threadIdx.x; i < c; i += LP_NT) {
+    const uint64_t k = list[i];
+    int r = 0;
+#pragma unroll 4
+    for (int j = 0; j < c; j++) r += list[j] > k;
+    if (r < n) put(r, k);
+  }
+}
+// Keys that a selection of the n best can list: those of the n lanes whose best are the n largest
+inline size_t lp_list(int groups, int n) {
+  const int a = n * ((groups + 63) / 64) < groups ? n * ((groups + 63) / 64) : groups, b = n < 64 ? (n > 8 ? n * n : 64) : n * 64;
+  return (size_t)(a > b ? a : b);
+}
+__device__ __forceinline__ uint32_t lp_value(float x) { return x > -INFINITY ? okey(x) : 0; }
+
 // RANK: 0 no given tokens' ranks, 1 one token per row (held in registers), 2 several (in LDS).  U vectors of a thread make a
 // block: loaded together, one step of the running maximum.
 template <typename T, int RANK, bool TOP, int U>
@@ -180,7 +259,19 @@ __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
   const int lead = (int)((uintptr_t)p / sizeof(T)) & (E - 1), end = lead + a.V;
   const T* base = p - lead;
   const float c = lse_scale(a.temp ? a.temp[row] : 1.0f);
-  const int nstripes = (end + SE - 1) / SE, s_end = min((ch + 1) * a.per, nstripes);
+  const int nstripes = (end + SE - 1) / SE, s_begin = ch * a.per, s_end = min(s_begin + a.per, nstripes);
+  vu4 r[U];
+  auto load = [&](int s) {
+    const int first = s * SE;
+    if (first >= lead && first + U * SE <= end && s + U <= s_end) {
+#pragma unroll
+      for (int u = 0; u < U; u++) r[u] = __builtin_nontemporal_load((const QWS_G vu4*)(base + first + u * SE + tid * E));  // read once
+    } else {  // past the row's end, or into the next workgroup's stripes: nothing
+#pragma unroll
+      for (int u = 0; u < U; u++) r[u] = lp_load_edge(base, first + u * SE + tid * E, s + u < s_end ? lead : end, end);
+    }
+  };
+  if constexpr (U == 1) load(s_begin);  // the one block, before the given tokens' two loads in a row
   float xt = 0.0f;
   int tv = -1, cnt = 0;  // virtual position of the token (-1: skipped), logits before it
   bool moderate = c <= LSE_MOST;  // no given token's logit is extreme
@@ -206,17 +297,10 @@ __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
   Lse v = {-INFINITY, 0.0f, 0.0f};
   LpFast f = {-INFINITY, -1e30f, -INFINITY, 0.0f, 0.0f};
   char* gmax = (char*)(a.gmax + (long long)row * a.groups);
-  for (int s = ch * a.per; s < s_end; s += U) {
-    float top[U];
-    vu4 r[U];
+  for (int s = s_begin; s < s_end; s += U) {
     const int first = s * SE;
-    if (first >= lead && first + U * SE <= end && s + U <= s_end) {
-#pragma unroll
-      for (int u = 0; u < U; u++) r[u] = __builtin_nontemporal_load((const QWS_G vu4*)(base + first + u * SE + tid * E));  // read once
-    } else {  // past the row's end, or into the next workgroup's stripes: nothing
-#pragma unroll
-      for (int u = 0; u < U; u++) r[u] = lp_load_edge(base, first + u * SE + tid * E, s + u < s_end ? lead : end, end);
-    }
+    if constexpr (U != 1) load(s);
+    float top[U];
     float x[U][E], best = -INFINITY, least = INFINITY;
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -274,7 +358,7 @@ __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
       }
     }
   }
-  v = lse_join_lanes(lse_join(v, lp_fast_end(f, c), c), c, 1, 32);
+  v = lse_join_wave(lse_join(v, lp_fast_end(f, c), c), c);
   if constexpr (RANK == 1) {
     if (tid == 0) s_cnt[0] = 0;
     bar();
@@ -291,84 +375,38 @@ __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
     if (tid < (RANK == 1 ? 1 : a.M)) a.cnt[o * a.M + tid] = s_cnt[tid];
 }
 
-struct LpSel {
-  uint64_t col[LP_NW][64], best[64], thr;
-  int rank[64], n;
-  int win[LP_NMAX];
-};
-// A lower bound of the block's n-th largest key (n <= 64; keys distinct, 0 = none): the n-th largest of the 64 lanes' best
-// keys, each over the lane of every wave.  0 when fewer lanes have a key.  Clears s.n; ends with a barrier.
-__device__ inline uint64_t lp_threshold(uint64_t mine, int n, LpSel& s) {
-  const int lane = lane_id(), wave = wave_id();
-  bar();
-  s.col[wave][lane] = mine;
-  if (wave == 0) s.rank[lane] = 0;
-  if (threadIdx.x == 0) s.thr = 0, s.n = 0;
-  bar();
-#pragma unroll
-  for (int w = 0; w < LP_NW; w++) mine = max(mine, s.col[w][lane]);
-  if (wave == 0) s.best[lane] = mine;
-  bar();
-  int above = 0;
-#pragma unroll
-  for (int j = 0; j < 64 / LP_NW; j++) above += s.best[wave * (64 / LP_NW) + j] > mine;
-  atomicAdd(&s.rank[lane], above);
-  bar();
-  if (wave == 0 && mine && s.rank[lane] == n - 1) s.thr = mine;
-  bar();
-  return s.thr;
-}
-__device__ __forceinline__ void lp_take(uint64_t k, uint64_t thr, LpSel& s, uint64_t* list) {
-  if (k && k >= thr) list[atomicAdd(&s.n, 1)] = k;
-}
-// calls put(rank, key) for every key of the list that is among its n best (after a barrier behind lp_take)
-template <typename F>
-__device__ __forceinline__ void lp_ranked(LpSel& s, const uint64_t* list, int n, F put) {
-  const int c = s.n, lane = lane_id(), wave = wave_id();
-  if (c <= 64) {  // each wave compares the lanes' keys with a quarter of the list
-    if (wave == 0) s.rank[lane] = 0;
-    bar();
-    const uint64_t k = lane < c ? list[lane] : 0;
-    const int q = (c + LP_NW - 1) / LP_NW, hi = min((wave + 1) * q, c);
-    int r = 0;
-#pragma unroll 4
-    for (int j = wave * q; j < hi; j++) r += list[j] > k;
-    atomicAdd(&s.rank[lane], r);
-    bar();
-    if (wave == 0 && lane < c && s.rank[lane] < n) put(s.rank[lane], k);
-    return;
-  }
-  for (int i = threadIdx.x; i < c; i += LP_NT) {
-    const uint64_t k = list[i];
-    int r = 0;
-#pragma unroll 4
-    for (int j = 0; j < c; j++) r += list[j] > k;
-    if (r < n) put(r, k);
-  }
-}
-
-// KPT: groups of a thread at most (0: no alternatives), all loaded at once
-template <typename T, int KPT>
+// A row's second stage: joins its parts, writes the given tokens' results and the entropy, and selects the
+// alternatives.  Both selections first take the values at or above lp_bound, which are few where values differ: up to 64
+// groups are all looked through, whether among the n best or not, and up to 64 logits are ranked.  Where more are (ties, or
+// n near 64), keys with their places decide.
+template <typename T, bool TOP>
 __global__ void __launch_bounds__(LP_NT) k_lp_row(LpArgs a) {
-  constexpr int E = lp_e<T>();
-  extern __shared__ uint64_t list[];  // lp_list(groups, top) keys
   __shared__ LpSel s;
   __shared__ Lse s_lse[LP_NW];
+  extern __shared__ uint64_t list[];  // lp_list(groups, top) keys
+  constexpr int E = lp_e<T>(), KPT = 16;  // groups of a thread that are held in registers: all, up to V = 262,144
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), row = blockIdx.x;
   const T* p = (const T*)a.x + (long long)row * a.stride;
   const int lead = (int)((uintptr_t)p / sizeof(T)) & (E - 1), end = lead + a.V;
   const int ng = (end + LP_GRP - 1) / LP_GRP;
   const float* gm = a.gmax + (long long)row * a.groups;
-  float gv[KPT ? KPT : 1];
+  float gv[TOP ? KPT : 1];
+  auto load_groups = [&](int g0) {
 #pragma unroll
-  for (int i = 0; i < KPT; i++) gv[i] = *gmem(gm + min(i * LP_NT + tid, ng - 1));
+    for (int i = 0; i < KPT; i++) {
+      const int g = g0 + i * LP_NT + tid;
+      const float x = *gmem(gm + min(g, ng - 1));
+      gv[i] = g < ng ? x : -INFINITY;
+    }
+  };
+  if constexpr (TOP) load_groups(0);
   const float temp = a.temp ? a.temp[row] : 1.0f, c = lse_scale(temp);
   Lse v = {-INFINITY, 0.0f, 0.0f};
   for (int g = tid; g < a.G; g += LP_NT) {
     const float4 q = a.part[(long long)row * a.G + g];
     v = lse_join(v, {q.x, q.y, q.z}, c);
   }
-  v = lse_join_lanes(v, c, 1, 32);
+  v = lse_join_wave(v, c);
   if (lane == 0) s_lse[wave] = v;
   bar();
   v = s_lse[0];
@@ -389,58 +427,103 @@ __global__ void __launch_bounds__(LP_NT) k_lp_row(LpArgs a) {
       if (lane == 0) a.out_rank[o] = ok ? n : -1;
     }
   }
-  if constexpr (KPT != 0) {
-    auto group = [&](int i) {
-      const int g = i * LP_NT + tid;
-      return g < ng && gv[i] > -INFINITY ? comp(okey(gv[i]), (uint32_t)g) : 0;
+  if constexpr (TOP) {
+    const int n = a.top;
+    const bool held = ng <= KPT * LP_NT;
+    auto chunks = [&](auto f) {  // f(first group) with gv loaded, over the row
+      for (int g0 = 0; g0 < ng; g0 += KPT * LP_NT) {
+        if (!held) load_groups(g0);
+        f(g0);
+      }
     };
-    uint64_t best = 0;
+    float best = -INFINITY;
+    chunks([&](int) {
 #pragma unroll
-    for (int i = 0; i < KPT; i++) best = max(best, group(i));
-    uint64_t thr = lp_threshold(best, a.top, s);
+      for (int i = 0; i < KPT; i += 2) best = lse_max3(best, gv[i], gv[i + 1]);
+    });
+    const uint32_t bound = max(lp_bound(lp_value(best), n, s), KEY_NEGINF + 1);
+    const float least = okey_val(bound);
+    chunks([&](int g0) {
+      uint32_t mine = 0;
 #pragma unroll
-    for (int i = 0; i < KPT; i++) lp_take(group(i), thr, s, list);
+      for (int i = 0; i < KPT; i++) mine |= gv[i] >= least ? 1u << i : 0u;
+      if (mine) {
+        int at = atomicAdd(&s.n, __popc(mine));
+        for (; mine; mine &= mine - 1, at++)
+          if (at < 64) s.win[at] = g0 + (__ffs(mine) - 1) * LP_NT + tid;
+      }
+    });
     bar();
-    lp_ranked(s, list, a.top, [&](int r, uint64_t k) { s.win[r] = (int)comp_idx(k); });
-    const int nw = min(s.n, a.top);
-    bar();
-    constexpr int PER = LP_NMAX / LP_NW;  // winning groups of a wave at most
+    int nw = s.n;
+    if (nw > 64) {
+      auto key = [&](int g0, int i) { return gv[i] > -INFINITY ? comp(okey(gv[i]), (uint32_t)(g0 + i * LP_NT + tid)) : 0; };
+      uint64_t top = 0;
+      chunks([&](int g0) {
+#pragma unroll
+        for (int i = 0; i < KPT; i++) top = max(top, key(g0, i));
+      });
+      const uint64_t thr = lp_threshold(top, n, s);
+      chunks([&](int g0) {
+#pragma unroll
+        for (int i = 0; i < KPT; i++) lp_take(key(g0, i), thr, s, list);
+      });
+      bar();
+      lp_ranked(s, list, n, [&](int r, uint64_t k) { s.win[r] = (int)comp_idx(k); });
+      nw = min(s.n, n);
+      bar();
+    }
+    // the groups' logits: lane l takes place l of every fourth group
+    constexpr int PER = 64 / LP_NW;
+    const int mine = s.win[min(lane * LP_NW + wave, 63)];  // this wave's groups, by lanes
+    auto place = [&](int i) { return __builtin_amdgcn_readlane(mine, i) * LP_GRP + lane - lead; };
     float x[PER];
 #pragma unroll
-    for (int i = 0; i < PER; i++)
-      if (i * LP_NW < nw) x[i] = lp_one(p + (min(max(s.win[min(i * LP_NW + wave, nw - 1)] * LP_GRP + lane, lead), end - 1) - lead));
-    uint64_t key[PER];
-    best = 0;
+    for (int i = 0; i < PER; i++) {
+      x[i] = -INFINITY;
+      if (i * LP_NW + wave < nw) x[i] = lp_one(p + min(max(place(i), 0), a.V - 1));
+    }
+    best = -INFINITY;
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-      const int k = i * LP_NW + wave;
-      key[i] = 0;
-      if (k < nw) {
-        const int e = s.win[k] * LP_GRP + lane;
-        if (e >= lead && e < end && x[i] > -INFINITY) key[i] = comp(okey(x[i]), (uint32_t)(e - lead));
-      }
-      best = max(best, key[i]);
+      if (i * LP_NW + wave < nw && (place(i) < 0 || place(i) >= a.V)) x[i] = -INFINITY;
+      best = fmaxf(best, x[i]);
     }
-    thr = lp_threshold(best, a.top, s);
+    const float low = okey_val(max(lp_bound(lp_value(best), n, s), KEY_NEGINF + 1));
+    {
+      uint32_t took = 0;
 #pragma unroll
-    for (int i = 0; i < PER; i++) lp_take(key[i], thr, s, list);
+      for (int i = 0; i < PER; i++) took |= x[i] >= low ? 1u << i : 0u;
+      if (took) {
+        int at = atomicAdd(&s.n, __popc(took));
+        for (; took; took &= took - 1, at++)
+          if (at < 64) {
+            const int e = s.win[(__ffs(took) - 1) * LP_NW + wave] * LP_GRP + lane - lead;
+            list[at] = comp(okey(lp_one(p + e)), (uint32_t)e);
+          }
+      }
+    }
     bar();
-    int* ids = a.out_ids + (long long)row * a.top;
-    float* lps = a.out_top + (long long)row * a.top;
-    lp_ranked(s, list, a.top, [&](int r, uint64_t k) {
+    if (s.n > 64) {
+      auto key = [&](int i) { return x[i] > -INFINITY ? comp(okey(x[i]), (uint32_t)place(i)) : 0; };
+      uint64_t top = 0;
+#pragma unroll
+      for (int i = 0; i < PER; i++) top = max(top, key(i));
+      const uint64_t thr = lp_threshold(top, n, s);
+#pragma unroll
+      for (int i = 0; i < PER; i++) lp_take(key(i), thr, s, list);
+      bar();
+    }
+    int* ids = a.out_ids + (long long)row * n;
+    float* lps = a.out_top + (long long)row * n;
+    lp_ranked(s, list, n, [&](int r, uint64_t k) {
       ids[r] = (int)comp_idx(k);
       lps[r] = lse_logprob(v, okey_val(comp_key(k)), temp);
     });
-    for (int r = s.n + tid; r < a.top; r += LP_NT) {
+    for (int r = s.n + tid; r < n; r += LP_NT) {
       ids[r] = -1;
       lps[r] = -INFINITY;
     }
   }
-}
-// Keys that a selection of the n best can list: those of the n lanes whose best are the n largest
-inline size_t lp_list(int groups, int n) {
-  const int a = n * ((groups + 63) / 64) < groups ? n * ((groups + 63) / 64) : groups, b = n < 64 ? n * n : n * 64;
-  return (size_t)(a > b ? a : b);
 }
 
 struct LpPlan {
@@ -494,19 +577,17 @@ int lp_launch(LpArgs a, int R, char* ws, size_t ws_bytes, hipStream_t st) {
   a.part = (float4*)(ws + q.part);
   a.cnt = (int*)(ws + q.cnt);
   a.gmax = (float*)(ws + q.gmax);
+  const size_t lds = a.top ? sizeof(uint64_t) * lp_list(q.groups, a.top) : 0;
   if (a.top)
     lp_launch_scan<T, true>(a, R, st);
   else
     lp_launch_scan<T, false>(a, R, st);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return (int)e;
-  const size_t lds = a.top ? sizeof(uint64_t) * lp_list(q.groups, a.top) : 0;
-  if (!a.top)
-    hipLaunchKernelGGL((k_lp_row<T, 0>), dim3(R), dim3(LP_NT), 0, st, a);
-  else if (q.groups <= 16 * LP_NT)
-    hipLaunchKernelGGL((k_lp_row<T, 16>), dim3(R), dim3(LP_NT), lds, st, a);
+  if (a.top)
+    hipLaunchKernelGGL((k_lp_row<T, true>), dim3(R), dim3(LP_NT), lds, st, a);
   else
-    hipLaunchKernelGGL((k_lp_row<T, 33>), dim3(R), dim3(LP_NT), lds, st, a);
+    hipLaunchKernelGGL((k_lp_row<T, false>), dim3(R), dim3(LP_NT), 0, st, a);
   return (int)hipGetLastError();
 }
 

@@ -55,6 +55,11 @@ __device__ __forceinline__ Lse lse_join(Lse a, Lse b, float c) {
   const float da = lse_d(a.m, m, c), db = lse_d(b.m, m, c), ea = lse_exp2(da), eb = lse_exp2(db);
   return {m, fmaf(ea, a.s, eb * b.s), fmaf(ea, fmaf(da, a.s, a.t), eb * fmaf(db, b.s, b.t))};
 }
+// the wave's values joined, in every lane
+__device__ __forceinline__ Lse lse_join_wave(Lse v, float c) {
+  const float m = wave_max_f(v.m), d = lse_d(v.m, m, c), e = lse_exp2(d);
+  return {m, wave_sum<float>(e * v.s), wave_sum<float>(e * fmaf(d, v.s, v.t))};
+}
 __device__ inline Lse lse_join_lanes(Lse v, float c, int from, int to) {  // butterfly over lane bits `from` .. `to` (powers of two)
   for (int i = from; i <= to; i <<= 1) v = lse_join(v, {__shfl_xor(v.m, i), __shfl_xor(v.s, i), __shfl_xor(v.t, i)}, c);
   return v;

@@ -97,13 +97,13 @@ class LogProbs:
             given(temperature, lead, torch.float32, dev, "temperature")
         where, stream = on_stream(dev.index)
         with where:
-            if M:
-                lp = torch.empty(shape, dtype=torch.float32, device=dev)
-                if ranks:
-                    rk = torch.empty_like(tokens)
             h = torch.empty(lead, dtype=torch.float32, device=dev)
             ids = torch.empty((*lead, top), dtype=torch.int32, device=dev)
-            tlp = torch.empty((*lead, top), dtype=torch.float32, device=dev)
+            tlp = h.new_empty((*lead, top))
+            if M:
+                lp = h.new_empty(shape)
+                if ranks:
+                    rk = ids.new_empty(shape)
             if R:
                 dt = _lib.DTYPE_F32 if dtype == torch.float32 else _lib.DTYPE_BF16
                 key = (dt, R, V, M, top)
