@@ -238,9 +238,10 @@ __device__ __forceinline__ void lp_ranked(LpSel& s, const uint64_t* list, int n,
     if (r < n) put(r, k);
   }
 }
-// Keys that a selection of the n best can list: those of the n lanes whose best are the n largest
+// Keys that a selection of the n best can list: those of the n lanes whose best are the n largest; a lane has one of every 64
+// groups, then one of each of up to 64 groups looked through.
 inline size_t lp_list(int groups, int n) {
-  const int a = n * ((groups + 63) / 64) < groups ? n * ((groups + 63) / 64) : groups, b = n < 64 ? (n > 8 ? n * n : 64) : n * 64;
+  const int a = n * ((groups + 63) / 64), b = n * 64;
   return (size_t)(a > b ? a : b);
 }
 __device__ __forceinline__ uint32_t lp_value(float x) { return x > -INFINITY ? okey(x) : 0; }
@@ -592,6 +593,9 @@ int lp_launch(LpArgs a, int R, char* ws, size_t ws_bytes, hipStream_t st) {
 }
 
 }  // namespace qws
+
+static_assert(sizeof(qws_logprobs_batch) == 96 && offsetof(qws_logprobs_batch, tokens) == 32 && offsetof(qws_logprobs_batch, out_top_logprobs) == 88,
+              "qws_logprobs_batch layout (the ctypes binding's)");
 
 extern "C" size_t qws_logprobs_ws_bytes(int dtype, int R, int V, int M, int top) {
   using namespace qws;

@@ -108,6 +108,22 @@ def test_orders(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_ties_in_few_places(dtype):
+    """Many groups of 64 logits tie, their ties in fewer places than alternatives are asked for: the selections then list as
+    many keys as they ever can."""
+    V = 9001
+    x = torch.zeros(8, V)
+    places = torch.arange(V) % 64
+    for r, (groups, lanes) in enumerate(((40, 19), (64, 19), (64, 4), (140, 1), (21, 20), (30, 64), (63, 7), (140, 19))):
+        x[r, (torch.arange(V) // 64 < groups) & (places < lanes)] = 5.0
+    x[1] -= 3.0
+    tokens = torch.tensor([[0, 18, 19, 64, 9000]] * 8, dtype=torch.int32)
+    for top in (5, 8, 9, 20, 45, 63, 64):
+        for pad, offset in ((0, 0), (3, 1)):
+            check(x.to(dtype), tokens, top, None, f"ties top={top}", pad, offset)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("temperature", [None, 0.4, 1.7])
 def test_masks(dtype, temperature):
     """Rows of nothing, of one token, with NaN, infinities and the type's lowest value, alone and mixed."""

@@ -82,6 +82,11 @@ def test_logprobs_refuses(lib, kw):
     assert lib.qws_logprobs(C.byref(_batch(**kw)), P, 1 << 30, None) == _lib.ERR_INVALID
 
 
+def test_logprobs_struct_layout():
+    """The library's own layout is asserted where it is built (qws_logprobs.hip)."""
+    assert C.sizeof(_lib.LogprobsBatch) == 96 and _lib.LogprobsBatch.tokens.offset == 32 and _lib.LogprobsBatch.out_top_logprobs.offset == 88
+
+
 def test_logprobs_limits(lib):
     for kw in (dict(V=(1 << 19) + 1), dict(M=65), dict(top=65)):
         assert lib.qws_logprobs(C.byref(_batch(**kw)), P, 1 << 30, None) == _lib.ERR_NOT_SUPPORTED
