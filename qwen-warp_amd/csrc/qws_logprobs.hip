@@ -33,6 +33,12 @@ constexpr int lp_stripe() { return LP_NT * lp_e<T>(); }  // elements that a work
 template <typename T>
 using lp_bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
 
+// the next larger value
+__device__ __forceinline__ float lp_above(float x) {
+  const int b = __float_as_int(x + 0.0f);
+  return __int_as_float(b >= 0 ? b + 1 : b - 1);
+}
+
 struct LpArgs {
   const void* x;
   long long stride;
@@ -246,13 +252,12 @@ inline size_t lp_list(int groups, int n) {
 }
 __device__ __forceinline__ uint32_t lp_value(float x) { return x > -INFINITY ? okey(x) : 0; }
 
-// RANK: 0 no given tokens' ranks, 1 one token per row (held in registers), 2 several (in LDS).  U vectors of a thread make a
+// RANK: 0 no given tokens' ranks, 1 one token per row (held in registers), 2 several (a lane each).  U vectors of a thread make a
 // block: loaded together, one step of the running maximum.
 template <typename T, int RANK, bool TOP, int U>
 __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
   constexpr int E = lp_e<T>(), SE = lp_stripe<T>();
-  __shared__ float s_xt[LP_NMAX];
-  __shared__ int s_tv[LP_NMAX], s_cnt[LP_NMAX];
+  __shared__ int s_cnt[LP_NMAX];
   __shared__ Lse s_lse[LP_NW];
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_id();
   const int row = blockIdx.x / a.G, ch = blockIdx.x % a.G;
@@ -273,8 +278,8 @@ __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
     }
   };
   if constexpr (U == 1) load(s_begin);  // the one block, before the given tokens' two loads in a row
-  float xt = 0.0f;
-  int tv = -1, cnt = 0;  // virtual position of the token (-1: skipped), logits before it
+  float xt = 0.0f;  // the given token's logit; with several, lane m's is token m's
+  int tv = -1, cnt = 0;  // its place (-1: skipped), logits before it
   bool moderate = c <= LSE_MOST;  // no given token's logit is extreme
   if constexpr (RANK == 1) {
     const int t = a.tok[row];
@@ -285,15 +290,12 @@ __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
     }
   }
   if constexpr (RANK == 2) {
-    if (tid < a.M) {
-      const int t = a.tok[(long long)row * a.M + tid];
-      const bool ok = t >= 0 && t < a.V;
-      s_tv[tid] = ok ? t + lead : -1;
-      s_xt[tid] = ok ? lp_one(p + t) : 0.0f;
-      s_cnt[tid] = 0;
+    const int t = lane < a.M ? a.tok[(long long)row * a.M + lane] : -1;
+    if (t >= 0 && t < a.V) {
+      tv = t + lead;
+      xt = lp_one(p + t);
     }
-    bar();
-    for (int k = 0; k < a.M; k += 64) moderate = moderate && !__any(k + lane < a.M && !(fabsf(s_xt[min(k + lane, a.M - 1)]) < LSE_MOST));
+    moderate = moderate && __all(fabsf(xt) < LSE_MOST);
   }
   Lse v = {-INFINITY, 0.0f, 0.0f};
   LpFast f = {-INFINITY, -1e30f, -INFINITY, 0.0f, 0.0f};
@@ -330,40 +332,68 @@ __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
       for (int u = 0; u < U; u++)  // byte offsets in 32 bits: one address register for all
         if ((lane & (LP_GRP / E - 1)) == 0 && s + u < s_end) *(float*)(gmax + (unsigned)((first + u * SE + tid * E) / LP_GRP * 4)) = top[u];
     }
-    if constexpr (RANK != 0) {
-      const int n = RANK == 1 ? 1 : a.M;
-      for (int k = 0; k < n; k++) {
-        const float xk = RANK == 1 ? xt : s_xt[k];
-        const int tk = RANK == 1 ? tv : s_tv[k];
-        int add = 0;
-        if (!__any(best >= xk)) continue;  // a likely token: nothing here is before it
+    // Before a token: the logits at or above its own in places before it, the larger ones behind it.  A wave's 64 E places lie
+    // on one side of almost every token: one comparison a logit.
+    if constexpr (RANK == 1) {
+      if (__any(best >= xt)) {  // else a likely token: nothing here is before it
 #pragma unroll
         for (int u = 0; u < U; u++) {
           // this wave's elements: [lo, lo + 64 E); a stripe of the next workgroup lies behind every token
           const int lo = s + u < s_end ? first + u * SE + wave * 64 * E : 0x7FFFFFFF - 64 * E;
-          if (lo + 64 * E <= tk) {
+          if (lo + 64 * E <= tv) {
 #pragma unroll
-            for (int j = 0; j < E; j++) add += __popcll(__ballot(x[u][j] >= xk));
-          } else if (lo > tk) {
+            for (int j = 0; j < E; j++) cnt += __popcll(__ballot(x[u][j] >= xt));
+          } else if (lo > tv) {
 #pragma unroll
-            for (int j = 0; j < E; j++) add += __popcll(__ballot(x[u][j] > xk));
+            for (int j = 0; j < E; j++) cnt += __popcll(__ballot(x[u][j] > xt));
           } else {
 #pragma unroll
-            for (int j = 0; j < E; j++) add += __popcll(__ballot(x[u][j] > xk || (x[u][j] == xk && lo + lane * E + j < tk)));
+            for (int j = 0; j < E; j++) cnt += __popcll(__ballot(x[u][j] > xt || (x[u][j] == xt && lo + lane * E + j < tv)));
           }
         }
-        if constexpr (RANK == 1)
-          cnt += add;
-        else if (lane == 0)
-          atomicAdd(&s_cnt[k], add);
+      }
+    }
+    if constexpr (RANK == 2) {  // without branches, a bound for each side; a token that is among them has its equals added
+      float bound[U];
+      int lo[U];
+      bool among = false;
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        lo[u] = s + u < s_end ? first + u * SE + wave * 64 * E : 0x7FFFFFFF - 64 * E;
+        bound[u] = lo[u] + 64 * E <= tv ? xt : lp_above(xt);
+        among = among || (tv >= lo[u] && tv < lo[u] + 64 * E);
+      }
+      uint64_t left = __ballot(among);
+#pragma unroll 2
+      for (int k = 0; k < a.M; k++) {
+        int n = 0;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          const float b = readlane<float>(bound[u], k);
+#pragma unroll
+          for (int j = 0; j < E; j++) n += __popcll(__ballot(x[u][j] >= b));
+        }
+        cnt += lane == k ? n : 0;
+      }
+      for (; left; left &= left - 1) {
+        const int k = __ffsll((long long)left) - 1, tk = readlane<int>(tv, k);
+        const float xk = readlane<float>(xt, k);
+        int n = 0;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+          if (tk >= lo[u] && tk < lo[u] + 64 * E)
+#pragma unroll
+            for (int j = 0; j < E; j++) n += __popcll(__ballot(x[u][j] == xk && lo[u] + lane * E + j < tk));
+        cnt += lane == k ? n : 0;
       }
     }
   }
   v = lse_join_wave(lse_join(v, lp_fast_end(f, c), c), c);
-  if constexpr (RANK == 1) {
-    if (tid == 0) s_cnt[0] = 0;
+  if constexpr (RANK != 0) {
+    const int n = RANK == 1 ? 1 : a.M;
+    if (tid < n) s_cnt[tid] = 0;
     bar();
-    if (lane == 0) atomicAdd(&s_cnt[0], cnt);
+    if (lane < n) atomicAdd(&s_cnt[lane], cnt);
   }
   if (lane == 0) s_lse[wave] = v;
   bar();
@@ -384,6 +414,7 @@ template <typename T, bool TOP>
 __global__ void __launch_bounds__(LP_NT) k_lp_row(LpArgs a) {
   __shared__ LpSel s;
   __shared__ Lse s_lse[LP_NW];
+  __shared__ int s_cnt[LP_NMAX];
   extern __shared__ uint64_t list[];  // lp_list(groups, top) keys
   constexpr int E = lp_e<T>(), KPT = 16;  // groups of a thread that are held in registers: all, up to V = 262,144
   const int tid = threadIdx.x, lane = lane_id(), wave = wave_id(), row = blockIdx.x;
@@ -402,6 +433,21 @@ __global__ void __launch_bounds__(LP_NT) k_lp_row(LpArgs a) {
   };
   if constexpr (TOP) load_groups(0);
   const float temp = a.temp ? a.temp[row] : 1.0f, c = lse_scale(temp);
+  // thread m has given token m; the parts of its count are spread over all threads
+  bool ok = false;
+  float xt = 0.0f;
+  if (tid < a.M) {
+    const int t = a.tok[(long long)row * a.M + tid];
+    ok = t >= 0 && t < a.V;
+    if (ok) xt = lp_one(p + t);
+    s_cnt[tid] = 0;
+  }
+  int cnt = 0;
+  if (a.M && a.out_rank) {
+    const int parts = LP_NT / a.M;
+    if (tid < parts * a.M)
+      for (int g = tid / a.M; g < a.G; g += parts) cnt += a.cnt[((long long)row * a.G + g) * a.M + tid % a.M];
+  }
   Lse v = {-INFINITY, 0.0f, 0.0f};
   for (int g = tid; g < a.G; g += LP_NT) {
     const float4 q = a.part[(long long)row * a.G + g];
@@ -410,22 +456,21 @@ __global__ void __launch_bounds__(LP_NT) k_lp_row(LpArgs a) {
   v = lse_join_wave(v, c);
   if (lane == 0) s_lse[wave] = v;
   bar();
+  if (cnt) atomicAdd(&s_cnt[tid % a.M], cnt);
   v = s_lse[0];
 #pragma unroll
   for (int w = 1; w < LP_NW; w++) v = lse_join(v, s_lse[w], c);
+  bar();
   if (tid == 0 && a.out_h) a.out_h[row] = lse_entropy(v);
-  for (int m = wave; m < a.M; m += LP_NW) {
-    const long long o = (long long)row * a.M + m;
-    const int t = a.tok[o];
-    const bool ok = t >= 0 && t < a.V;
-    const float x = ok ? lp_one(p + t) : 0.0f;
-    if (lane == 0) a.out_lp[o] = ok ? lse_logprob(v, x, temp) : 0.0f;
-    if (a.out_rank) {
-      int n = 0;
-      for (int g = lane; g < a.G; g += 64) n += a.cnt[((long long)row * a.G + g) * a.M + m];
-      n = wave_sum<int>(n);
-      if (x == -INFINITY) n -= lead;  // the places before the row were counted as -inf of lower indices
-      if (lane == 0) a.out_rank[o] = ok ? n : -1;
+  if (tid < a.M) {
+    const long long o = (long long)row * a.M + tid;
+    if (ok) {
+      const int places = xt == -INFINITY ? lead : 0;  // before the row: they were counted as -inf of lower indices
+      a.out_lp[o] = lse_logprob(v, xt, temp);
+      if (a.out_rank) a.out_rank[o] = s_cnt[tid] - places;
+    } else {
+      a.out_lp[o] = 0.0f;
+      if (a.out_rank) a.out_rank[o] = -1;
     }
   }
   if constexpr (TOP) {
