@@ -582,20 +582,32 @@ __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int t
   }
 }
 
-// One wave per hidden state: its parts joined
+// One workgroup per hidden state: its parts joined (up to 3,880 of them at the full head)
 __global__ void __launch_bounds__(256) k_f8_score(F8Args a, float* out_lp, float* out_h) {
-  const int lane = lane_id(), t = blockIdx.x * 4 + wave_id();
-  if (t >= a.T) return;
+  __shared__ Lse s_lse[4];
+  const int lane = lane_id(), wave = wave_id(), t = blockIdx.x;
   const float temp = a.temp ? a.temp[t] : 1.0f, c = lse_scale(temp);
-  Lse v = {-INFINITY, 0.0f, 0.0f};
-  for (int i = lane; i < a.parts; i += 64) {
-    const float4 q = a.part[(size_t)t * a.parts + i];
-    v = lse_join(v, {q.x, q.y, q.z}, c);
-  }
-  v = lse_join_lanes(v, c, 1, 32);
-  if (lane) return;
   const int tok = a.tok[t];
-  out_lp[t] = tok >= 0 && tok < a.N ? lse_logprob(v, a.given[t], temp) : 0.0f;
+  const bool ok = tok >= 0 && tok < a.N;
+  const float given = ok ? a.given[t] : 0.0f;
+  const float4* part = a.part + (size_t)t * a.parts;
+  Lse v = {-INFINITY, 0.0f, 0.0f};
+  constexpr int U = 4;  // parts of a thread loaded together
+  for (int i = threadIdx.x; i < a.parts; i += 256 * U) {
+    float4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) q[u] = part[min(i + 256 * u, a.parts - 1)];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (i + 256 * u < a.parts) v = lse_join(v, {q[u].x, q[u].y, q[u].z}, c);
+  }
+  v = lse_join_wave(v, c);
+  if (lane == 0) s_lse[wave] = v;
+  bar();
+  if (threadIdx.x) return;
+#pragma unroll
+  for (int w = 1; w < 4; w++) v = lse_join(v, s_lse[w], c);
+  out_lp[t] = ok ? lse_logprob(v, given, temp) : 0.0f;
   if (out_h) out_h[t] = lse_entropy(v);
 }
 
@@ -781,6 +793,6 @@ extern "C" int qws_fp8_score(const void* packed, int N, int K, const void* x, lo
   a.parts = f8_plan(T, N).parts;
   const int e = f8_product<void>(a, K, x, x_stride, (char*)ws, (hipStream_t)stream);
   if (e) return e;
-  hipLaunchKernelGGL(k_f8_score, dim3((T + 3) / 4), dim3(256), 0, (hipStream_t)stream, a, out_logprobs, out_entropy);
+  hipLaunchKernelGGL(k_f8_score, dim3(T), dim3(256), 0, (hipStream_t)stream, a, out_logprobs, out_entropy);
   return (int)hipGetLastError();
 }
