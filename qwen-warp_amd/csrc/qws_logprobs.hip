@@ -3,12 +3,19 @@
 //
 //   k_lp_scan   R x G workgroups of 256: one pass over the logits.  Each lane keeps the running maximum and sums of its
 //               elements; each given token's rank is counted by ballots; and the maximum of every 64 consecutive logits
-//               (a group) goes to the workspace.
+//               (a group) goes to the workspace.  Bound by the logits' bytes in fp32 (256 rows of 248,320: 42.4 us, 6.0
+//               TB/s), in bf16 by the vector instructions, five and a half a logit, beside them (2,048 rows: 206 us, 4.9
+//               TB/s), and for few rows by one load's and one launch's latency (1 bf16 row 4.0 us, 36 fp32 rows 9.0).
 //   k_lp_row    R workgroups of 256: joins the row's parts, writes log probabilities, ranks and entropy, and takes the
 //               alternatives in two selections: the n groups with the best maxima (ties: the first), then the n best of
 //               those groups' logits.  That is exact: a logit outside those groups has n better ones, the maxima of the n
 //               groups (each larger, or equal and of a lower index, since groups are consecutive runs of tokens).  So the
 //               pass over the logits does nothing more for 64 alternatives than for none, whatever their order in memory.
+//               Bound by latency: a chain of five loads and some twenty barriers (8-10.6 us up to 256 rows; 2,048 rows
+//               20.6 us, in two rounds of workgroups on the card).
+// The join is a launch of its own: a row's last workgroup finishing it in k_lp_scan has to make every workgroup's results
+// visible to other dies' caches first (256 fp32 rows 125 us with stores through the cache, 518 with a release each, against
+// 53; only a single row gained, 21.8 -> 17.9).
 #include "qws_lse.h"
 
 #include <type_traits>
@@ -277,7 +284,7 @@ __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
       for (int u = 0; u < U; u++) r[u] = lp_load_edge(base, first + u * SE + tid * E, s + u < s_end ? lead : end, end);
     }
   };
-  if constexpr (U == 1) load(s_begin);  // the one block, before the given tokens' two loads in a row
+  load(s_begin);  // before the given tokens' two loads in a row (36 fp32 rows 23.2 us a call, 22.7 so)
   float xt = 0.0f;  // the given token's logit; with several, lane m's is token m's
   int tv = -1, cnt = 0;  // its place (-1: skipped), logits before it
   bool moderate = c <= LSE_MOST;  // no given token's logit is extreme
@@ -302,7 +309,6 @@ __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
   char* gmax = (char*)(a.gmax + (long long)row * a.groups);
   for (int s = s_begin; s < s_end; s += U) {
     const int first = s * SE;
-    if constexpr (U != 1) load(s);
     float top[U];
     float x[U][E], best = -INFINITY, least = INFINITY;
 #pragma unroll
@@ -387,6 +393,8 @@ __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
         cnt += lane == k ? n : 0;
       }
     }
+    if constexpr (U != 1)
+      if (s + U < s_end) load(s + U);  // here, not before the sums: a second block in registers costs waves (bf16 219 -> 273 us)
   }
   v = lse_join_wave(lse_join(v, lp_fast_end(f, c), c), c);
   if constexpr (RANK != 0) {

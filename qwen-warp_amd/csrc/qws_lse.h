@@ -4,9 +4,12 @@
 // With c = log2(e) / T and d_i = c (x_i - m), m the largest x so far:
 //   s = sum 2^d_i,   t = sum 2^d_i d_i    (fp32)
 // A larger maximum m' (delta = c (m' - m)) turns them into 2^-delta s and 2^-delta (t - delta s): one pass, any order.
-// Then, with both terms of H >= 0 (s >= 1, t <= 0: nothing cancels),
+// Then
 //   log p_i = (x_i - m) / T - ln s,   H = ln s - ln 2 * t / s.
-// Differences to the maximum are taken before the scaling, so rows at the type's lowest value and rows mixing it with
+// With m the largest x both terms of H are >= 0 (s >= 1, t <= 0): nothing cancels.  m may be any value near it instead: with
+// one that lies up to 8 units of d below (k_lp_scan's, so that it rarely moves) the terms cancel by at most 8 ln 2 = 5.5, an
+// error of a few 5.5 * 2^-24 in H.
+// The general form takes differences to m before the scaling, so rows at the type's lowest value and rows mixing it with
 // -inf are exact; NaN counts as -inf (the sampling stage's rule), +inf as the largest finite value (so tokens at +inf share
 // the row); d is held above -D_MIN, where 2^d is 0 in fp32: no infinity meets a 0 in t.
 #pragma once
