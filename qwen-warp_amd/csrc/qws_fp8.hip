@@ -77,7 +77,10 @@ __device__ __forceinline__ uint32_t f8_four(const float* v, int e) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false), true);
 }
 
-// One wave per block of 16 rows: lane l takes row l % 16, values 16 (l / 16) .. + 15 of both fragments.
+// One wave per block of 16 rows: lane l takes row l % 16, values 16 (l / 16) .. + 15 of both fragments, so that a block's
+// largest value is two steps over lanes away and a fragment leaves as 1 KB.  Bound by memory (248,320 x 5,120 bf16 weights, 2.54
+// GB read and 1.28 GB written: 780 us, 4.9 TB/s, the rate of a large copy); a few hidden states are one launch's latency
+// (4.7 us).
 //   WIDE: the values as bf16 instead (exact), as k_f8_tile takes hidden states: product h of fragment c is 1 KB of its own.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) k_f8_pack(const T* x, long long stride, int rows, int K, F8Layout l, char* out) {
@@ -248,7 +251,9 @@ template <typename O>
 using f8_out = std::conditional_t<std::is_void_v<O>, float, O>;
 
 // Few hidden states (T <= 16 TF): the weights' bytes bound it.  A workgroup takes G groups of 16 weight rows, its 4 waves a
-// quarter of K each, straight from memory into registers, one block ahead; their sums meet in LDS.
+// quarter of K each, straight from memory into registers, one block ahead; their sums meet in LDS.  Every weight is used by one
+// wave, so LDS would only add a step; K is split because that leaves 3,880 workgroups of 64 rows at N = 248,320 and still
+// enough at N = 8,191.  One hidden state at K = 5,120, N = 248,320: 214 us, 5.95 TB/s of weights; sixteen: 235, 5.4 TB/s.
 //   RAW (TF = 1): the hidden states as they came, 16-byte aligned vectors of 8; each workgroup rounds them into LDS itself,
 //   under its first loads of weights, which for a few KB takes less than a launch of k_f8_pack.
 template <int G, int TF>
@@ -410,15 +415,20 @@ __device__ __forceinline__ void f8_meet() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// Tiles of 32 FN weight rows (128 or 256) x 32 FT hidden states: 4 waves of 16 FN x 16 FT, one to a SIMD.  A stage is 64
-// values along K, 2 FN KB of weights and 4 FT KB of hidden states (already bf16: k_f8_pack), copied by the memory system straight into one of three
-// LDS buffers, three stages ahead.  A stage has two halves of 32 values: the first half's products run while the second
-// half's hidden states are read, then everybody meets (a wave first waits for its own copies of the next stage; the newest
-// stage's stay in flight), and the second half's products run while the next stage's operands are read.  A half has a step
-// for each fragment of weights: its FT products, and beside them the next fragment's widening to bf16, a few reads and one
-// copy (into the buffer that the last meeting freed: over the second half and the next first one), little enough for the
-// time of as many products.  A workgroup takes every 256th tile; the first stages of its next one are copied while it
-// finishes the last.
+// Many hidden states: the products bound it.  Tiles of 32 FN weight rows (128 or 256) x 32 FT hidden states: 4 waves of 16 FN
+// x 16 FT, one to a SIMD, so that each has the registers for 128 x 128 sums and an operand read from LDS serves eight
+// products.  A stage is 64 values along K, 2 FN KB of weights and 4 FT KB of hidden states (already bf16: k_f8_pack; in 8
+// bits each wave would widen them again: 3,687 us against 3,600), copied by the memory system straight into one of three LDS
+// buffers, three stages ahead.  A stage has two halves of 32 values: the first half's products run while the second half's
+// hidden states are read, then everybody meets (a wave first waits for its own copies of the next stage; the newest stage's
+// stay in flight), and the second half's products run while the next stage's operands are read.  A half has a step for each
+// fragment of weights: its FT products, and beside them the next fragment's widening to bf16, a few reads and one copy (into
+// the buffer that the last meeting freed: over the second half and the next first one), little enough for the time of as many
+// products.  A workgroup takes every 256th tile; the first stages of its next one are copied while it finishes the last.
+//   2,048 states scored at K = 5,120, N = 248,320: 3,610 us, 1,443 TFLOP/s; without the copies 3,120, the products alone 2,330:
+//   the card's power bounds them all (nothing but these products, on such values, makes 2,200 TFLOP/s, and with 32x32x16
+//   products 1,910).  300 states' bf16 logits: 652 us, 1,170 TFLOP/s (20 of 320 columns are padding, and the last of 8
+//   rounds of tiles is 0.6 of one).
 template <int FN, int FT>
 struct F8Buf {
   vu4 w[2 * FN * 64];
@@ -582,7 +592,8 @@ __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int t
   }
 }
 
-// One workgroup per hidden state: its parts joined (up to 3,880 of them at the full head)
+// One workgroup per hidden state: its parts joined, up to 3,880 of them at the full head, four loads of a thread at once
+// (by one wave a state's call took 247 us, 228 so; 2,048 states at 970 parts, 32 MB: 8.2 us)
 __global__ void __launch_bounds__(256) k_f8_score(F8Args a, float* out_lp, float* out_h) {
   __shared__ Lse s_lse[4];
   const int lane = lane_id(), wave = wave_id(), t = blockIdx.x;
