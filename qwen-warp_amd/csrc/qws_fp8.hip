@@ -253,7 +253,8 @@ using f8_out = std::conditional_t<std::is_void_v<O>, float, O>;
 // Few hidden states (T <= 16 TF): the weights' bytes bound it.  A workgroup takes G groups of 16 weight rows, its 4 waves a
 // quarter of K each, straight from memory into registers, one block ahead; their sums meet in LDS.  Every weight is used by one
 // wave, so LDS would only add a step; K is split because that leaves 3,880 workgroups of 64 rows at N = 248,320 and still
-// enough at N = 8,191.  One hidden state at K = 5,120, N = 248,320: 214 us, 5.95 TB/s of weights; sixteen: 235, 5.4 TB/s.
+// enough at N = 8,191.  One hidden state at K = 5,120, N = 248,320: 214 us, 6.0 TB/s of weights; eight: 225, 5.7 TB/s.
+// From nine on large heads are k_f8_tile's, whose weights each workgroup widens once for 32 columns (f8_plan).
 //   RAW (TF = 1): the hidden states as they came, 16-byte aligned vectors of 8; each workgroup rounds them into LDS itself,
 //   under its first loads of weights, which for a few KB takes less than a launch of k_f8_pack.
 template <int G, int TF>
@@ -415,33 +416,37 @@ __device__ __forceinline__ void f8_meet() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// Many hidden states: the products bound it.  Tiles of 32 FN weight rows (128 or 256) x 32 FT hidden states: 4 waves of 16 FN
-// x 16 FT, one to a SIMD, so that each has the registers for 128 x 128 sums and an operand read from LDS serves eight
-// products.  A stage is 64 values along K, 2 FN KB of weights and 4 FT KB of hidden states (already bf16: k_f8_pack; in 8
-// bits each wave would widen them again: 3,687 us against 3,600), copied by the memory system straight into one of three LDS
-// buffers, three stages ahead.  A stage has two halves of 32 values: the first half's products run while the second half's
-// hidden states are read, then everybody meets (a wave first waits for its own copies of the next stage; the newest stage's
-// stay in flight), and the second half's products run while the next stage's operands are read.  A half has a step for each
-// fragment of weights: its FT products, and beside them the next fragment's widening to bf16, a few reads and one copy (into
-// the buffer that the last meeting freed: over the second half and the next first one), little enough for the time of as many
-// products.  A workgroup takes every 256th tile; the first stages of its next one are copied while it finishes the last.
+// Many hidden states: the products bound it, below some 200 the weights' bytes.  A tile is WN x WT = 4 waves of 16 FN weight
+// rows x 16 FT hidden states: 2 x 2, one wave to a SIMD, so that each has the registers for up to 128 x 128 sums and an operand
+// read from LDS serves eight products; for up to 64 hidden states 4 x 1, so that only one wave widens a weight (widening and
+// LDS reads, not products, fill its time), and two workgroups to a CU.  A stage is 64 values along K, WN FN KB of weights and
+// 2 WT FT KB of hidden states (already bf16: k_f8_pack; in 8 bits each wave would widen them again: 3,687 us against 3,600),
+// copied by the memory system straight into one of three LDS buffers, three stages ahead.  A stage has two halves of 32 values:
+// the first half's products run while the second half's hidden states are read, then everybody meets (a wave first waits for
+// its own copies of the next stage; the newest stage's stay in flight), and the second half's products run while the next
+// stage's operands are read.  A half has a step for each fragment of weights: its FT products, and beside them the next
+// fragment's widening to bf16, a few reads and one copy (into the buffer that the last meeting freed: over the second half and
+// the next first one), little enough for the time of as many products.  A workgroup takes every 256th (512th) tile; the first
+// stages of its next one are copied while it finishes the last.
 //   2,048 states scored at K = 5,120, N = 248,320: 3,610 us, 1,443 TFLOP/s; without the copies 3,120, the products alone 2,330:
 //   the card's power bounds them all (nothing but these products, on such values, makes 2,200 TFLOP/s, and with 32x32x16
 //   products 1,910).  300 states' bf16 logits: 652 us, 1,170 TFLOP/s (20 of 320 columns are padding, and the last of 8
-//   rounds of tiles is 0.6 of one).
-template <int FN, int FT>
+//   rounds of tiles is 0.6 of one).  16 states' fp32 logits: 227 us, 5.7 TB/s with them; 64: 263, 5.1 TB/s.
+template <int FN, int FT, int WT>
 struct F8Buf {
-  vu4 w[2 * FN * 64];
-  vu4 x[2 * FT * 128];
-  uint32_t e[256];  // exponents of the 32 FN rows
+  vu4 w[4 / WT * FN * 64];
+  vu4 x[WT * FT * 128];
+  uint32_t e[256];  // exponents of the tile's weight rows
 };
-template <typename O, int FN, int FT>
+template <typename O, int FN, int FT, int WT>
 __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int tiles_t) {
-  constexpr int WN = 2, WT = 2, GN = WN * FN, BN = 16 * GN, BT = 16 * WT * FT;
+  constexpr int WN = 4 / WT, GN = WN * FN, BN = 16 * GN, BT = 16 * WT * FT, XW = WT * FT / 2;
+  static_assert(GN % 4 == 0 && XW * 2 == WT * FT, "a stage's weights and hidden states in KB, split over the waves");
   constexpr int SUB = F8_ROWS / BN;  // workgroups' tiles of a tile as it is packed
-  constexpr int NEW = GN / 4 + FT + 1;  // copies of a wave per stage: FN / 2 KB of weights, FT of hidden states, 64 exponents
+  constexpr int NEW = GN / 4 + XW + 1;  // copies of a wave per stage: KB of weights, of hidden states, 64 exponents
   constexpr int CP = (NEW + 2 * FN - 1) / (2 * FN);  // copies of a step
-  __shared__ F8Buf<FN, FT> b0, b1, b2;
+  using Buf = F8Buf<FN, FT, WT>;
+  __shared__ Buf b0, b1, b2;
   __shared__ Lse s_lse[std::is_void_v<O> ? WN : 1][std::is_void_v<O> ? BT : 1];
   const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), wn = wave / WT, wt = wave % WT;
   const int kb4 = a.lw.kb4, stages = 2 * a.lw.kb;
@@ -453,16 +458,16 @@ __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int t
   auto point = [&](int id) {
     const int tn = row_tile(id), tt = (id >> 3) % tiles_t;
     pw = a.w + ((size_t)(tn / SUB) * stages * GN * SUB + tn % SUB * GN + GN / 4 * wave) * F8_FRAG;
-    px = a.x + ((size_t)tt * stages * 4 * FT + FT * wave) * 1024;
+    px = a.x + ((size_t)tt * stages * 2 * WT * FT + XW * wave) * 1024;
     pe = a.w + a.lw.scales + (size_t)(tn / SUB) * kb4 * 4 * F8_ROWS + (tn % SUB * BN + 64 * wave % BN) * 4;  // where BN is 128, twice
   };
-  auto copy = [&](int k, F8Buf<FN, FT>& b, auto D) {  // copy D of stage k
+  auto copy = [&](int k, Buf& b, auto D) {  // copy D of stage k
     constexpr int d = decltype(D)::value, xd = d - GN / 4;
     k = min(k, stages - 1);  // past the end: the last stage again, into a buffer that is not read any more
     if constexpr (d < GN / 4)
       f8_copy<d * 1024>(pw + (size_t)k * (F8_ROWS / 16 * F8_FRAG), o16, b.w + GN / 4 * wave * 64);
     else if constexpr (d < NEW - 1)
-      f8_copy<xd % 4 * 1024>(px + (size_t)k * (4 * FT * 1024) + xd / 4 * 4096, o16, b.x + (FT * wave + xd / 4 * 4) * 64);
+      f8_copy<xd % 4 * 1024>(px + (size_t)k * (2 * WT * FT * 1024) + xd / 4 * 4096, o16, b.x + (XW * wave + xd / 4 * 4) * 64);
     else if constexpr (d == NEW - 1)
       f8_copy_words(pe + (size_t)(k / 8) * (4 * F8_ROWS), o4, b.e + 64 * wave);
   };
@@ -470,12 +475,12 @@ __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int t
     [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>()), ...); }(std::make_integer_sequence<int, FN>());
   };
   // step i of the first FN steps of a stage's copies, and of the others
-  auto copy_first = [&](int k, F8Buf<FN, FT>& b, auto I) {
+  auto copy_first = [&](int k, Buf& b, auto I) {
     copy(k, b, std::integral_constant<int, decltype(I)::value * CP>());
     if constexpr (CP > 1) copy(k, b, std::integral_constant<int, decltype(I)::value * CP + 1>());
   };
-  auto copy_others = [&](int k, F8Buf<FN, FT>& b, auto I) { copy_first(k, b, std::integral_constant<int, decltype(I)::value + FN>()); };
-  auto copy_all = [&](int k, F8Buf<FN, FT>& b) {
+  auto copy_others = [&](int k, Buf& b, auto I) { copy_first(k, b, std::integral_constant<int, decltype(I)::value + FN>()); };
+  auto copy_all = [&](int k, Buf& b) {
     each([&](auto I) { copy_first(k, b, I); });
     each([&](auto I) { copy_others(k, b, I); });
   };
@@ -483,13 +488,13 @@ __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int t
   uint32_t word[FN];
   f8_b8 x0[FT], x1[FT], q;
   vf4 acc[FN][FT];
-  auto read_x = [&](const F8Buf<FN, FT>& b, int h, int j) { return __builtin_bit_cast(f8_b8, b.x[((wt * FT + j) * 2 + h) * 64 + lane]); };
-  auto read_w = [&](const F8Buf<FN, FT>& b, int i) {
+  auto read_x = [&](const Buf& b, int h, int j) { return __builtin_bit_cast(f8_b8, b.x[((wt * FT + j) * 2 + h) * 64 + lane]); };
+  auto read_w = [&](const Buf& b, int i) {
     w[i] = b.w[(wn * FN + i) * 64 + lane];
     word[i] = b.e[16 * (wn * FN + i) + (lane & 15)];
   };
   // stage k in b; `next` holds the next one, `last` the one before (free; the copies of stage k + 2 go on into it)
-  auto stage = [&](int k, F8Buf<FN, FT>& b, const F8Buf<FN, FT>& next, F8Buf<FN, FT>& last) {
+  auto stage = [&](int k, Buf& b, const Buf& next, Buf& last) {
     const int kb = k >> 1, kn = (k + 1) >> 1;
     each([&](auto I) {
       constexpr int i = decltype(I)::value;
@@ -629,20 +634,34 @@ int f8_pack(const void* x, long long stride, int rows, int K, F8Layout l, char* 
 }
 
 // What runs T hidden states against N weight rows: k_f8_few with `groups` row groups to a workgroup and `frags` fragments of
-// hidden states, or (groups = 0) k_f8_tile with tiles of 32 fn x 32 frags; the parts that scoring joins per hidden state.
-// Measured (us of a scoring call at K = 5,120, N = 248,320, k_f8_few / k_f8_tile): 24 states 262 / 256, 64 states 382 / 267;
-// but where the tiles are fewer than half the CUs (N = 8,191, K = 1,000) 64 states 19 / 24.
+// hidden states, or (groups = 0) k_f8_tile with waves of fn x frags fragments, wt of them along the hidden states; the parts
+// that scoring joins per hidden state.
+// Measured, us, k_f8_few / tiles of 256 x 32: 9 states' logits at K = 5,120, N = 248,320 231 / 229, 16 246 / 236, 32 267 / 245; 12
+// states at K = 1,280, N = 24,000 18 / 23, at 40,000 23 / 24, at 50,000 27 / 26 (32: 21 / 23, 26 / 24, 29 / 26): from more
+// tiles than half the CUs on.  Tiles of 256 x 64 / of 2 x 2 waves: 64 states 274 / 290, 96 361 / 304; at N = 24,000 26 / 25.
+// Without that many tiles k_f8_few / 2 x 2 waves: 64 states at N = 8,191, K = 1,000 19 / 24, at N = 32,001, K = 1,280 30 / 27.
 struct F8Plan {
-  int groups, frags, fn, parts;
+  int groups, frags, fn, wt, parts;
+  int rows() const { return 64 / wt * fn; }  // of a tile
+  int cols() const { return 16 * wt * frags; }
 };
 inline F8Plan f8_plan(int T, int N) {
   F8Plan p = {};
-  if (T <= 32 || (T <= 64 && N < 128 * F8_CUS / 2)) {
+  const bool many = N > 256 * F8_CUS / 2;
+  if (T <= 8 || (T <= 32 && !many) || (T <= 64 && N < 128 * F8_CUS / 2)) {
     p.frags = T <= 16 ? 1 : T <= 32 ? 2 : 4;
     p.groups = p.frags == 4 ? 2 : 4;
     p.parts = f8_up(N, 16 * p.groups) / (16 * p.groups);
     return p;
   }
+  if (T <= 64 && many) {
+    p.fn = 4;
+    p.wt = 1;
+    p.frags = T <= 32 ? 2 : 4;
+    p.parts = f8_up(N, p.rows()) / p.rows();
+    return p;
+  }
+  p.wt = 2;
   // The least rounds of workgroups times a tile's time: its products, per fragment of weights their widening, and a constant
   // (512 states: tiles of 256 x 256 965 us, 128 x 256 1,080, 256 x 128 1,063; 300: 256 x 160 654, 256 x 128 796; 77 states
   // at N = 32,001, K = 1,280: 128 x 96 27, 256 x 96 33).
@@ -657,19 +676,19 @@ inline F8Plan f8_plan(int T, int N) {
         p.frags = frags;
       }
     }
-  p.parts = f8_up(N, 32 * p.fn) / (32 * p.fn);
+  p.parts = f8_up(N, p.rows()) / p.rows();
   return p;
 }
 // Whether each workgroup of k_f8_few rounds the hidden states itself: up to 20,480 values (us with / without, K = 5,120:
 // one state at N = 248,320 222 / 226, at N = 64,000 59 / 62, four 65 / 66, five 66.2 / 65.8; sixteen 552 / 241).
 constexpr int F8_RAW = 20480;
-inline bool f8_raw(int T, int K, const void* x, long long stride) {
-  return T <= 16 && K % 8 == 0 && ((uintptr_t)x & 15) == 0 && (T == 1 || stride % 8 == 0) && T * f8_up(K, F8_KB) <= F8_RAW;
+inline bool f8_raw(const F8Plan& p, int T, int K, const void* x, long long stride) {
+  return p.groups && p.frags == 1 && K % 8 == 0 && ((uintptr_t)x & 15) == 0 && (T == 1 || stride % 8 == 0) && T * f8_up(K, F8_KB) <= F8_RAW;
 }
 // the packed hidden states: a workgroup's are a tile, 8-bit or (k_f8_tile) bf16
 inline F8Layout f8_states(int T, int N, int K) {
   const F8Plan p = f8_plan(T, N);
-  return p.groups ? f8_layout(T, K, p.frags, 1) : f8_layout(T, K, 2 * p.frags, 2);
+  return p.groups ? f8_layout(T, K, p.frags, 1) : f8_layout(T, K, p.wt * p.frags, 2);
 }
 struct F8Ws {
   size_t part, given, total;
@@ -731,21 +750,22 @@ static void f8_few(const F8Args& a, hipStream_t st) {
   const int raw = RAW ? f8_raw_bytes(a.T, a.lw.kb) : 0, sums = f8_sums<G, TF>();
   hipLaunchKernelGGL((k_f8_few<O, G, TF, RAW>), dim3((a.N + 16 * G - 1) / (16 * G)), dim3(256), raw > sums ? raw : sums, st, a);
 }
-template <typename O, int FN, int FT>
+template <typename O, int FN, int FT, int WT>
 static void f8_tile(const F8Args& a, hipStream_t st) {
-  const int tn = f8_up(a.N, 32 * FN) / (32 * FN), tt = f8_up(a.T, 32 * FT) / (32 * FT);
+  constexpr int BN = 64 / WT * FN, BT = 16 * WT * FT, wgs = WT == 1 ? 2 * F8_CUS : F8_CUS;
+  const int tn = f8_up(a.N, BN) / BN, tt = f8_up(a.T, BT) / BT;
   const long long total = (long long)((tn + 7) / 8 * 8) * tt;
-  hipLaunchKernelGGL((k_f8_tile<O, FN, FT>), dim3(total < F8_CUS ? (int)total : F8_CUS), dim3(256), 0, st, a, tn, tt);
+  hipLaunchKernelGGL((k_f8_tile<O, FN, FT, WT>), dim3(total < wgs ? (int)total : wgs), dim3(256), 0, st, a, tn, tt);
 }
 template <typename O, int FN>
 static void f8_tiles(const F8Args& a, int frags, hipStream_t st) {
   switch (frags) {
-    case 3: return f8_tile<O, FN, 3>(a, st);
-    case 4: return f8_tile<O, FN, 4>(a, st);
-    case 5: return f8_tile<O, FN, 5>(a, st);
-    case 6: return f8_tile<O, FN, 6>(a, st);
-    case 7: return f8_tile<O, FN, 7>(a, st);
-    default: return f8_tile<O, FN, 8>(a, st);
+    case 3: return f8_tile<O, FN, 3, 2>(a, st);
+    case 4: return f8_tile<O, FN, 4, 2>(a, st);
+    case 5: return f8_tile<O, FN, 5, 2>(a, st);
+    case 6: return f8_tile<O, FN, 6, 2>(a, st);
+    case 7: return f8_tile<O, FN, 7, 2>(a, st);
+    default: return f8_tile<O, FN, 8, 2>(a, st);
   }
 }
 // packs the hidden states and runs the product
@@ -753,8 +773,8 @@ template <typename O>
 static int f8_product(F8Args a, int K, const void* x, long long x_stride, char* ws, hipStream_t st) {
   const F8Plan p = f8_plan(a.T, a.N);
   a.parts = p.parts;
-  if (p.groups == 0 && (long long)(p.parts + 7) * (f8_up(a.T, 32 * p.frags) / (32 * p.frags)) > 0x7FFF0000) return QWS_ERR_NOT_SUPPORTED;
-  if (f8_raw(a.T, K, x, x_stride)) {
+  if (p.groups == 0 && (long long)(p.parts + 7) * (f8_up(a.T, p.cols()) / p.cols()) > 0x7FFF0000) return QWS_ERR_NOT_SUPPORTED;
+  if (f8_raw(p, a.T, K, x, x_stride)) {
     a.x = (const char*)x;
     a.x_stride = x_stride;
     f8_few<O, 4, 1, true>(a, st);
@@ -762,7 +782,9 @@ static int f8_product(F8Args a, int K, const void* x, long long x_stride, char* 
   }
   const int e = p.groups ? f8_pack<uint16_t, false>(x, x_stride, a.T, K, a.lx, ws, st) : f8_pack<uint16_t, true>(x, x_stride, a.T, K, a.lx, ws, st);
   if (e) return e;
-  if (p.groups == 0)
+  if (p.groups == 0 && p.wt == 1)
+    p.frags == 2 ? f8_tile<O, 4, 2, 1>(a, st) : f8_tile<O, 4, 4, 1>(a, st);
+  else if (p.groups == 0)
     p.fn == 8 ? f8_tiles<O, 8>(a, p.frags, st) : f8_tiles<O, 4>(a, p.frags, st);
   else if (p.frags == 1)
     f8_few<O, 4, 1, false>(a, st);

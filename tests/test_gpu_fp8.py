@@ -138,6 +138,28 @@ def test_score(T, N, K, temperature):
     assert (again[0].double().cpu().numpy() == lp).all() and (again[1].double().cpu().numpy() == h).all()
 
 
+@pytest.mark.parametrize("T,N,K", [(9, 33001, 130), (16, 40000, 257), (17, 140003, 100), (32, 33025, 384), (33, 32769, 129), (50, 140003, 130), (64, 36000, 640)])
+def test_few_states_of_a_large_head(T, N, K):
+    """More weight rows than 128 tiles of 256, the last one partly filled; more tiles than two a CU among them."""
+    w, x = data(T, N, K, T + N + K)
+    y, tol = product(w, x)
+    head = q.Fp8Head(w.cuda())
+    buf = torch.full((T, N + 9), 7.0, device="cuda")
+    got = head(x.cuda(), out=buf[:, 5:5 + N])
+    err = np.abs(got.double().cpu().numpy() - y)
+    assert (err <= tol).all(), f"off by {(err / tol).max()} of the bound"
+    assert (buf[:, :5] == 7).all() and (buf[:, 5 + N:] == 7).all()
+    assert torch.equal(head(x.cuda(), dtype=torch.bfloat16), got.to(torch.bfloat16))
+    tokens = torch.randint(0, N, (T,), generator=torch.Generator().manual_seed(T)).to(torch.int32)
+    tokens[1], tokens[2], tokens[3] = -1, N, N - 1
+    lp, h = (v.double().cpu().numpy() for v in head.score(x.cuda(), tokens.cuda()))
+    for r in range(T):  # the bounds of test_score
+        want, _, wh, _, _ = L.row(y[r], [int(tokens[r])], 0, 1.0)
+        off, sums = tol[r].max(), (256 + 30) * 2.0 ** -24
+        assert abs(lp[r] - want[0]) <= 2 * off + sums + 8 * abs(want[0]) * 2.0 ** -24, f"row {r}: {lp[r]} {want[0]}"
+        assert abs(h[r] - wh) <= off * (2 * np.log(N) + 2) + sums * (1 + 2 * wh), f"row {r}: entropy {h[r]} {wh}"
+
+
 def test_score_agrees_with_the_logits():
     """score() against LogProbs over the same head's logits, through the package."""
     w, x = data(90, 6000, 512, 9)
