@@ -134,7 +134,8 @@ __device__ __forceinline__ void lp_group_max(float (&m)[U]) {
 
 // A lane's sums over blocks of logits of moderate size (below LSE_MOST in magnitude at their largest, no -inf, no NaN),
 // relative to any reference M = fl(c m) within LP_SLACK of the largest, so that M rarely moves: a multiply-add, an
-// exponential and two sums per logit.  Blocks with anything else go to Lse's general form (lp_slow).
+// exponential and two sums per logit.  Blocks with anything else, and those that would move M to LSE_NEAR or past it (a lane's
+// first tokens all under a mask's -1e9), go to Lse's general form (lp_slow).
 constexpr float LP_SLACK = 8.0f;    // in log2 units: d <= 8, so the entropy's two terms cancel by 8 units at most
 struct LpFast {
   float m, M, limit, s, t;
@@ -142,6 +143,7 @@ struct LpFast {
 template <int U, int E>
 __device__ __forceinline__ bool lp_fast(LpFast& f, const float (&x)[U][E], float best, float c) {
   if (__any(best > f.limit)) {
+    if (__any(best > f.limit && !(fabsf(c * best) < LSE_NEAR))) return false;
     if (best > f.limit) {
       const float M = c * best, d = f.M - M, e = lse_exp2(d);
       f = {best, M, best + LP_SLACK / c, f.s * e, e * fmaf(d, f.s, f.t)};

@@ -46,8 +46,9 @@ __device__ __forceinline__ float lse_max3(float a, float b, float c) {
   return r;
 }
 // Sums of moderate values (below LSE_MOST in magnitude, c as well) relative to M = fl(c m) take one multiply-add for d; what
-// rounding M took, r = c m - M, is given back at the end.
-constexpr float LSE_MOST = 0x1p60f;
+// rounding M took, r = c m - M, is given back at the end.  m itself has d = r, so M stays below LSE_NEAR, where |r| <= 1/2: at
+// 2^31 r passes 64, and from 2^32 on a lane's 2^r is 0 or infinite (at temperature 1e-9, or beside a mask's -1e11).
+constexpr float LSE_MOST = 0x1p60f, LSE_NEAR = 0x1p24f;
 __device__ __forceinline__ Lse lse_exact(float m, float M, float s, float t, float c) {
   const float r = fmaf(c, m, -M), e = lse_exp2(-r);
   return {m, s * e, e * fmaf(-r, s, t)};

@@ -270,3 +270,43 @@ def test_refusals():
                  lambda: op(x, temperature=torch.ones(3, device="cuda")), lambda: op(x, temperature=torch.ones(4)), lambda: op(x.double())):
         with pytest.raises(q.ValidationError):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R", [12, 84])
+def test_small_temperatures(dtype, R):
+    """Ordinary logits at temperatures that a near-greedy request may have, down to 1e-30: a sure row, two equal best logits
+    and two neighbours, in both forms of the pass (one and several vectors of a thread)."""
+    V = 32000
+    x, g = rows(R, V, dtype, 17)
+    x[:, 77] = 20.0
+    x[1::3, 31999] = 20.0
+    x[2::3, 5] = float(np.nextafter(np.float32(20), np.float32(0))) if dtype == torch.float32 else 19.875
+    t = torch.tensor([1e-5, 1e-6, 1e-7, 1e-8, 5e-9, 3e-9, 1e-9, 1e-10, 1e-12, 1e-17, 1e-18, 1e-30]).repeat_interleave(R // 12)
+    tokens = torch.randint(0, V, (R,), generator=g).to(torch.int32)
+    tokens[::2] = 77
+    check(x, tokens, 3, t[torch.randperm(R, generator=g)], "small temperatures")
+    check(x, tokens.view(R, 1).expand(R, 3).contiguous(), 0, t, "small temperatures, several tokens")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R", [12, 84])
+@pytest.mark.parametrize("temperature", [None, 0.7])
+def test_finite_masks(dtype, R, temperature):
+    """All but a dozen tokens masked with a finite value, rows of nothing but that value, and logits as large."""
+    V = 32000
+    x, g = rows(R, V, dtype, 18)
+    values = [-1e4, -1e7, -1e9, -1e10, -5e10, -1e11, -1e12, -1e13, -1e14, -1e15, -1e20, -1e30]
+    few = torch.rand(R, V, generator=g) * V < 12
+    for r in range(R):
+        value = values[r % 12]
+        if r < 60:
+            x[r, ~few[r]] = value
+        elif r < 72:
+            x[r] = value
+        else:
+            x[r] *= -value
+    tokens = torch.randint(0, V, (R,), generator=g).to(torch.int32)
+    tokens[::2] = torch.where(few, x.float(), -INF).argmax(1)[::2].to(torch.int32)
+    t = torch.full((R,), temperature) if temperature else None
+    check(x, tokens, 5, t, "finite masks", 1, 3)
