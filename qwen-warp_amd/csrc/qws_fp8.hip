@@ -220,9 +220,9 @@ __device__ __forceinline__ Lse f8_stats(const F8Args& a, const vf4* y, int t, in
       s += e;
       q = fmaf(e, d, q);
     }
-  if (n0 + 16 * F <= a.N && __all(fabsf(m) < LSE_MOST && c <= LSE_MOST && fabsf(q) < INFINITY)) {
+  if (n0 + 16 * F <= a.N && __all(fabsf(M) < LSE_NEAR && c <= LSE_MOST && fabsf(q) < INFINITY)) {
     v = lse_exact(m, M, s, q, c);
-  } else {  // rows behind the last, NaN or extreme logits
+  } else {  // rows behind the last, NaN or extreme logits, small temperatures
     v = {-INFINITY, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < F; i++)

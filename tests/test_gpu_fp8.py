@@ -237,3 +237,26 @@ def test_refusals():
                  lambda: head.score(x, i32, temperature=torch.ones(4))):
         with pytest.raises(q.ValidationError):
             call()
+
+
+@pytest.mark.parametrize("T,N,K", [(1, 8191, 130), (7, 1000, 256), (12, 33001, 130), (24, 4000, 300), (40, 33001, 64), (40, 5000, 64), (80, 3001, 384)])
+def test_score_small_temperatures(T, N, K):
+    """Temperatures down to 1e-30 and large logits, against the definition over the head's own logits (the same products in
+    the same order)."""
+    w, x = data(T, N, K, T + N)
+    temps = torch.tensor([1e-5, 1e-6, 1e-7, 1e-8, 5e-9, 3e-9, 1e-9, 1e-10, 1e-12, 1e-17, 1e-18, 1e-30])
+    head = q.Fp8Head(w.cuda())
+    y = head(x.cuda()).double().cpu().numpy()
+    tokens = torch.randint(0, N, (T,), generator=torch.Generator().manual_seed(T)).to(torch.int32)
+    tokens[::2] = torch.from_numpy(y.argmax(1)[::2])
+    for i in range(14):  # each temperature alone (a wave takes one form for all its states), then mixed ones, then large logits
+        t = torch.ones(T) if i == 13 else temps.repeat(T)[:T] if i == 12 else temps[i].repeat(T)
+        if i == 13:
+            x = (x.float() * 2.0 ** 36).to(torch.bfloat16)
+            y = head(x.cuda()).double().cpu().numpy()
+        lp, h = (v.double().cpu().numpy() for v in head.score(x.cuda(), tokens.cuda(), temperature=t.cuda()))
+        for r in range(T):
+            want, _, wh, _, _ = L.row(y[r], [int(tokens[r])], 0, float(t[r]))
+            sums = (256 + 30) * 2.0 ** -24
+            assert abs(lp[r] - want[0]) <= sums + 8 * abs(want[0]) * 2.0 ** -24, f"row {r} at {float(t[r])}: {lp[r]} {want[0]}"
+            assert abs(h[r] - wh) <= sums * (1 + 2 * wh), f"row {r} at {float(t[r])}: entropy {h[r]} {wh}"
