@@ -6,9 +6,9 @@
 // A larger maximum m' (delta = c (m' - m)) turns them into 2^-delta s and 2^-delta (t - delta s): one pass, any order.
 // Then
 //   log p_i = (x_i - m) / T - ln s,   H = ln s - ln 2 * t / s.
-// With m the largest x both terms of H are >= 0 (s >= 1, t <= 0): nothing cancels.  m may be any value near it instead: with
-// one that lies up to 8 units of d below (k_lp_scan's, so that it rarely moves) the terms cancel by at most 8 ln 2 = 5.5, an
-// error of a few 5.5 * 2^-24 in H.
+// With m the largest x both terms of H are >= 0 (s >= 1, t <= 0; either may be off by a rounding): nothing cancels.  m may be
+// any value near it instead: with one that lies up to 8 units of d below (k_lp_scan's, so that it rarely moves) the terms cancel
+// by at most 8 ln 2 = 5.5, an error of a few 5.5 * 2^-24 in H.
 // The general form takes differences to m before the scaling, so rows at the type's lowest value and rows mixing it with
 // -inf are exact; NaN counts as -inf (the sampling stage's rule), +inf as the largest finite value (so tokens at +inf share
 // the row); d is held above -D_MIN, where 2^d is 0 in fp32: no infinity meets a 0 in t.
@@ -69,8 +69,15 @@ __device__ inline Lse lse_join_lanes(Lse v, float c, int from, int to) {  // but
   return v;
 }
 __device__ __forceinline__ float lse_log(Lse v) { return logf(v.s); }
-// log p of a (clean) logit; -inf for a masked one and in a row without a candidate
-__device__ __forceinline__ float lse_logprob(Lse v, float x, float T) { return x == -INFINITY ? -INFINITY : (x - v.m) / lse_temp(T) - lse_log(v); }
-__device__ __forceinline__ float lse_entropy(Lse v) { return v.m == -INFINITY ? 0.0f : lse_log(v) - LN2 * (v.t / v.s); }
+// log p of a (clean) logit; -inf for a masked one and in a row without a candidate.  Neither it nor the entropy leaves its range
+// where the sums are off by a rounding (a sure token's s = 1 - 2^-24); a NaN would pass.
+__device__ __forceinline__ float lse_logprob(Lse v, float x, float T) {
+  const float p = x == -INFINITY ? -INFINITY : (x - v.m) / lse_temp(T) - lse_log(v);
+  return p > 0.0f ? 0.0f : p;
+}
+__device__ __forceinline__ float lse_entropy(Lse v) {
+  const float h = v.m == -INFINITY ? 0.0f : lse_log(v) - LN2 * (v.t / v.s);
+  return h < 0.0f ? 0.0f : h;
+}
 
 }  // namespace qws

@@ -260,3 +260,16 @@ def test_score_small_temperatures(T, N, K):
             sums = (256 + 30) * 2.0 ** -24
             assert abs(lp[r] - want[0]) <= sums + 8 * abs(want[0]) * 2.0 ** -24, f"row {r} at {float(t[r])}: {lp[r]} {want[0]}"
             assert abs(h[r] - wh) <= sums * (1 + 2 * wh), f"row {r} at {float(t[r])}: entropy {h[r]} {wh}"
+
+
+@pytest.mark.parametrize("T,N", [(1, 9000), (8, 4000), (16, 33001), (32, 4000), (64, 33001), (64, 4000), (200, 4000)])
+def test_score_signs(T, N):
+    """No log probability above 0 and no entropy below 0 where a token is sure, at many temperatures."""
+    w, x = data(T, N, 256, T)
+    likely = torch.arange(T) * 7 % N
+    x = (x.float() + 600 * w[likely].float()).to(torch.bfloat16)
+    head = q.Fp8Head(w.cuda())
+    for t in (None, torch.full((T,), 0.37), 0.05 + torch.rand(T, generator=torch.Generator().manual_seed(T))):
+        lp, h = head.score(x.cuda(), likely.to(torch.int32).cuda(), temperature=t.cuda() if t is not None else None)
+        assert (lp <= 0).all() and (h >= 0).all()
+        assert T == 1 or (lp > -0.1).float().mean() > 0.5  # mostly sure ones

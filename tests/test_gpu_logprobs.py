@@ -310,3 +310,16 @@ def test_finite_masks(dtype, R, temperature):
     tokens[::2] = torch.where(few, x.float(), -INF).argmax(1)[::2].to(torch.int32)
     t = torch.full((R,), temperature) if temperature else None
     check(x, tokens, 5, t, "finite masks", 1, 3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [None, 0.37])
+def test_signs(dtype, temperature):
+    """No log probability above 0 and no entropy below 0: rows with one sure token, whose best logits differ, and rows of one token."""
+    for R, V in ((400, 1500), (300, 30011), (64, 1)):
+        x, g = rows(R, V, dtype, 19)
+        x[:, V // 2] = (60.0 + 10 * torch.rand(R, generator=g)).to(dtype)
+        tokens = torch.full((R,), V // 2, dtype=torch.int32)
+        t = torch.full((R,), temperature) if temperature else None
+        out = check(x, tokens, 2, t, "signs")
+        assert (out.logprobs <= 0).all() and (out.top_logprobs <= 0).all() and (out.entropy >= 0).all()
