@@ -324,16 +324,23 @@ __global__ void __launch_bounds__(LP_NT, lp_waves<T>(U)) k_lp_scan(LpArgs a) {
       least = fminf(least, top[u]);
     }
     if (!(moderate && __all(best < LSE_MOST && least > -LSE_MOST)) || !lp_fast(f, x, best, c)) {
-      best = -INFINITY;
+      bool unclean = best == INFINITY;  // or a NaN: else the values and their largest are right as they are
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        top[u] = -INFINITY;
+      for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int j = 0; j < E; j++) {
-          x[u][j] = lse_clean(x[u][j]);
-          top[u] = fmaxf(top[u], x[u][j]);
+        for (int j = 0; j < E; j += 2) unclean = unclean || __builtin_isunordered(x[u][j], x[u][j + 1]);
+      if (__any(unclean)) {
+        best = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          top[u] = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < E; j++) {
+            x[u][j] = lse_clean(x[u][j]);
+            top[u] = fmaxf(top[u], x[u][j]);
+          }
+          best = fmaxf(best, top[u]);
         }
-        best = fmaxf(best, top[u]);
       }
       lp_slow(v, x, best, c);
     }

@@ -26,13 +26,13 @@ struct Lse {
 };
 
 __device__ __forceinline__ float lse_exp2(float d) { return __builtin_amdgcn_exp2f(d); }
-// NaN -> -inf (the median of three with a NaN is the smaller of the others), +inf -> the largest finite value.  The -inf
-// comes from a register that the compiler does not see through: it would fold the median into min(x, F32_MAX), whose
-// answer for NaN is F32_MAX.
+// NaN -> -inf (the median of three with a quiet NaN is the smaller of the others; with a signalling one it is not, so x is
+// quieted first), +inf -> the largest finite value.  The -inf comes from a register that the compiler does not see through: it
+// would fold the median into min(x, F32_MAX), whose answer for NaN is F32_MAX.
 __device__ __forceinline__ float lse_clean(float x) {
   float lowest;
   asm("s_mov_b32 %0, 0xff800000" : "=s"(lowest));
-  return __builtin_amdgcn_fmed3f(x, lowest, F32_MAX);
+  return __builtin_amdgcn_fmed3f(__builtin_canonicalizef(x), lowest, F32_MAX);
 }
 __device__ __forceinline__ float lse_temp(float T) { return T > 0.0f ? T : 1.0f; }  // 0 (a greedy row) and NaN: as T = 1
 __device__ __forceinline__ float lse_scale(float T) { return fminf((float)LOG2E / lse_temp(T), F32_MAX); }

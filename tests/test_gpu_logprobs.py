@@ -323,3 +323,24 @@ def test_signs(dtype, temperature):
         t = torch.full((R,), temperature) if temperature else None
         out = check(x, tokens, 2, t, "signs")
         assert (out.logprobs <= 0).all() and (out.top_logprobs <= 0).all() and (out.entropy >= 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R", [6, 180])
+def test_signalling_nan(dtype, R):
+    """NaN of both kinds and signs counts as -inf: as a given token, among the best, in a row of nothing else, in both forms of the pass."""
+    V = 16001
+    ints, codes = (torch.int32, (0x7F800001, -0x7FFFFF, 0x7FBFFFFF, 0x7FC00000, -1)) if dtype == torch.float32 else (torch.int16, (0x7F81, -0x7F, 0x7FBF, 0x7FC0, -1))
+    x, g = rows(R, V, dtype, 20)
+    for r in range(R):
+        bits = x[r].view(ints)
+        if r % 6 == 5:
+            bits[:] = codes[r // 6 % 5]
+            if r % 12 == 11:
+                x[r, 9000] = -2.0
+        else:
+            bits[[0, 63, 64, 777, 1023, 9000, 16000]] = codes[r % 5]
+    assert x.isnan().sum() > 7 * R // 2
+    tokens = torch.tensor([[0, 777, 5, 16000]], dtype=torch.int32).repeat(R, 1)
+    check(x, tokens, 3, None, "signalling NaN", 1, 1)
+    check(x, tokens[:, 1].contiguous(), 3, torch.full((R,), 0.6), "signalling NaN, one token")
