@@ -332,7 +332,7 @@ const float* qws_head_ws_exact(const void* ws);
  * As in qws_sample, NaN logits count as -inf.  Several logits at +inf share the row's probability.  A given token at -inf,
  * or in a row without a candidate, has log probability -inf; a token outside [0, V) (the -1 behind a verify call's
  * accepted tokens) is skipped: log probability 0, rank -1.  Sums and statistics are fp32.
- * Limits: V <= 524,288, M <= 64 and top <= 64 (else QWS_ERR_NOT_SUPPORTED).  out_logprobs is needed with M > 0,
+ * Limits: R < 2^24, V <= 524,288, M <= 64 and top <= 64 (else QWS_ERR_NOT_SUPPORTED).  out_logprobs is needed with M > 0,
  * out_top_* with top > 0; the others are optional.  Zero-initialise the struct.  ws: qws_logprobs_ws_bytes(dtype, R, V, M,
  * top) bytes of device memory, 256-byte aligned, no zeroing needed; calls that share one must be ordered.  Allocates
  * nothing; two launches; deterministic.  No counterpart in the reference, whose server refuses `logprobs`

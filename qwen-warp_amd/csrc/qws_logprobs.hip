@@ -28,6 +28,7 @@ constexpr int LP_GRP = 64;      // consecutive logits of a group
 constexpr int LP_NMAX = 64;     // alternatives and given tokens of a row at most
 constexpr int LP_VMAX = 1 << 19;
 constexpr int LP_CUS = 256;
+constexpr int LP_WGS = (int)((1ll << 32) / LP_NT - 1);  // workgroups of a launch at most: below 2^32 threads
 constexpr int LP_U = 4;         // vectors of a thread loaded together, where it has more than one
 
 template <typename T>
@@ -595,6 +596,7 @@ __global__ void __launch_bounds__(LP_NT) k_lp_row(LpArgs a) {
 struct LpPlan {
   int G, per, groups;
   size_t part, cnt, gmax, total;  // byte offsets
+  bool fits(int R) const { return (long long)R * G <= LP_WGS; }
 };
 // Stripes of a workgroup: one while the card holds them all at once; then four (a block), eight, and as many as leave eight
 // rounds of workgroups, so that the last round is a small part (2,048 bf16 rows of 248,320: 257 us with one round of whole
@@ -636,7 +638,8 @@ void lp_launch_scan(const LpArgs& a, int R, hipStream_t st) {
 template <typename T>
 int lp_launch(LpArgs a, int R, char* ws, size_t ws_bytes, hipStream_t st) {
   const LpPlan q = lp_plan<T>(R, a.V, a.M, a.top);
-  if (ws_bytes < q.total || (uint64_t)R * q.G > 0x7FFFFFFFull) return ws_bytes < q.total ? QWS_ERR_INVALID : QWS_ERR_NOT_SUPPORTED;
+  if (!q.fits(R)) return QWS_ERR_NOT_SUPPORTED;
+  if (ws_bytes < q.total) return QWS_ERR_INVALID;
   a.G = q.G;
   a.per = q.per;
   a.groups = q.groups;
@@ -665,8 +668,9 @@ static_assert(sizeof(qws_logprobs_batch) == 96 && offsetof(qws_logprobs_batch, t
 extern "C" size_t qws_logprobs_ws_bytes(int dtype, int R, int V, int M, int top) {
   using namespace qws;
   if (R < 1 || V < 1 || V > LP_VMAX || M < 0 || M > LP_NMAX || top < 0 || top > LP_NMAX) return 0;
-  if (dtype == QWS_DTYPE_F32) return lp_plan<float>(R, V, M, top).total;
-  return dtype == QWS_DTYPE_BF16 ? lp_plan<uint16_t>(R, V, M, top).total : 0;
+  if (dtype != QWS_DTYPE_F32 && dtype != QWS_DTYPE_BF16) return 0;
+  const LpPlan q = dtype == QWS_DTYPE_F32 ? lp_plan<float>(R, V, M, top) : lp_plan<uint16_t>(R, V, M, top);
+  return q.fits(R) ? q.total : 0;
 }
 
 extern "C" int qws_logprobs(const qws_logprobs_batch* b, void* ws, size_t ws_bytes, void* stream) {

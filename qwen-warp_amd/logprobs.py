@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -13,6 +14,7 @@ from ._lib import check
 from .sampling import ValidationError
 
 LOGPROBS_MAX = 64  # given tokens and alternatives of a row at most
+INT_MAX = 2 ** 31 - 1
 
 
 class LogProbsResult(NamedTuple):
@@ -24,10 +26,12 @@ class LogProbsResult(NamedTuple):
 
 
 def rows_of(x: torch.Tensor, name: str):
-    """(rows, stride) of a tensor [..., n] read as rows of n contiguous elements at one stride."""
+    """(rows, stride) of a tensor [..., n] read as rows of n contiguous elements at one stride.  Both counts fit an int."""
     shape, strides = x.shape, x.stride()
     if len(shape) < 2 or (shape[-1] > 1 and strides[-1] != 1):
         raise ValidationError(f"{name} must be [..., n] with contiguous rows", name)
+    if max(shape) > INT_MAX or (len(shape) > 2 and math.prod(shape[:-1]) > INT_MAX):
+        raise ValidationError(f"{name}: at most 2^31 - 1 rows of as many elements", name)
     if len(shape) == 2:
         return shape[0], strides[0] if shape[0] > 1 else 0
     rows, stride = 1, 0

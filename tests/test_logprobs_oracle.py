@@ -142,3 +142,17 @@ def test_rows_of():
     for bad in (x[:, :3], x.transpose(1, 2), torch.zeros(10), torch.zeros(1, 10).expand(6, 10).view(2, 3, 10).transpose(0, 1)[..., ::2]):
         with pytest.raises(q.ValidationError):
             rows_of(bad, "x")
+
+
+def test_row_counts_past_the_ranges(lib):
+    """More workgroups than a launch has threads for, and counts that do not fit the entry points' int."""
+    most = (1 << 24) - 1  # workgroups of 256 threads below 2^32 threads
+    for dtype, V in ((0, 1), (0, 1000), (1, 2000), (1, 1)):
+        over = most + 1
+        assert lib.qws_logprobs(C.byref(_batch(R=over, V=V, dtype=dtype)), P, 1 << 62, None) == _lib.ERR_NOT_SUPPORTED
+        assert lib.qws_logprobs_ws_bytes(dtype, over, V, 1, 3) == 0 and lib.qws_logprobs_ws_bytes(dtype, most, V, 1, 3) > 0
+    one = torch.zeros(1, 1)
+    for bad in (one.expand(1 << 31, 1), one.expand((1 << 32) + 2, 1), one.view(1, 1, 1).expand(1 << 16, 1 << 16, 1), torch.empty(2, 1 << 31, device="meta")):
+        with pytest.raises(q.ValidationError):
+            rows_of(bad, "x")
+    assert rows_of(one.expand((1 << 31) - 1, 1), "x") == ((1 << 31) - 1, 0)
