@@ -71,7 +71,8 @@ class LogProbs:
 
     logits: fp32 or bf16 [..., V] on the GPU, rows contiguous, at any stride.  tokens: int32 [...] (one token a row: those
     that `Sampler` returned; -1 = skipped: log probability 0, rank -1) or [..., M] (several: labels); None: no tokens.
-    temperature: fp32 [...] (0: as 1) or None.  ranks=False leaves the ranks out."""
+    temperature: fp32 [...] (0: as 1) or None.  ranks=False leaves the ranks out.  device: the logits'; without an index,
+    any GPU's."""
 
     def __init__(self, device="cuda"):
         self.lib = _lib.load()
@@ -83,6 +84,8 @@ class LogProbs:
         dtype, dev = logits.dtype, logits.device
         if not logits.is_cuda or (dtype != torch.float32 and dtype != torch.bfloat16):
             raise ValidationError("logits must be a CUDA fp32 / bf16 tensor", "logits")
+        if dev != self.device and (self.device.type != "cuda" or self.device.index is not None):
+            raise ValidationError(f"logits must be on {self.device}", "logits")
         R, stride = rows_of(logits, "logits")
         lead, V, top = logits.shape[:-1], logits.shape[-1], int(top)
         if V < 1 or not 0 <= top <= LOGPROBS_MAX:

@@ -344,3 +344,13 @@ def test_signalling_nan(dtype, R):
     tokens = torch.tensor([[0, 777, 5, 16000]], dtype=torch.int32).repeat(R, 1)
     check(x, tokens, 3, None, "signalling NaN", 1, 1)
     check(x, tokens[:, 1].contiguous(), 3, torch.full((R,), 0.6), "signalling NaN, one token")
+
+
+def test_device():
+    """The operator's device is the logits': another one's are refused; without an index, any GPU's are taken."""
+    x = torch.zeros(2, 50, device="cuda:0")
+    want = q.LogProbs("cuda")(x)
+    assert torch.equal(q.LogProbs("cuda:0")(x).entropy, want.entropy) and torch.equal(q.LogProbs(torch.device("cuda", 0))(x).entropy, want.entropy)
+    for other in ("cpu", "cuda:1"):
+        with pytest.raises(q.ValidationError):
+            q.LogProbs(other)(x)
