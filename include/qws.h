@@ -358,7 +358,9 @@ int qws_logprobs(const qws_logprobs_batch* b, void* ws, size_t ws_bytes, void* s
  * head product, engine/src/head_q.cu:15-100, in another format), and scoring.  Each block of 128 consecutive values of a row
  * along K (the last may be shorter) is e4m3 values times 2^e, e the least whole number >= -127 with max|x| <= 448 * 2^e;
  * values are rounded to nearest even; a value that is not finite makes its row's products NaN.  Weights are packed once,
- * hidden states (bf16) within each call:  y[t][n] = sum over blocks of 2^(ex + ew) * sum_k qx qw, in fp32.
+ * hidden states (bf16) within each call:  y[t][n] = sum over blocks of 2^(ex + ew) * sum_k qx qw, in fp32.  The values
+ * enter the products in bf16, whose least one is 2^-133: in a block of fp32 weights with e < -124 (none above 1.06e-35) they
+ * are rounded to multiples of it.
  *   qws_fp8_pack:  w [N][K] (dtype QWS_DTYPE_*, rows row_stride elements apart) -> packed (device, qws_fp8_pack_bytes(N, K)
  *                  bytes, 256-byte aligned): about N * K * 65 / 64 bytes, N and K padded to multiples of 256 and 128.
  *   qws_fp8_head:  x [T][K] bf16 (rows x_stride elements apart) -> out [T][N] (fp32 or bf16, rows out_stride >= N apart).

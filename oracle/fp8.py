@@ -2,7 +2,8 @@
 
 A block of 128 consecutive values of a row (the last may be shorter) is q * 2^e: e the least whole number >= -127 with
 max|x| <= 448 * 2^e, q = x / 2^e rounded to the nearest e4m3 value (sign, 4 exponent bits of bias 7, 3 fraction bits,
-subnormals of 2^-9; ties to the even fraction).  A value that is not finite becomes NaN."""
+subnormals of 2^-9; ties to the even fraction).  The value is then held in bf16, which takes something from it only below
+2^-133, bf16's least value (e < -124: nearest, ties to even).  A value that is not finite becomes NaN."""
 import numpy as np
 
 BLOCK = 128
@@ -40,4 +41,5 @@ def values(x):
     bad = ~np.isfinite(x)
     x = np.where(bad, 0.0, x)
     e = np.repeat(block_exponents(x), BLOCK, 1)[:, :x.shape[1]]
-    return np.where(bad, np.nan, np.ldexp(round_e4m3(np.ldexp(x, -e)), e))
+    v = np.ldexp(round_e4m3(np.ldexp(x, -e)), e)
+    return np.where(bad, np.nan, np.ldexp(np.rint(np.ldexp(v, 133)), -133))

@@ -7,8 +7,9 @@
 // Why the products run on the bf16 matrix instruction.  The 8-bit ones (16x16x32 and 16x16x128, with and without scales)
 // align a group's products to the largest and cut what lies about 2^-13 below it: measured over 128 products of normal
 // data 1.4e-5 of the result's norm, and ten times that with a few large columns.  e4m3 values times a power of two are
-// exact in bf16, whose instruction sums exact products in fp32 (measured 7e-8).  v_cvt_scalef32_pk_bf16_fp8 turns two
-// values and their block's scale into bf16 at the rate of any vector instruction, so the scales cost nothing more.
+// exact in bf16 (down to its least, 2^-133), whose instruction sums exact products in fp32 (measured 7e-8).
+// v_cvt_scalef32_pk_bf16_fp8 turns two values and their block's scale into bf16 at the rate of any vector instruction, so the
+// scales cost nothing more.
 //
 // Layout.  16 rows x 64 values are a fragment of 1 KB: lane l's 16 bytes are row l % 16, values 16 (l / 16) .. + 15, the
 // operands of two 16x16x32 products.  (Which 32 of the values share a product does not matter, as long as both operands
@@ -51,7 +52,8 @@ __host__ __device__ inline F8Layout f8_layout(int rows, int K, int groups, int b
 }
 __host__ __device__ inline F8Layout f8_weights(int N, int K) { return f8_layout(N, K, F8_ROWS / 16, 1); }
 
-// bf16 operand of product h (0, 1) of a fragment's 16 bytes, times the block's scale
+// bf16 operand of product h (0, 1) of a fragment's 16 bytes, times the block's scale.  Of the scale the instruction reads the
+// exponent bits alone: none set (0.0f as a number, biased exponent 0) is 2^-127, as any others are theirs.
 template <int H>
 __device__ __forceinline__ f8_b8 f8_wide(vu4 r, float scale) {
   union {

@@ -273,3 +273,38 @@ def test_score_signs(T, N):
         lp, h = head.score(x.cuda(), likely.to(torch.int32).cuda(), temperature=t.cuda() if t is not None else None)
         assert (lp <= 0).all() and (h >= 0).all()
         assert T == 1 or (lp > -0.1).float().mean() > 0.5  # mostly sure ones
+
+
+@pytest.mark.parametrize("wdtype", [torch.float32, torch.bfloat16])
+def test_smallest_scales(wdtype):
+    """Blocks whose largest value is 2^-95 down to the type's least, ties among them, as weights and as hidden states, by every
+    kernel that widens them: read back exactly."""
+    K = 128
+    g = torch.Generator().manual_seed(14)
+    least = -149 if wdtype == torch.float32 else -133
+    rows = range(-95, least - 1, -1)
+    v = torch.randn(len(rows), K, generator=g, dtype=torch.float64)
+    v[:, 0], v[:, 1:40], v[:, 40:60], v[:, 60:90] = 1.0, v[:, 1:40] * 2.0 ** -6, torch.arange(1, 21) * 2.0 ** -10, torch.arange(1, 31) * 2.0 ** -5
+    v = (v.clamp(-1, 1) * 2.0 ** torch.tensor(list(rows), dtype=torch.float64).view(-1, 1)).to(wdtype)
+    want = F.values(v.double().numpy())
+    eye = torch.eye(K, dtype=torch.bfloat16, device="cuda")
+    wide = torch.zeros(33000, K, dtype=wdtype, device="cuda")
+    wide[:len(rows)] = v.cuda()
+    odd = torch.zeros(K, K + 1, dtype=torch.bfloat16, device="cuda")[:, :K]  # rows that k_f8_few does not take as they are
+    odd.copy_(eye)
+    for w, T in ((v.cuda(), (1, 8, 16, 32, 64, 128)), (wide, (16, 64, 128))):
+        head = q.Fp8Head(w)
+        for x in (eye, odd):
+            for t in T:
+                got = torch.cat([head(x[i:i + t]) for i in range(0, K, t)]).t()[:len(rows)].double().cpu().numpy()
+                assert (got == want).all(), f"{t} states of {w.shape[0]} rows: {np.abs(got - want).max(1)}"
+    if wdtype == torch.bfloat16:  # hidden states of that size
+        x = torch.zeros(128, K, dtype=wdtype, device="cuda")
+        x[:len(rows)] = v.cuda()
+        unit = torch.zeros(33000, K, dtype=wdtype, device="cuda")
+        unit[:K] = eye
+        for w in (eye, unit):
+            head = q.Fp8Head(w)
+            for t in (1, 8, 16, 32, 64, 128):
+                got = torch.cat([head(x[i:i + t])[:, :K] for i in range(0, 128, t)])[:len(rows)].double().cpu().numpy()
+                assert (got == want).all(), f"hidden states, {t} at {w.shape[0]} rows"
