@@ -308,3 +308,45 @@ def test_smallest_scales(wdtype):
             for t in (1, 8, 16, 32, 64, 128):
                 got = torch.cat([head(x[i:i + t])[:, :K] for i in range(0, 128, t)])[:len(rows)].double().cpu().numpy()
                 assert (got == want).all(), f"hidden states, {t} at {w.shape[0]} rows"
+
+
+# Each instance of the kernel for many hidden states (waves of 16 FN weight rows x 16 FT states, two by two), by sizes that
+# f8_plan gives to it: in one round of workgroups, and with more than 256 tiles, so that workgroups take a second one, whose
+# copies start under the first one's end.  No size is a multiple of a tile's.
+TILES = {(4, 3): ((90, 16449, 257), (70, 65601, 130)), (4, 4): ((100, 16449, 257), (100, 65601, 100)), (4, 5): ((131, 16449, 130), (131, 65601, 130)),
+         (4, 6): ((170, 16449, 384), (170, 65601, 130)), (4, 7): ((200, 22081, 130), (200, 65601, 100)), (4, 8): ((230, 22081, 257), (230, 65601, 130)),
+         (8, 3): ((70, 32833, 130), (70, 100001, 100)), (8, 4): ((100, 32833, 257), (290, 32833, 130)), (8, 5): ((140, 32833, 130), (390, 32833, 100)),
+         (8, 6): ((165, 32833, 384), (485, 32833, 130)), (8, 7): ((200, 32833, 130), (390, 49217, 100)), (8, 8): ((240, 43585, 130), (680, 32833, 257))}
+
+
+@pytest.mark.parametrize("FN,FT,T,N,K", [(*k, *s) for k, v in TILES.items() for s in v])
+def test_many_states(FN, FT, T, N, K):
+    w, x = data(T, N, K, T + N + K)
+    y, tol = product(w, x)
+    head = q.Fp8Head(w.cuda())
+    buf = torch.full((T, N + 9), 7.0, device="cuda")
+    got = head(x.cuda(), out=buf[:, 5:5 + N])
+    err = np.abs(got.double().cpu().numpy() - y)
+    assert (err <= tol).all(), f"off by {(err / tol).max()} of the bound"
+    assert (buf[:, :5] == 7).all() and (buf[:, 5 + N:] == 7).all()
+    wide = torch.full((T, N + 9), 7.0, dtype=torch.bfloat16, device="cuda")
+    half = head(x.cuda(), out=wide[:, 3:3 + N])
+    assert torch.equal(half, got.to(torch.bfloat16)) and (wide[:, :3] == 7).all() and (wide[:, 3 + N:] == 7).all()
+    assert torch.equal(head(x.cuda(), dtype=torch.bfloat16), half)
+    g = torch.Generator().manual_seed(T)
+    tokens = torch.randint(0, N, (T,), generator=g).to(torch.int32)
+    tokens[1], tokens[2], tokens[3], tokens[-1] = -1, N, N - 1, 0
+    t = 0.3 + 2 * torch.rand(T, generator=g)
+    for temperature in (None, t):
+        lp, h = (v.double().cpu().numpy() for v in head.score(x.cuda(), tokens.cuda(), temperature=temperature.cuda() if temperature is not None else None))
+        assert np.isfinite(lp).all() and np.isfinite(h).all()
+        for r in sorted({*range(5), *range(5, T, 13), *range(T - 5, T)}):  # the bounds of test_score
+            temp = 1.0 if temperature is None else float(t[r])
+            want, _, wh, _, _ = L.row(y[r], [int(tokens[r])], 0, temp)
+            off, sums = tol[r].max() / temp, (256 + 30) * 2.0 ** -24
+            assert abs(lp[r] - want[0]) <= 2 * off + sums + 8 * abs(want[0]) * 2.0 ** -24, f"row {r}: {lp[r]} {want[0]}"
+            assert abs(h[r] - wh) <= off * (2 * np.log(N) + 2) + sums * (1 + 2 * wh), f"row {r}: entropy {h[r]} {wh}"
+        # every row against the log probabilities of the same logits
+        same = q.LogProbs("cuda")(got, tokens.cuda(), temperature=temperature.cuda() if temperature is not None else None)
+        assert torch.allclose(torch.from_numpy(lp).float(), same.logprobs.cpu(), atol=5e-5, rtol=1e-5)
+        assert torch.allclose(torch.from_numpy(h).float(), same.entropy.cpu(), atol=5e-5, rtol=1e-5)
