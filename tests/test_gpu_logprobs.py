@@ -354,3 +354,64 @@ def test_device():
     for other in ("cpu", "cuda:1"):
         with pytest.raises(q.ValidationError):
             q.LogProbs(other)(x)
+
+
+# Rows and vocabularies by the stripes that a workgroup then takes (lp_plan): one, a block of them, two, more, and as many as a
+# short row has.  The last workgroup of a row is partly filled in most.
+@pytest.mark.parametrize("dtype,R,V,stripes", [(torch.float32, 20, 62465, 1), (torch.float32, 70, 62465, 4), (torch.float32, 400, 62465, 8), (torch.float32, 2200, 62465, 12),
+                                               (torch.float32, 1024, 248321, 16), (torch.float32, 3000, 3000, 4), (torch.float32, 3000, 1000, 1),
+                                               (torch.bfloat16, 20, 62465, 1), (torch.bfloat16, 100, 62465, 4), (torch.bfloat16, 400, 62465, 8),
+                                               (torch.bfloat16, 2700, 62465, 12), (torch.bfloat16, 2048, 248321, 28), (torch.bfloat16, 3000, 3000, 4), (torch.bfloat16, 3000, 1000, 1)])
+def test_plans(dtype, R, V, stripes):
+    """Every form of the pass (no tokens, one, several; ranks or not; alternatives or not) over ordinary, masked and NaN rows.  A
+    lane's chain is its share of the workgroup's stripes; the other roundings are those of the bound above."""
+    pad, offset = 3, 5
+    g = torch.Generator(device="cuda").manual_seed(R + V)
+    buf = torch.full((R * (V + pad) + offset + 16,), float("nan"), dtype=dtype, device="cuda")
+    y = buf[offset:offset + R * (V + pad)].view(R, V + pad)[:, :V]
+    y.normal_(0, 3, generator=g)
+    few = torch.rand(V, device="cuda", generator=g) * V < 12
+    y[5::11, ~few] = -INF
+    y[7::11, ~few] = torch.finfo(dtype).min
+    y[9::11, ~few] = -1e9
+    y[3::11, ::7] = float("nan")
+    y[2] = -INF
+    tokens = torch.randint(0, V, (R, 3), device="cuda", generator=g).to(torch.int32)
+    for r in range(0, R, 2):
+        tokens[r, 0] = y[r].nan_to_num(nan=-INF).argmax()
+    tokens[::5, 2] = -1
+    tokens[1::5, 2] = V - 1
+    t = 0.4 + 2 * torch.rand(R, device="cuda", generator=g)
+    rows_ = sorted({*range(14), R // 2, *range(R - 6, R)})
+    n = stripes * 16 // dtype.itemsize + 64 + 66
+    op = q.LogProbs("cuda")
+    for temperature in (None, t):
+        want = {r: L.row(y[r].double().cpu().numpy(), tokens[r].tolist(), 6, 1.0 if temperature is None else float(t[r])) for r in rows_}
+
+        def near(got, of, r, what):
+            got = np.atleast_1d(got.double().cpu().numpy())
+            of = np.atleast_1d(of).astype(np.float32).astype(np.float64)
+            fine = np.isfinite(of)
+            assert (got[~fine] == of[~fine]).all(), f"row {r}: {what}"
+            assert (np.abs(got[fine] - of[fine]) <= (n + 30 + 6 * np.abs(of[fine])) * U).all(), f"row {r}: {what} {got} {of}"
+
+        for M in (0, 1, 3):
+            for ranks in (True, False):
+                if not M and not ranks:
+                    continue
+                for top in (0, 6):
+                    given = None if not M else tokens[:, 0].contiguous() if M == 1 else tokens
+                    out = op(y, given, top=top, temperature=temperature, ranks=ranks)
+                    at = f"M={M} ranks={ranks} top={top}"
+                    assert (out.logprobs is None) == (M == 0) and (out.ranks is None) == (not ranks or not M) and out.top_ids.shape == (R, top)
+                    assert torch.isfinite(out.entropy).all() and (out.entropy >= 0).all()
+                    for r in rows_:
+                        lp, rank, h, ids, tlp = want[r]
+                        assert abs(float(out.entropy[r]) - h) <= (n * (1 + 2 * h) + 6 * h) * U, f"{at} row {r}: entropy {float(out.entropy[r])} {h}"
+                        if M:
+                            near(out.logprobs[r], lp[:M], r, at)
+                            if ranks:
+                                assert out.ranks[r].view(-1).tolist() == rank[:M].tolist(), f"{at} row {r}"
+                        if top:
+                            assert out.top_ids[r].tolist() == ids.tolist(), f"{at} row {r}"
+                            near(out.top_logprobs[r], tlp, r, at)
