@@ -35,8 +35,10 @@ __device__ __forceinline__ float lse_clean(float x) {
   return __builtin_amdgcn_fmed3f(__builtin_canonicalizef(x), lowest, F32_MAX);
 }
 __device__ __forceinline__ float lse_temp(float T) { return T > 0.0f ? T : 1.0f; }  // 0 (a greedy row) and NaN: as T = 1
-__device__ __forceinline__ float lse_scale(float T) { return fminf((float)LOG2E / lse_temp(T), F32_MAX); }
-__device__ __forceinline__ float lse_d(float x, float m, float c) { return fmaxf((x - m) * c, -LSE_DMIN); }  // NaN (-inf - -inf): -D_MIN
+__device__ __forceinline__ float lse_scale(float T) { return fminf((float)LOG2E / lse_temp(T), 0.5f * F32_MAX); }
+// (x - m) / 2: the difference of the largest and the lowest value is past fp32, its half is not
+__device__ __forceinline__ float lse_half(float x, float m) { return fmaf(0.5f, x, -0.5f * m); }
+__device__ __forceinline__ float lse_d(float x, float m, float c) { return fmaxf(lse_half(x, m) * (2.0f * c), -LSE_DMIN); }  // NaN (-inf - -inf): -D_MIN
 
 // The largest of three; a NaN does not show in it.  One instruction, where fmaxf on values that may be signalling NaNs also
 // has to quiet them.
@@ -72,7 +74,7 @@ __device__ __forceinline__ float lse_log(Lse v) { return logf(v.s); }
 // log p of a (clean) logit; -inf for a masked one and in a row without a candidate.  Neither it nor the entropy leaves its range
 // where the sums are off by a rounding (a sure token's s = 1 - 2^-24); a NaN would pass.
 __device__ __forceinline__ float lse_logprob(Lse v, float x, float T) {
-  const float p = x == -INFINITY ? -INFINITY : (x - v.m) / lse_temp(T) - lse_log(v);
+  const float p = x == -INFINITY ? -INFINITY : 2.0f * (lse_half(x, v.m) / lse_temp(T)) - lse_log(v);
   return p > 0.0f ? 0.0f : p;
 }
 __device__ __forceinline__ float lse_entropy(Lse v) {

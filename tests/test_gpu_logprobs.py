@@ -415,3 +415,19 @@ def test_plans(dtype, R, V, stripes):
                         if top:
                             assert out.top_ids[r].tolist() == ids.tolist(), f"{at} row {r}"
                             near(out.top_logprobs[r], tlp, r, at)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_largest_differences(dtype):
+    """+inf (or the type's largest value) and the lowest value in one row: their difference is past fp32, over the temperature it
+    is not."""
+    V = 3000
+    t = torch.tensor([1.0, 2.0, 4.0, 1e3, 1e30, 1e37, 1e38, 3e38, INF])
+    x, _ = rows(18, V, dtype, 21)
+    x[:, 5], x[:9, 100], x[9:, 100], x[3:, 2000] = torch.finfo(dtype).min, INF, torch.finfo(dtype).max, torch.finfo(dtype).min
+    x[6:9, ::2] = torch.finfo(dtype).min
+    tokens = torch.tensor([[5, 100, 7, 2000]], dtype=torch.int32).repeat(18, 1)
+    check(x, tokens, 3, t.repeat(2), "differences")
+    low = x[:, 5:6].expand(18, 64).contiguous()
+    low[:, 7] = INF
+    check(low, torch.full((18, 1), 3, dtype=torch.int32), 64, t.repeat(2), "nothing between")
