@@ -135,16 +135,19 @@ __device__ __forceinline__ void lp_group_max(float (&m)[U]) {
 
 // A lane's sums over blocks of logits of moderate size (below LSE_MOST in magnitude at their largest, no -inf, no NaN),
 // relative to any reference M = fl(c m) within LP_SLACK of the largest, so that M rarely moves: a multiply-add, an
-// exponential and two sums per logit.  Blocks with anything else, and those that would move M to LSE_NEAR or past it (a lane's
-// first tokens all under a mask's -1e9), go to Lse's general form (lp_slow).
+// exponential and two sums per logit.  Blocks with anything else, and those that would move M to LSE_NEAR or past it, go to Lse's
+// general form (lp_slow).  A lane that has seen nothing but a mask's finite value may go on to -2^31 (-1e9 at temperatures from
+// 0.7 on): |r| <= 64 there, and only a row with nothing above -2^23, where fp32 logits are whole numbers, has its entropy's terms
+// cancel by as much (such masks, 256 bf16 rows of 248,320: 47.5 us with lp_slow, 42.5 so).
 constexpr float LP_SLACK = 8.0f;    // in log2 units: d <= 8, so the entropy's two terms cancel by 8 units at most
+constexpr float LP_MASKED = -0x1p23f, LP_FAR = -0x1p31f;
 struct LpFast {
   float m, M, limit, s, t;
 };
 template <int U, int E>
 __device__ __forceinline__ bool lp_fast(LpFast& f, const float (&x)[U][E], float best, float c) {
   if (__any(best > f.limit)) {
-    if (__any(best > f.limit && !(fabsf(c * best) < LSE_NEAR))) return false;
+    if (__any(best > f.limit && !(fabsf(c * best) < LSE_NEAR || (best < LP_MASKED && c * best > LP_FAR)))) return false;
     if (best > f.limit) {
       const float M = c * best, d = f.M - M, e = lse_exp2(d);
       f = {best, M, best + LP_SLACK / c, f.s * e, e * fmaf(d, f.s, f.t)};
