@@ -324,7 +324,7 @@ const float* qws_head_ws_exact(const void* ws);
 /* Log probabilities of given tokens, their ranks, the rows' entropies and their best alternatives, from rows of logits:
  * what a request for log probabilities returns with its tokens, and what scores a text or a choice among labels.  Row r is
  * logits[r * row_stride .. + V) (any V >= 1, any stride >= 0, any alignment of the element's size), as given: with
- * z_i = x_i / temperature[r] (temperature NULL, 0 or NaN: 1),
+ * z_i = x_i / temperature[r] (temperature NULL, 0, negative or NaN: 1),
  *   log p_i = z_i - ln sum_j e^(z_j);  entropy = -sum_i p_i log p_i (0 for a row without a candidate);
  *   rank of token i = the tokens before it in the order (larger logit, then lower index): 0 = the best;
  *   alternatives = the first `top` tokens of that order, without those at -inf (id -1 and log probability -inf past the

@@ -1,6 +1,6 @@
 """CPU definition of the log probabilities (TEST INFRASTRUCTURE ONLY: see oracle/__init__.py), in 64 bits.
 
-Row x, temperature T (0 or NaN: 1), z = x / T with NaN logits at -inf and +inf ones at the largest fp32 value:
+Row x, temperature T (0, negative or NaN: 1), z = x / T with NaN logits at -inf and +inf ones at the largest fp32 value:
   log p_i = z_i - ln sum_j e^(z_j), -inf for a logit at -inf; entropy = -sum p_i log p_i, 0 for a row without a candidate;
   rank of i = tokens before it by (larger logit, lower index); alternatives: that order without the logits at -inf.
 A given token outside [0, V): log probability 0, rank -1.  No alternative left: id -1, log probability -inf."""

@@ -34,7 +34,7 @@ __device__ __forceinline__ float lse_clean(float x) {
   asm("s_mov_b32 %0, 0xff800000" : "=s"(lowest));
   return __builtin_amdgcn_fmed3f(__builtin_canonicalizef(x), lowest, F32_MAX);
 }
-__device__ __forceinline__ float lse_temp(float T) { return T > 0.0f ? T : 1.0f; }  // 0 (a greedy row) and NaN: as T = 1
+__device__ __forceinline__ float lse_temp(float T) { return T > 0.0f ? T : 1.0f; }  // 0 (a greedy row), negative, NaN: as T = 1
 __device__ __forceinline__ float lse_scale(float T) { return fminf((float)LOG2E / lse_temp(T), 0.5f * F32_MAX); }
 // (x - m) / 2: the difference of the largest and the lowest value is past fp32, its half is not
 __device__ __forceinline__ float lse_half(float x, float m) { return fmaf(0.5f, x, -0.5f * m); }

@@ -77,7 +77,7 @@ class Fp8Head:
 
     def score(self, x: torch.Tensor, tokens: torch.Tensor, temperature: Optional[torch.Tensor] = None):
         """(log probabilities, entropies), fp32 [T]: of tokens int32 [T] under softmax(logits of x / temperature); a token
-        outside [0, N) is skipped (log probability 0).  temperature: fp32 [T] (0: as 1) or None."""
+        outside [0, N) is skipped (log probability 0).  temperature: fp32 [T] (0, negative or NaN: as 1) or None."""
         T, stride = self._states(x)
         given(tokens, (T,), torch.int32, self.device, "tokens")
         if temperature is not None:

@@ -71,8 +71,8 @@ class LogProbs:
 
     logits: fp32 or bf16 [..., V] on the GPU, rows contiguous, at any stride.  tokens: int32 [...] (one token a row: those
     that `Sampler` returned; -1 = skipped: log probability 0, rank -1) or [..., M] (several: labels); None: no tokens.
-    temperature: fp32 [...] (0: as 1) or None.  ranks=False leaves the ranks out.  device: the logits'; without an index,
-    any GPU's."""
+    temperature: fp32 [...] (0, negative or NaN: as 1) or None.  ranks=False leaves the ranks out.  device: the logits';
+    without an index, any GPU's."""
 
     def __init__(self, device="cuda"):
         self.lib = _lib.load()

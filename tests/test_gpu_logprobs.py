@@ -431,3 +431,15 @@ def test_largest_differences(dtype):
     low = x[:, 5:6].expand(18, 64).contiguous()
     low[:, 7] = INF
     check(low, torch.full((18, 1), 3, dtype=torch.int32), 64, t.repeat(2), "nothing between")
+
+
+def test_temperatures_that_are_none():
+    """0, NaN and negative ones (infinity's among them) read as 1, in LogProbs and in score."""
+    x, g = rows(6, 1000, torch.float32, 22)
+    t = torch.tensor([0.0, -0.0, float("nan"), -1.0, -1e-30, -INF], device="cuda")
+    tokens = torch.randint(0, 1000, (6,), generator=g).to(torch.int32).cuda()
+    op = q.LogProbs("cuda")
+    assert all(torch.equal(a, b) for a, b in zip(op(x.cuda(), tokens, top=3, temperature=t), op(x.cuda(), tokens, top=3)))
+    head = q.Fp8Head(x.t().contiguous().cuda())
+    states = torch.randn(6, 6, generator=g).to(torch.bfloat16).cuda()
+    assert all(torch.equal(a, b) for a, b in zip(head.score(states, tokens, temperature=t), head.score(states, tokens)))
