@@ -3,16 +3,19 @@
 //
 //   k_lp_scan   R x G workgroups of 256: one pass over the logits.  Each lane keeps the running maximum and sums of its
 //               elements; each given token's rank is counted by ballots; and the maximum of every 64 consecutive logits
-//               (a group) goes to the workspace.  Bound by the logits' bytes in fp32 (256 rows of 248,320: 42 us, 6.0
-//               TB/s), in bf16 by the vector instructions, five and a half a logit, beside them (2,048 rows: 206 us, 4.9
-//               TB/s), and for few rows by one load's and one launch's latency (1 bf16 row 4.0 us, 36 fp32 rows 9.0).
+//               (a group) goes to the workspace.  Bound by the logits' bytes in fp32 (256 rows of 248,320: 41 us, 6.1
+//               TB/s), in bf16 by the vector instructions, five and a half a logit, beside them (2,048 rows: 201-209 us, 5
+//               TB/s), and for few rows by one load's and one launch's latency (1 bf16 row 3.9 us, 36 fp32 rows 9.2).  With
+//               several tokens by the ranks, a comparison and two scalar instructions for each logit and token (128 rows x
+//               16 tokens: fp32 56 us, bf16 50, where one token a row takes 21 and 13 by the bytes at 6 TB/s).
 //   k_lp_row    R workgroups of 256: joins the row's parts, writes log probabilities, ranks and entropy, and takes the
 //               alternatives in two selections: the n groups with the best maxima (ties: the first), then the n best of
 //               those groups' logits.  That is exact: a logit outside those groups has n better ones, the maxima of the n
 //               groups (each larger, or equal and of a lower index, since groups are consecutive runs of tokens).  So the
 //               pass over the logits does nothing more for 64 alternatives than for none, whatever their order in memory.
-//               Bound by latency: a chain of five loads and some twenty barriers (6.6-9.2 us up to 256 rows; 2,048
-//               rows, all on the card at once, 16.5).
+//               Bound by latency: a chain of five loads and some twenty barriers (6.4-9.2 us up to 256 rows; 2,048
+//               rows, all on the card at once, 16); for alternatives near 64 by the ranking of the keys that the value
+//               bounds leave (64 of one row: 48 us, of 256 rows 62).
 // The join is a launch of its own: a row's last workgroup finishing it in k_lp_scan has to make every workgroup's results
 // visible to other dies' caches first (256 fp32 rows 125 us with stores through the cache, 518 with a release each, against
 // 53; only a single row gained, 21.8 -> 17.9).
