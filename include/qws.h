@@ -378,6 +378,29 @@ size_t qws_fp8_score_ws_bytes(int T, int N, int K);
 int qws_fp8_score(const void* packed, int N, int K, const void* x, long long x_stride, int T, const int* tokens, const float* temperature,
                   float* out_logprobs, float* out_entropy, void* ws, size_t ws_bytes, void* stream);
 
+/* A head held in 4 bits: logits of a few hidden states, beside qws_fp8_head (the reference's W4 products are
+ * engine/src/gemv.cu's and engine/src/head_q.cu:15-100's; format and kernel are this library's).  Along K a row's weights are
+ * codes q in 0 .. 15 with a scale s and a zero point z for each group of 32, 64 or 128 (the last may be shorter):
+ *   y[t][n] = sum over groups of s * (sum_k q x - z * sum_k x), in fp32, the products exact.
+ *   qws_int4_pack:       w [N][K] (dtype QWS_DTYPE_*, rows row_stride elements apart) -> packed (device, qws_int4_pack_bytes(N, K,
+ *                        group) bytes, 256-byte aligned).  Per group lo = min(0, least), hi = max(0, largest), s = (hi - lo) / 15
+ *                        rounded to bf16, z = -lo / s and q = w / s + z, quotients rounded to the nearest (ties to even), both held
+ *                        in 0 .. 15.  A group with a value that is not finite makes its row's products NaN.
+ *   qws_int4_pack_codes: codes [N][K], one in the low four bits of a byte, rows code_stride apart; scales [N][ceil(K / group)] bf16
+ *                        (or fp16) rows scale_stride apart; zeros, like scales, in the low four bits, or NULL: 8.
+ *   qws_int4_head:       x [T][K] bf16 (rows x_stride elements apart) -> out [T][N] (fp32 or bf16, rows out_stride >= N apart).
+ * A hidden state that is not finite makes its logits NaN; finite ones are to stay below 2^115, so that a group's sum of 31 * 128
+ * of them stays in fp32.  Any N <= 2^24, K <= 2^20, T <= 2^22 (else QWS_ERR_NOT_SUPPORTED), any stride and alignment of the
+ * element's size; T = 0 does nothing.  ws: qws_int4_head_ws_bytes(T, N, K, group) bytes, 256-byte aligned, no zeroing needed; calls that
+ * share one must be ordered.  Stream-ordered, allocate nothing, deterministic. */
+size_t qws_int4_pack_bytes(int N, int K, int group);
+int qws_int4_pack(const void* w, int dtype, int N, int K, long long row_stride, int group, void* packed, void* stream);
+int qws_int4_pack_codes(const unsigned char* codes, long long code_stride, const void* scales, int scales_fp16, long long scale_stride,
+                        const unsigned char* zeros, long long zero_stride, int N, int K, int group, void* packed, void* stream);
+size_t qws_int4_head_ws_bytes(int T, int N, int K, int group);
+int qws_int4_head(const void* packed, int N, int K, int group, const void* x, long long x_stride, int T, void* out, int out_dtype, long long out_stride,
+                  void* ws, size_t ws_bytes, void* stream);
+
 /* Argmax over fp32 logits [T][N] -> out_tok[t] (lowest index on ties, NaN never wins) and optional
  * out_val[t].  Same signature and contract as the reference's smk_argmax
  * (engine/include/engine.h:68-71, engine/src/misc.cu:133-137); ws of qws_argmax_ws_bytes() bytes. */

@@ -86,7 +86,7 @@ EXPORTS = ("qws_sample_ws_bytes", "qws_sample", "qws_sample_noalloc", "qws_verif
            "qws_state_bytes", "qws_state_begin", "qws_state_note", "qws_state_read",
            "qws_finish", "qws_finish_rows", "qws_finish_forced", "qws_head_ws_bytes", "qws_head_select_rescore", "qws_head_ws_cand", "qws_head_ws_exact",
            "qws_logprobs_ws_bytes", "qws_logprobs", "qws_fp8_pack_bytes", "qws_fp8_pack", "qws_fp8_head_ws_bytes", "qws_fp8_head", "qws_fp8_score_ws_bytes",
-           "qws_fp8_score", "qws_pld_default_cfg", "qws_pld_bytes", "qws_pld_reset", "qws_pld_append", "qws_pld_propose",
+           "qws_fp8_score", "qws_int4_pack_bytes", "qws_int4_pack", "qws_int4_pack_codes", "qws_int4_head_ws_bytes", "qws_int4_head", "qws_pld_default_cfg", "qws_pld_bytes", "qws_pld_reset", "qws_pld_append", "qws_pld_propose",
            "qws_row_init", "qws_row_check", "qws_abi_sizes",
            "qws_timing", "qws_timing_read", "qws_timing_read_verify", "qws_test_philox", "qws_test_proc_logits", "qws_test_dist")
 
@@ -136,6 +136,11 @@ def load(path=None):
     lib.qws_fp8_head.argtypes, lib.qws_fp8_head.restype = [vp, ci, ci, vp, ll, ci, vp, ci, ll, vp, sz, vp], ci
     lib.qws_fp8_score_ws_bytes.argtypes, lib.qws_fp8_score_ws_bytes.restype = [ci] * 3, sz
     lib.qws_fp8_score.argtypes, lib.qws_fp8_score.restype = [vp, ci, ci, vp, ll, ci, vp, vp, vp, vp, vp, sz, vp], ci
+    lib.qws_int4_pack_bytes.argtypes, lib.qws_int4_pack_bytes.restype = [ci] * 3, sz
+    lib.qws_int4_pack.argtypes, lib.qws_int4_pack.restype = [vp, ci, ci, ci, ll, ci, vp, vp], ci
+    lib.qws_int4_pack_codes.argtypes, lib.qws_int4_pack_codes.restype = [vp, ll, vp, ci, ll, vp, ll, ci, ci, ci, vp, vp], ci
+    lib.qws_int4_head_ws_bytes.argtypes, lib.qws_int4_head_ws_bytes.restype = [ci] * 4, sz
+    lib.qws_int4_head.argtypes, lib.qws_int4_head.restype = [vp, ci, ci, ci, vp, ll, ci, vp, ci, ll, vp, sz, vp], ci
     lib.qws_pld_default_cfg.argtypes, lib.qws_pld_default_cfg.restype = [C.POINTER(PldCfg)], None
     lib.qws_pld_bytes.argtypes, lib.qws_pld_bytes.restype = [ci, ci], sz
     lib.qws_pld_reset.argtypes, lib.qws_pld_reset.restype = [vp, ci, ci, ci, vp, ci, vp], ci

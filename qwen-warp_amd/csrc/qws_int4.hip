@@ -1,0 +1,385 @@
+// qws 4-bit head: logits of T hidden states from a head kept in 4 bits with a scale and a zero point for each group of 32, 64 or
+// 128 weights along K (the definitions: include/qws.h qws_int4_*).
+//
+// Products.  y = sum over groups of s (sum_k q x - z sum_k x), q and z in 0 .. 15.  The codes enter the bf16 matrix instruction
+// as 16 + q, which is exact in bf16 and takes one shift and one and-or for two of them: a code's four bits are the top of the
+// fraction of a number in [16, 32).  The hidden states enter as they are, so a group's products are exact and summed in fp32; the
+// 16 is taken off with the zero point, (16 + z) sum_k x, whose sum of hidden states is a product with ones, once for
+// all of a wave's weights.  Then the scale is applied in fp32: nothing is rounded to fewer bits.  The offset makes a group's sum
+// some five times as large as what is left of it, so its error is a few 2^-24 of the group's terms.
+//
+// Layout.  16 weight rows x 128 values are a fragment of 1 KB: lane l's 16 bytes are row l % 16, word j values 32 j + 8 (l / 16)
+// .. + 7, the second operand of the 16x16x32 product j; value 2 i and 2 i + 1 of a word are bits 4 i .. and 4 i + 16 .., so that one
+// mask takes a pair into the halves of a register.  Four fragments (64 rows) lie together for each 128 values of K, 4 KB that one
+// wave reads at once.  A scale is a word: fp32 (from bf16 or fp16: the low 13 bits are 0) with 16 + z in its low byte; the 64 words of a
+// tile's rows lie together for each group.  Rows and values beyond N and K have scale 0.
+#include "qws_lse.h"
+
+#include <type_traits>
+
+namespace qws {
+
+typedef __bf16 i4_b8 __attribute__((ext_vector_type(8)));
+
+constexpr int I4_KB = 128;     // values of a fragment's row
+constexpr int I4_ROWS = 64;    // weight rows that lie together
+constexpr int I4_NMAX = 1 << 24, I4_KMAX = 1 << 20, I4_TMAX = 1 << 22;
+
+__host__ __device__ inline int i4_up(int n, int m) { return (n + m - 1) / m * m; }
+struct I4Layout {
+  int tiles, kb, kg;     // tiles of 64 rows, blocks of 128 values, groups of a row
+  size_t scales, total;  // byte offsets
+};
+__host__ __device__ inline I4Layout i4_layout(int N, int K, int group) {
+  I4Layout l;
+  l.tiles = i4_up(N, I4_ROWS) / I4_ROWS;
+  l.kb = i4_up(K, I4_KB) / I4_KB;
+  l.kg = l.kb * (I4_KB / group);
+  l.scales = (size_t)l.tiles * l.kb * (I4_ROWS * I4_KB / 2);
+  l.total = l.scales + (size_t)l.tiles * l.kg * I4_ROWS * 4;
+  return l;
+}
+
+// ------------------------------------------------------------------------------------------------ packing
+struct I4Pack {
+  const void* w;  // weights, or codes
+  long long stride;
+  const uint16_t* scales;  // given codes: bf16 or fp16 bits, a row's groups together
+  long long scale_stride;
+  int half;  // fp16
+  const uint8_t* zeros;  // or null: 8
+  long long zero_stride;
+  int N, K;
+  I4Layout l;
+  char* out;
+};
+__device__ __forceinline__ uint32_t i4_nearest_bf16(float x) {  // a finite x >= 0 as the bits of a bf16 value, ties to even
+  const uint32_t u = __float_as_uint(x);
+  return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
+}
+
+// One wave per fragment.  T: float, uint16_t (bf16) or uint8_t (codes).  A group of a row's values lies in one to four words of
+// each of four lanes.  Bound by memory.
+template <typename T, int GROUP>
+__global__ void __launch_bounds__(256) k_i4_pack(I4Pack a) {
+  constexpr int J = GROUP / 32;  // words of a group
+  const int lane = lane_id(), quad = lane >> 4, kb = blockIdx.y * 4 + wave_id();
+  if (kb >= a.l.kb) return;
+  const int r = blockIdx.x * 16 + (lane & 15), at = min(r, a.N - 1);
+  const T* row = (const T*)a.w + (long long)at * a.stride;
+  const int tile = r / I4_ROWS, in_tile = r % I4_ROWS;
+  uint32_t* words = (uint32_t*)(a.out + a.l.scales) + (size_t)tile * a.l.kg * I4_ROWS + in_tile;
+  uint32_t q[4];
+#pragma unroll
+  for (int g = 0; g < 4 / J; g++) {
+    const int kg = kb * (4 / J) + g;
+    uint32_t word = 16;
+    if constexpr (sizeof(T) == 1) {
+#pragma unroll
+      for (int j = 0; j < J; j++) {
+        const int k0 = kb * I4_KB + 32 * (g * J + j) + 8 * quad;
+        uint32_t v = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const uint32_t code = *gmem((const uint8_t*)row + min(k0 + e, a.K - 1)) & 15u;
+          v |= (k0 + e < a.K ? code : 0u) << (4 * (e >> 1) + 16 * (e & 1));
+        }
+        q[g * J + j] = v;
+      }
+      if (r < a.N && kg * GROUP < a.K) {
+        const uint32_t s = *gmem(a.scales + (long long)at * a.scale_stride + kg);
+        const uint32_t z = a.zeros ? *gmem(a.zeros + (long long)at * a.zero_stride + kg) & 15u : 8u;
+        const uint32_t f = a.half ? __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)s)) : s << 16;
+        word = ((f & 0x7FFFFFFFu) < 0x7F800000u ? f : 0x7FC00000u) | (16 + z);
+      }
+    } else {
+      float v[J][8], lo = 0.0f, hi = 0.0f;
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < J; j++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int k = kb * I4_KB + 32 * (g * J + j) + 8 * quad + e;
+          float f;
+          if constexpr (sizeof(T) == 4)
+            f = *gmem((const float*)row + min(k, a.K - 1));
+          else
+            f = __uint_as_float((uint32_t)*gmem((const uint16_t*)row + min(k, a.K - 1)) << 16);
+          if (r >= a.N || k >= a.K) f = 0.0f;
+          bad = bad || !(fabsf(f) <= F32_MAX);
+          v[j][e] = f;
+          lo = fminf(lo, f);
+          hi = fmaxf(hi, f);
+        }
+#pragma unroll
+      for (int i = 16; i <= 32; i <<= 1) {
+        lo = fminf(lo, __shfl_xor(lo, i));
+        hi = fmaxf(hi, __shfl_xor(hi, i));
+        bad = __shfl_xor((int)bad, i) || bad;
+      }
+      const float range = (hi - lo) / 15.0f;
+      bad = bad || !(range <= F32_MAX);
+      const uint32_t s = bad ? 0 : i4_nearest_bf16(range);
+      bad = bad || s >= 0x7F80u;
+      const float d = s && !bad ? __uint_as_float(s << 16) : 1.0f;
+      const float z = fminf(fmaxf(rintf(-lo / d), 0.0f), 15.0f);
+#pragma unroll
+      for (int j = 0; j < J; j++) {
+        uint32_t u = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float c = fminf(fmaxf(rintf(v[j][e] / d) + z, 0.0f), 15.0f);
+          u |= (bad ? 0u : (uint32_t)c) << (4 * (e >> 1) + 16 * (e & 1));
+        }
+        q[g * J + j] = u;
+      }
+      if (bad)
+        word = 0x7FC00000u | 16;  // a value that is not finite, or a range past fp32: NaN
+      else
+        word = s << 16 | (16 + (uint32_t)z);
+    }
+    if (quad == 0) words[(size_t)kg * I4_ROWS] = word;
+  }
+  vu4* d = (vu4*)(a.out + ((size_t)tile * a.l.kb + kb) * (I4_ROWS * I4_KB / 2)) + (in_tile >> 4) * 64;
+  d[lane] = (vu4){q[0], q[1], q[2], q[3]};
+}
+
+// Hidden states as rows of kb * 128 values, the last ones 0, for those whose rows a lane cannot read 16 bytes at a time
+__global__ void __launch_bounds__(256) k_i4_states(const uint16_t* x, long long stride, int K, int width, uint16_t* out) {
+  const uint16_t* row = x + (long long)blockIdx.x * stride;
+  uint16_t* to = out + (size_t)blockIdx.x * width;
+  for (int k = blockIdx.y * 256 + threadIdx.x; k < width; k += gridDim.y * 256) to[k] = k < K ? *gmem(row + k) : (uint16_t)0;
+}
+
+// ------------------------------------------------------------------------------------------------ products
+struct I4Args {
+  const char* w;
+  I4Layout l;
+  const uint16_t* x;
+  long long x_stride;
+  int N, T, K;
+  int tiles_t;
+  void* out;
+  long long out_stride;
+};
+
+// the pairs of a word's eight codes as 16 + q in bf16
+__device__ __forceinline__ i4_b8 i4_wide(uint32_t w) {
+  const vu4 u = {(w << 3 & 0x00780078u) | 0x41804180u, (w >> 1 & 0x00780078u) | 0x41804180u, (w >> 5 & 0x00780078u) | 0x41804180u,
+                 (w >> 9 & 0x00780078u) | 0x41804180u};
+  return __builtin_bit_cast(i4_b8, u);
+}
+__device__ __forceinline__ vf4 i4_mfma(i4_b8 a, i4_b8 b, vf4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ uint32_t i4_bf16(float x) {  // nearest even; NaN stays NaN
+  const uint32_t u = __float_as_uint(x);
+  return x != x ? 0x7FC0u : (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
+}
+
+// A workgroup takes 64 weight rows and 16 TF hidden states, its 4 waves a quarter of K each; their sums meet in LDS.
+template <typename O, int GROUP, int TF>
+__global__ void __launch_bounds__(256, TF > 2 ? 2 : 4) k_i4_few(I4Args a) {
+  constexpr int G = I4_ROWS / 16, C = I4_KB / GROUP, J = GROUP / 32;  // fragments, groups of a block, products of a group
+  __shared__ vf4 s_acc[4][G * TF][64];
+  const int lane = lane_id(), wave = wave_id(), quad = lane >> 4;
+  // XCD x (workgroups x, x + 8, ..) takes the tiles of weight rows x, x + 8, .., all of their hidden states in a row
+  const int tile = (blockIdx.x >> 3) / a.tiles_t * 8 + (blockIdx.x & 7), t0 = (blockIdx.x >> 3) % a.tiles_t * 16 * TF;
+  if (tile >= a.l.tiles) return;
+  const int kb = a.l.kb, per = (kb + 3) / 4, lo = wave * per, hi = min(lo + per, kb);
+  const char* pw = a.w + (size_t)tile * kb * (I4_ROWS * I4_KB / 2) + 16 * lane;
+  const uint32_t* ps = (const uint32_t*)(a.w + a.l.scales) + (size_t)tile * a.l.kg * I4_ROWS + (lane & 15);
+  const uint16_t* px[TF];
+#pragma unroll
+  for (int j = 0; j < TF; j++) px[j] = a.x + (long long)min(t0 + 16 * j + (lane & 15), a.T - 1) * a.x_stride + 8 * quad;
+  const vu4 one = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+  const i4_b8 ones = __builtin_bit_cast(i4_b8, one);
+  vf4 acc[G][TF] = {};
+  vu4 w[G];
+  uint32_t sw[G][C];
+  auto load = [&](int k) {
+#pragma unroll
+    for (int g = 0; g < G; g++) w[g] = __builtin_nontemporal_load((const QWS_G vu4*)(pw + ((size_t)k * G + g) * 1024));
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int g = 0; g < G; g++) sw[g][c] = *gmem(ps + ((size_t)k * C + c) * I4_ROWS + 16 * g);
+  };
+  if (lo < hi) load(lo);
+  for (int k = lo; k < hi; k++) {
+    vu4 cw[G], x[TF][4];
+    uint32_t cs[G][C];
+#pragma unroll
+    for (int j = 0; j < TF; j++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int at = k * I4_KB + 32 * i;
+        if (at + 8 * quad < a.K)
+          x[j][i] = *gmem((const vu4*)(px[j] + at));
+        else
+          x[j][i] = (vu4){0, 0, 0, 0};
+      }
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      cw[g] = w[g];
+#pragma unroll
+      for (int c = 0; c < C; c++) cs[g][c] = sw[g][c];
+    }
+    load(min(k + 1, hi - 1));
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      vf4 sum[TF] = {};
+#pragma unroll
+      for (int i = 0; i < J; i++)
+#pragma unroll
+        for (int j = 0; j < TF; j++) sum[j] = i4_mfma(__builtin_bit_cast(i4_b8, x[j][c * J + i]), ones, sum[j]);
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        vf4 d[TF] = {};
+#pragma unroll
+        for (int i = 0; i < J; i++) {
+          const i4_b8 b = i4_wide(cw[g][c * J + i]);
+#pragma unroll
+          for (int j = 0; j < TF; j++) d[j] = i4_mfma(__builtin_bit_cast(i4_b8, x[j][c * J + i]), b, d[j]);
+        }
+        const float z = (float)(cs[g][c] & 255u), s = __uint_as_float(cs[g][c] & 0xFFFFFF00u);
+#pragma unroll
+        for (int j = 0; j < TF; j++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) acc[g][j][r] = fmaf(s, fmaf(-z, sum[j][r], d[j][r]), acc[g][j][r]);
+      }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < G; g++)
+#pragma unroll
+    for (int j = 0; j < TF; j++) s_acc[wave][g * TF + j][lane] = acc[g][j];
+  bar();
+  for (int i = wave; i < G * TF; i += 4) {
+    const vf4 y = (s_acc[0][i][lane] + s_acc[1][i][lane]) + (s_acc[2][i][lane] + s_acc[3][i][lane]);
+    const int n = tile * I4_ROWS + 16 * (i / TF) + (lane & 15), t = t0 + 16 * (i % TF) + 4 * quad;
+    if (n < a.N) {
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        if (t + r < a.T) {
+          O* p = (O*)a.out + (long long)(t + r) * a.out_stride + n;
+          if constexpr (sizeof(O) == 4)
+            *p = y[r];
+          else
+            *p = (O)i4_bf16(y[r]);
+        }
+    }
+  }
+}
+
+inline bool i4_group(int group) { return group == 32 || group == 64 || group == 128; }
+inline bool i4_shape(int T, int N, int K, int group) { return T >= 1 && N >= 1 && K >= 1 && i4_group(group); }
+inline bool i4_fits(int T, int N, int K) { return N <= I4_NMAX && K <= I4_KMAX && T <= I4_TMAX; }
+inline bool i4_aligned(const void* p) { return p && ((uintptr_t)p & 255) == 0; }
+inline size_t i4_ws(int T, int K) { return ((size_t)T * i4_up(K, I4_KB) * 2 + 255) & ~(size_t)255; }
+// whether a lane can read hidden states 16 bytes at a time as they came
+inline bool i4_direct(const void* x, long long stride, int T, int K) { return K % 8 == 0 && ((uintptr_t)x & 15) == 0 && (T == 1 || stride % 8 == 0); }
+
+template <typename T>
+static int i4_pack(const I4Pack& a, int group, hipStream_t st) {
+  const dim3 grid(a.l.tiles * (I4_ROWS / 16), (a.l.kb + 3) / 4);
+  switch (group) {
+    case 32: hipLaunchKernelGGL((k_i4_pack<T, 32>), grid, dim3(256), 0, st, a); break;
+    case 64: hipLaunchKernelGGL((k_i4_pack<T, 64>), grid, dim3(256), 0, st, a); break;
+    default: hipLaunchKernelGGL((k_i4_pack<T, 128>), grid, dim3(256), 0, st, a); break;
+  }
+  return (int)hipGetLastError();
+}
+
+template <typename O, int GROUP>
+static int i4_run(I4Args a, hipStream_t st) {
+  const int tf = a.T <= 16 ? 1 : a.T <= 32 ? 2 : 4;
+  a.tiles_t = i4_up(a.T, 16 * tf) / (16 * tf);
+  const long long wgs = (long long)i4_up(a.l.tiles, 8) * a.tiles_t;
+  if (wgs > 0xFFFFFF) return QWS_ERR_NOT_SUPPORTED;  // below 2^32 threads
+  const dim3 grid((unsigned)wgs);
+  switch (tf) {
+    case 1: hipLaunchKernelGGL((k_i4_few<O, GROUP, 1>), grid, dim3(256), 0, st, a); break;
+    case 2: hipLaunchKernelGGL((k_i4_few<O, GROUP, 2>), grid, dim3(256), 0, st, a); break;
+    default: hipLaunchKernelGGL((k_i4_few<O, GROUP, 4>), grid, dim3(256), 0, st, a); break;
+  }
+  return (int)hipGetLastError();
+}
+template <typename O>
+static int i4_product(const I4Args& a, int group, hipStream_t st) {
+  return group == 32 ? i4_run<O, 32>(a, st) : group == 64 ? i4_run<O, 64>(a, st) : i4_run<O, 128>(a, st);
+}
+
+}  // namespace qws
+
+extern "C" size_t qws_int4_pack_bytes(int N, int K, int group) {
+  return qws::i4_shape(1, N, K, group) && qws::i4_fits(1, N, K) ? qws::i4_layout(N, K, group).total : 0;
+}
+
+extern "C" int qws_int4_pack(const void* w, int dtype, int N, int K, long long row_stride, int group, void* packed, void* stream) {
+  using namespace qws;
+  if (!i4_shape(1, N, K, group) || (dtype != QWS_DTYPE_F32 && dtype != QWS_DTYPE_BF16) || !w || row_stride < 0 || !i4_aligned(packed)) return QWS_ERR_INVALID;
+  if ((uintptr_t)w & (dtype == QWS_DTYPE_F32 ? 3 : 1)) return QWS_ERR_INVALID;
+  if (!i4_fits(1, N, K)) return QWS_ERR_NOT_SUPPORTED;
+  I4Pack a = {};
+  a.w = w;
+  a.stride = row_stride;
+  a.N = N;
+  a.K = K;
+  a.l = i4_layout(N, K, group);
+  a.out = (char*)packed;
+  return dtype == QWS_DTYPE_F32 ? i4_pack<float>(a, group, (hipStream_t)stream) : i4_pack<uint16_t>(a, group, (hipStream_t)stream);
+}
+
+extern "C" int qws_int4_pack_codes(const unsigned char* codes, long long code_stride, const void* scales, int scales_fp16, long long scale_stride,
+                                   const unsigned char* zeros, long long zero_stride, int N, int K, int group, void* packed, void* stream) {
+  using namespace qws;
+  if (!i4_shape(1, N, K, group) || !codes || !scales || ((uintptr_t)scales & 1) || code_stride < 0 || scale_stride < 0 || zero_stride < 0 || !i4_aligned(packed))
+    return QWS_ERR_INVALID;
+  if (!i4_fits(1, N, K)) return QWS_ERR_NOT_SUPPORTED;
+  I4Pack a = {};
+  a.w = codes;
+  a.stride = code_stride;
+  a.scales = (const uint16_t*)scales;
+  a.scale_stride = scale_stride;
+  a.half = scales_fp16 != 0;
+  a.zeros = zeros;
+  a.zero_stride = zero_stride;
+  a.N = N;
+  a.K = K;
+  a.l = i4_layout(N, K, group);
+  a.out = (char*)packed;
+  return i4_pack<uint8_t>(a, group, (hipStream_t)stream);
+}
+
+extern "C" size_t qws_int4_head_ws_bytes(int T, int N, int K, int group) {
+  return qws::i4_shape(T, N, K, group) && qws::i4_fits(T, N, K) ? qws::i4_ws(T, K) : 0;
+}
+
+extern "C" int qws_int4_head(const void* packed, int N, int K, int group, const void* x, long long x_stride, int T, void* out, int out_dtype,
+                             long long out_stride, void* ws, size_t ws_bytes, void* stream) {
+  using namespace qws;
+  if (!i4_shape(1, N, K, group) || T < 0 || x_stride < 0 || !i4_aligned(packed) || (out_dtype != QWS_DTYPE_F32 && out_dtype != QWS_DTYPE_BF16)) return QWS_ERR_INVALID;
+  if (!i4_fits(T, N, K)) return QWS_ERR_NOT_SUPPORTED;
+  if (T == 0) return QWS_OK;
+  if (!x || ((uintptr_t)x & 1) || !out || ((uintptr_t)out & (out_dtype == QWS_DTYPE_F32 ? 3 : 1)) || (T > 1 && out_stride < N)) return QWS_ERR_INVALID;
+  if (!i4_aligned(ws) || ws_bytes < i4_ws(T, K)) return QWS_ERR_INVALID;
+  I4Args a = {};
+  a.w = (const char*)packed;
+  a.l = i4_layout(N, K, group);
+  a.x = (const uint16_t*)x;
+  a.x_stride = x_stride;
+  a.N = N;
+  a.T = T;
+  a.K = K;
+  a.out = out;
+  a.out_stride = out_stride;
+  if (!i4_direct(x, x_stride, T, K)) {
+    const int width = i4_up(K, I4_KB);
+    hipLaunchKernelGGL(k_i4_states, dim3(T, (width + 1023) / 1024), dim3(256), 0, (hipStream_t)stream, a.x, x_stride, K, width, (uint16_t*)ws);
+    const int e = (int)hipGetLastError();
+    if (e) return e;
+    a.x = (const uint16_t*)ws;
+    a.x_stride = width;
+    a.K = width;
+  }
+  return out_dtype == QWS_DTYPE_F32 ? i4_product<float>(a, group, (hipStream_t)stream) : i4_product<uint16_t>(a, group, (hipStream_t)stream);
+}
