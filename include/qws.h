@@ -401,6 +401,65 @@ size_t qws_int4_head_ws_bytes(int T, int N, int K, int group);
 int qws_int4_head(const void* packed, int N, int K, int group, const void* x, long long x_stride, int T, void* out, int out_dtype, long long out_stride,
                   void* ws, size_t ws_bytes, void* stream);
 
+/* Losses over the tokens that were drawn, with their gradient at the logits: what follows qws_sample and qws_logprobs where a model
+ * learns from its own samples (no counterpart in the reference).
+ *
+ * The rows of both: row r of the logits (dtype QWS_DTYPE_*) is V contiguous values at logits + (r / block) * block_stride + (r %
+ * block) * row_stride (elements; block 0: row_stride alone), any alignment of the element's size; tokens [R]; temperature [R] or NULL,
+ * by qws_logprobs' rules (0, negative or NaN: 1), as are NaN logits (-inf) and +inf ones.  lp = the log probability of the row's
+ * token under softmax(x / T).  A token outside [0, V) (padding, a prompt's positions) leaves its row out: nothing of it is
+ * used, log probability 0.  A token that its row's mask forbids (lp = -inf; a row without a candidate as well) adds nothing and has no gradient.
+ *
+ * qws_policy_loss: the clipped policy loss with a KL term.  Per row, with r = e^(lp - old_logprobs) and d = ref_logprobs - lp,
+ *   l = -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl (e^d - 1 - d)    (ref_logprobs NULL: without the second term)
+ *   loss = sum w l; weights NULL: the mean over the rows with a token in [0, V) (0 without any).
+ *   dl/dlp = -r A where r A is the smaller one (or equal), else 0; plus kl (1 - e^d).  Differences above 80 count as 80.
+ *   out_logprobs, out_ratio (1 for rows left out), out_kl (0) [R]: optional.
+ * qws_preference_loss: the loss of P pairs by their log ratios.  starts [2 P + 1] (ascending, in [0, R]): sequence i is rows starts[i] ..
+ *   starts[i + 1], 2 p the preferred one of pair p and 2 p + 1 the other; rows outside are not used.  s_i = the sum of lp over
+ *   the sequence (average != 0: over its count of tokens in [0, V), at least 1),
+ *   u = beta ((s_2p - ref_2p) - (s_2p+1 - ref_2p+1)) - margin    (ref [2 P] or NULL: 0)
+ *   l = -(1 - smoothing) ln sigmoid(u) - smoothing ln sigmoid(-u);  loss = sum w l, weights [P] or NULL: the mean.
+ *   out_logprobs [2 P] = s, out_margins [P] = u, out_token_logprobs [R]: optional.
+ * NaN among what a used row or pair brings makes the loss and the gradient's rows that depend on it NaN.
+ *
+ * grad (optional): [R][V] of the logits' type, rows grad_stride >= V apart: the loss's derivative, every row written (0 where
+ * there is none).  qws_loss_grad writes it later, times *upstream (device, NULL: 1), from the state that the call left; r as in that call.
+ * state: qws_*_state_bytes, 256-byte aligned, no zeroing needed; one for each loss in flight.  R < 2^24, V <= 2^24, P < 2^23
+ * (else QWS_ERR_NOT_SUPPORTED); clip_low in [0, 1], clip_high >= 0, smoothing in [0, 1], all finite.  Statistics are fp32, what
+ * follows from log p is 64 bits.  Zero-initialise the structs.  Stream-ordered, allocate nothing, deterministic. */
+typedef struct qws_loss_rows {
+  const void* logits; /* device */
+  int dtype;          /* QWS_DTYPE_* */
+  int R, V;
+  int block;
+  long long row_stride, block_stride;
+  const int* tokens;        /* device [R] */
+  const float* temperature; /* device [R] or NULL */
+} qws_loss_rows;
+typedef struct qws_policy_batch {
+  qws_loss_rows rows;
+  const float *old_logprobs, *advantages; /* device [R] */
+  const float *ref_logprobs, *weights;    /* device [R] or NULL */
+  float clip_low, clip_high, kl;
+  float* out_loss; /* device, one */
+  float *out_logprobs, *out_ratio, *out_kl;
+} qws_policy_batch;
+typedef struct qws_preference_batch {
+  qws_loss_rows rows;
+  const int* starts; /* device [2 P + 1] */
+  int P, average;
+  const float *ref, *weights; /* device [2 P], [P] or NULL */
+  float beta, margin, smoothing;
+  float* out_loss; /* device, one */
+  float *out_logprobs, *out_margins, *out_token_logprobs;
+} qws_preference_batch;
+size_t qws_policy_state_bytes(int dtype, int R, int V);
+int qws_policy_loss(const qws_policy_batch* b, void* state, size_t state_bytes, void* grad, long long grad_stride, void* stream);
+size_t qws_preference_state_bytes(int dtype, int R, int V, int P);
+int qws_preference_loss(const qws_preference_batch* b, void* state, size_t state_bytes, void* grad, long long grad_stride, void* stream);
+int qws_loss_grad(const qws_loss_rows* r, const void* state, const float* upstream, void* grad, long long grad_stride, void* stream);
+
 /* Argmax over fp32 logits [T][N] -> out_tok[t] (lowest index on ties, NaN never wins) and optional
  * out_val[t].  Same signature and contract as the reference's smk_argmax
  * (engine/include/engine.h:68-71, engine/src/misc.cu:133-137); ws of qws_argmax_ws_bytes() bytes. */

@@ -81,12 +81,33 @@ class LogprobsBatch(C.Structure):
                 ("out_entropy", C.c_void_p), ("out_top_ids", C.c_void_p), ("out_top_logprobs", C.c_void_p)]
 
 
+class LossRows(C.Structure):
+    """include/qws.h qws_loss_rows."""
+    _fields_ = [("logits", C.c_void_p), ("dtype", C.c_int), ("R", C.c_int), ("V", C.c_int), ("block", C.c_int), ("row_stride", C.c_longlong),
+                ("block_stride", C.c_longlong), ("tokens", C.c_void_p), ("temperature", C.c_void_p)]
+
+
+class PolicyBatch(C.Structure):
+    """include/qws.h qws_policy_batch."""
+    _fields_ = [("rows", LossRows), ("old_logprobs", C.c_void_p), ("advantages", C.c_void_p), ("ref_logprobs", C.c_void_p), ("weights", C.c_void_p),
+                ("clip_low", C.c_float), ("clip_high", C.c_float), ("kl", C.c_float), ("out_loss", C.c_void_p), ("out_logprobs", C.c_void_p),
+                ("out_ratio", C.c_void_p), ("out_kl", C.c_void_p)]
+
+
+class PreferenceBatch(C.Structure):
+    """include/qws.h qws_preference_batch."""
+    _fields_ = [("rows", LossRows), ("starts", C.c_void_p), ("P", C.c_int), ("average", C.c_int), ("ref", C.c_void_p), ("weights", C.c_void_p),
+                ("beta", C.c_float), ("margin", C.c_float), ("smoothing", C.c_float), ("out_loss", C.c_void_p), ("out_logprobs", C.c_void_p),
+                ("out_margins", C.c_void_p), ("out_token_logprobs", C.c_void_p)]
+
+
 EXPORTS = ("qws_sample_ws_bytes", "qws_sample", "qws_sample_noalloc", "qws_verify_ws_bytes", "qws_verify", "qws_verify_map", "qws_draft_pick",
            "qws_row_init_pick", "qws_argmax_ws_bytes", "qws_argmax",
            "qws_state_bytes", "qws_state_begin", "qws_state_note", "qws_state_read",
            "qws_finish", "qws_finish_rows", "qws_finish_forced", "qws_head_ws_bytes", "qws_head_select_rescore", "qws_head_ws_cand", "qws_head_ws_exact",
            "qws_logprobs_ws_bytes", "qws_logprobs", "qws_fp8_pack_bytes", "qws_fp8_pack", "qws_fp8_head_ws_bytes", "qws_fp8_head", "qws_fp8_score_ws_bytes",
-           "qws_fp8_score", "qws_int4_pack_bytes", "qws_int4_pack", "qws_int4_pack_codes", "qws_int4_head_ws_bytes", "qws_int4_head", "qws_pld_default_cfg", "qws_pld_bytes", "qws_pld_reset", "qws_pld_append", "qws_pld_propose",
+           "qws_fp8_score", "qws_int4_pack_bytes", "qws_int4_pack", "qws_int4_pack_codes", "qws_int4_head_ws_bytes", "qws_int4_head",
+           "qws_policy_state_bytes", "qws_policy_loss", "qws_preference_state_bytes", "qws_preference_loss", "qws_loss_grad", "qws_pld_default_cfg", "qws_pld_bytes", "qws_pld_reset", "qws_pld_append", "qws_pld_propose",
            "qws_row_init", "qws_row_check", "qws_abi_sizes",
            "qws_timing", "qws_timing_read", "qws_timing_read_verify", "qws_test_philox", "qws_test_proc_logits", "qws_test_dist")
 
@@ -141,6 +162,11 @@ def load(path=None):
     lib.qws_int4_pack_codes.argtypes, lib.qws_int4_pack_codes.restype = [vp, ll, vp, ci, ll, vp, ll, ci, ci, ci, vp, vp], ci
     lib.qws_int4_head_ws_bytes.argtypes, lib.qws_int4_head_ws_bytes.restype = [ci] * 4, sz
     lib.qws_int4_head.argtypes, lib.qws_int4_head.restype = [vp, ci, ci, ci, vp, ll, ci, vp, ci, ll, vp, sz, vp], ci
+    lib.qws_policy_state_bytes.argtypes, lib.qws_policy_state_bytes.restype = [ci] * 3, sz
+    lib.qws_policy_loss.argtypes, lib.qws_policy_loss.restype = [C.POINTER(PolicyBatch), vp, sz, vp, ll, vp], ci
+    lib.qws_preference_state_bytes.argtypes, lib.qws_preference_state_bytes.restype = [ci] * 4, sz
+    lib.qws_preference_loss.argtypes, lib.qws_preference_loss.restype = [C.POINTER(PreferenceBatch), vp, sz, vp, ll, vp], ci
+    lib.qws_loss_grad.argtypes, lib.qws_loss_grad.restype = [C.POINTER(LossRows), vp, vp, vp, ll, vp], ci
     lib.qws_pld_default_cfg.argtypes, lib.qws_pld_default_cfg.restype = [C.POINTER(PldCfg)], None
     lib.qws_pld_bytes.argtypes, lib.qws_pld_bytes.restype = [ci, ci], sz
     lib.qws_pld_reset.argtypes, lib.qws_pld_reset.restype = [vp, ci, ci, ci, vp, ci, vp], ci

@@ -22,7 +22,8 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 SRC = [PKG / "csrc" / "qws_sample.hip", PKG / "csrc" / "qws_verify.hip", PKG / "csrc" / "qws_state.hip", PKG / "csrc" / "qws_pld.hip", PKG / "csrc" / "qws_head.hip",
-       PKG / "csrc" / "qws_hooks.hip", PKG / "csrc" / "qws_logprobs.hip", PKG / "csrc" / "qws_fp8.hip", PKG / "csrc" / "qws_int4.hip"]
+       PKG / "csrc" / "qws_hooks.hip", PKG / "csrc" / "qws_logprobs.hip", PKG / "csrc" / "qws_fp8.hip", PKG / "csrc" / "qws_int4.hip",
+       PKG / "csrc" / "qws_loss.hip"]
 OUT = PKG / "lib" / "libqws.so"
 HOST_SRC, HOST_OUT = PKG / "csrc" / "qws_hostpack.cpp", PKG / "lib" / ("_qws_hostpack" + EXTENSION_SUFFIXES[0])
 CXX = os.environ.get("CXX", "g++")

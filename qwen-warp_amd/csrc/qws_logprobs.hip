@@ -19,7 +19,7 @@
 // The join is a launch of its own: a row's last workgroup finishing it in k_lp_scan has to make every workgroup's results
 // visible to other dies' caches first (256 fp32 rows 125 us with stores through the cache, 518 with a release each, against
 // 53; only a single row gained, 21.8 -> 17.9).
-#include "qws_lse.h"
+#include "qws_logits.h"
 
 #include <type_traits>
 
@@ -35,14 +35,9 @@ constexpr int LP_WGS = (int)((1ll << 32) / LP_NT - 1);  // workgroups of a launc
 constexpr int LP_U = 4;         // vectors of a thread loaded together, where it has more than one
 
 template <typename T>
-constexpr int lp_e() { return 16 / (int)sizeof(T); }  // elements of a vector
-template <typename T>
 constexpr int lp_waves(int u) { return u * lp_e<T>() > 16 ? 5 : 8; }  // waves of a SIMD that the block's registers allow
 template <typename T>
 constexpr int lp_stripe() { return LP_NT * lp_e<T>(); }  // elements that a workgroup's threads load at once
-
-template <typename T>
-using lp_bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
 
 // the next larger value
 __device__ __forceinline__ float lp_above(float x) {
@@ -67,55 +62,6 @@ struct LpArgs {
   int* out_ids;
   float* out_top;
 };
-
-template <typename T>
-__device__ __forceinline__ float lp_one(const T* p) {
-  if constexpr (sizeof(T) == 4)
-    return lse_clean(*gmem((const float*)p));
-  else
-    return lse_clean(__uint_as_float((uint32_t)*gmem((const uint16_t*)p) << 16));
-}
-template <typename T>
-__device__ __forceinline__ void lp_unpack(vu4 r, float* x) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int j = 0; j < 4; j++) x[j] = __uint_as_float(r[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      x[2 * j] = __uint_as_float(r[j] << 16);
-      x[2 * j + 1] = __uint_as_float(r[j] & 0xFFFF0000u);
-    }
-  }
-}
-// the vector at position v of `base` (16-byte aligned), of which [lead, end) exist: the rest reads -inf
-template <typename T>
-__device__ __forceinline__ vu4 lp_load_edge(const T* base, int v, int lead, int end) {
-  constexpr int E = lp_e<T>();
-  vu4 r;
-  if (v >= lead && v + E <= end) {
-    r = *gmem((const vu4*)(base + v));
-  } else {
-    uint32_t y[E];
-#pragma unroll
-    for (int j = 0; j < E; j++) y[j] = *gmem((const lp_bits<T>*)base + min(max(v + j, lead), end - 1));
-#pragma unroll
-    for (int j = 0; j < E; j++)
-      if (v + j < lead || v + j >= end) y[j] = 0xFF800000u >> (sizeof(T) == 4 ? 0 : 16);
-#pragma unroll
-    for (int j = 0; j < 4; j++) r[j] = sizeof(T) == 4 ? y[j] : y[j * (E / 4)] | y[(j * (E / 4) + 1) % E] << 16;
-  }
-  return r;
-}
-
-// The largest of a vector; a NaN shows in the sums (lp_fast), not here
-template <int E>
-__device__ __forceinline__ float lp_max(const float* x) {
-  float m = lse_max3(x[0], x[1], x[2]);
-#pragma unroll
-  for (int j = 3; j + 1 < E; j += 2) m = lse_max3(m, x[j], x[j + 1]);
-  return lse_max3(m, x[E - 1], x[E - 1]);
-}
 
 // The largest of each group's lanes (8 or 16), in every lane: one instruction a step, where fmaxf of a moved value takes four.
 // A lane's value is written at least two instructions before another lane's step reads it (the hardware does not wait).

@@ -1,0 +1,259 @@
+"""Losses over drawn tokens with their gradient at the logits (include/qws.h qws_policy_loss, qws_preference_loss) on torch
+tensors: what follows `Sampler` and `LogProbs` where a model learns from its own samples."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import NamedTuple, Optional, Sequence, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import check
+from .logprobs import INT_MAX, given, on_stream
+from .sampling import ValidationError
+
+
+class PolicyLossResult(NamedTuple):
+    loss: torch.Tensor                    # fp32, one value; differentiable where the logits are
+    logprobs: torch.Tensor                # fp32 [...]: the tokens' log probabilities (0 for rows left out)
+    ratio: torch.Tensor                   # fp32 [...]: e^(logprobs - old_logprobs) (1 for rows left out)
+    kl: Optional[torch.Tensor]            # fp32 [...]: e^d - 1 - d, d = ref_logprobs - logprobs (None without ref_logprobs)
+
+
+class PreferenceLossResult(NamedTuple):
+    loss: torch.Tensor                    # fp32, one value; differentiable where the logits are
+    logprobs: torch.Tensor                # fp32 [2 P]: the sequences' summed (or mean) log probabilities
+    margins: torch.Tensor                 # fp32 [P]: what the sigmoid is taken of
+    token_logprobs: torch.Tensor          # fp32 [...] (0 for rows left out)
+
+
+def blocks_of(x: torch.Tensor, name: str):
+    """(rows, rows of a block, row stride, block stride) of a tensor [..., n] read as rows of n contiguous elements in blocks at one
+    stride, each of rows at one stride: what a slice [:, :-1] of [B, L, n] is.  One block: 0 rows of a block."""
+    shape, strides = x.shape, x.stride()
+    if len(shape) < 2 or (shape[-1] > 1 and strides[-1] != 1):
+        raise ValidationError(f"{name} must be [..., n] with contiguous rows", name)
+    if max(shape) > INT_MAX or math.prod(shape[:-1]) > INT_MAX:
+        raise ValidationError(f"{name}: at most 2^31 - 1 rows of as many elements", name)
+    levels = []  # (rows, stride), innermost first
+    for size, step in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+        if size == 1:
+            continue
+        if levels and step == levels[-1][0] * levels[-1][1]:
+            levels[-1] = (levels[-1][0] * size, levels[-1][1])
+        else:
+            levels.append((size, step))
+    rows = math.prod(shape[:-1])
+    if rows == 0 or not levels:
+        return rows, 0, 0, 0
+    if len(levels) == 1:
+        return rows, 0, levels[0][1], 0
+    if len(levels) == 2:
+        return rows, levels[0][0], levels[0][1], levels[1][1]
+    raise ValidationError(f"{name}: the leading dimensions must lie at two strides at most (reshape it)", name)
+
+
+class _Loss(torch.autograd.Function):
+    """The loss as a function of the logits; `call(None)` runs it and returns (loss, rows, state, what they refer to)."""
+
+    @staticmethod
+    def forward(ctx, logits, owner, call):
+        loss, ctx.rows, ctx.state, ctx.keep = call(None)
+        ctx.owner = owner
+        ctx.save_for_backward(logits)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, upstream):
+        (logits,) = ctx.saved_tensors
+        where, stream = on_stream(logits.device.index)
+        with where:
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            upstream = upstream.contiguous()
+            check(ctx.owner.lib.qws_loss_grad(C.byref(ctx.rows), ctx.state.data_ptr(), upstream.data_ptr(), grad.data_ptr(), logits.shape[-1], stream), "qws_loss_grad")
+        return grad, None, None
+
+
+class _Base:
+    def __init__(self, device):
+        self.lib = _lib.load()
+        self.device = torch.device(device)
+        self._bytes = {}
+
+    def _rows(self, logits, tokens, temperature=None):
+        """The checks of the rows, and their structure."""
+        dtype, dev = logits.dtype, logits.device
+        if not logits.is_cuda or (dtype != torch.float32 and dtype != torch.bfloat16):
+            raise ValidationError("logits must be a CUDA fp32 / bf16 tensor", "logits")
+        if dev != self.device and (self.device.type != "cuda" or self.device.index is not None):
+            raise ValidationError(f"logits must be on {self.device}", "logits")
+        R, block, stride, block_stride = blocks_of(logits, "logits")
+        if logits.shape[-1] < 1:
+            raise ValidationError("logits must have a value a row", "logits")
+        lead = logits.shape[:-1]
+        given(tokens, lead, torch.int32, dev, "tokens")
+        if temperature is not None:
+            self._number(temperature, lead, dev, "temperature")
+        return _lib.LossRows(logits.data_ptr(), _lib.DTYPE_F32 if dtype == torch.float32 else _lib.DTYPE_BF16, R, logits.shape[-1], block, stride, block_stride,
+                             tokens.data_ptr(), temperature.data_ptr() if temperature is not None else None)
+
+    @staticmethod
+    def _number(t, shape, dev, name):
+        if t is None:
+            raise ValidationError(f"{name} is needed", name)
+        given(t, shape, torch.float32, dev, name)
+        if t.requires_grad:
+            raise ValidationError(f"{name} is taken as a constant: detach it", name)
+
+    def _state(self, query, *key):
+        n = self._bytes.get(key)
+        if n is None:
+            n = self._bytes[key] = query(*key)
+        if n == 0:
+            raise ValidationError("logits: fewer than 2^24 rows of at most 2^24 values", "logits")
+        return n
+
+    def _forward(self, logits, call):
+        """call(grad), with autograd where the logits ask for it."""
+        if not (logits.requires_grad and torch.is_grad_enabled()):
+            return call(None)[0]
+        if logits.is_leaf and torch.cuda.is_current_stream_capturing():
+            raise ValidationError("inside a captured graph the gradient of a leaf is value_and_grad's", "logits")
+        return _Loss.apply(logits, self, call)
+
+
+class PolicyLoss(_Base):
+    """The clipped policy loss of drawn tokens, with a KL term towards reference log probabilities.
+
+        loss_fn = PolicyLoss("cuda", clip=(0.2, 0.2), kl=0.0)
+        out = loss_fn(logits, tokens, old_logprobs, advantages)   # logits [..., V]; the others [...]
+        out.loss.backward()
+        out, grad = loss_fn.value_and_grad(logits, tokens, old_logprobs, advantages)   # without autograd, in one call
+
+    Per row with r = e^(log p - old_logprobs) and d = ref_logprobs - log p:
+    -min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A) + kl (e^d - 1 - d), times its weight; without weights the mean over the rows with a token.
+    logits: fp32 or bf16, rows contiguous, the leading dimensions at up to two strides.  tokens: int32 (`Sampler`'s; one
+    outside [0, V), as -1, leaves its row out).  old_logprobs (`LogProbs`'), advantages, ref_logprobs, weights,
+    temperature (0, negative or NaN: as 1): fp32, constants.  Calls run on any streams; the workspace is allocated with each call."""
+
+    def __init__(self, device="cuda", clip: Sequence[float] = (0.2, 0.2), kl: float = 0.0):
+        super().__init__(device)
+        low, high = (float(c) for c in clip)
+        if not (0.0 <= low <= 1.0 and 0.0 <= high < 1e38):
+            raise ValidationError("clip must be (in [0, 1], >= 0)", "clip", clip)
+        if not abs(float(kl)) < 1e38:
+            raise ValidationError("kl must be finite", "kl", kl)
+        self.clip, self.kl = (low, high), float(kl)
+
+    def __call__(self, logits: torch.Tensor, tokens: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor, ref_logprobs: Optional[torch.Tensor] = None,
+                 weights: Optional[torch.Tensor] = None, temperature: Optional[torch.Tensor] = None) -> PolicyLossResult:
+        call, others = self._prepare(logits, tokens, old_logprobs, advantages, ref_logprobs, weights, temperature)
+        return PolicyLossResult(self._forward(logits, call), *others)
+
+    def value_and_grad(self, logits: torch.Tensor, tokens: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor,
+                       ref_logprobs: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,
+                       temperature: Optional[torch.Tensor] = None) -> Tuple[PolicyLossResult, torch.Tensor]:
+        """(the result, the loss's gradient at the logits: their type and shape, contiguous)."""
+        call, others = self._prepare(logits, tokens, old_logprobs, advantages, ref_logprobs, weights, temperature)
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return PolicyLossResult(call(grad)[0], *others), grad
+
+    def _prepare(self, logits, tokens, old, adv, ref, weights, temperature):
+        rows = self._rows(logits, tokens, temperature)
+        lead, dev = logits.shape[:-1], logits.device
+        for t, name in ((old, "old_logprobs"), (adv, "advantages"), (ref, "ref_logprobs"), (weights, "weights")):
+            if t is not None or name in ("old_logprobs", "advantages"):
+                self._number(t, lead, dev, name)
+        n = self._state(self.lib.qws_policy_state_bytes, rows.dtype, rows.R, rows.V)
+        where, stream = on_stream(dev.index)
+        with where:
+            lp = torch.empty(lead, dtype=torch.float32, device=dev)
+            ratio = torch.empty_like(lp)
+            kl = torch.empty_like(lp) if ref is not None else None
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+
+        def call(grad):
+            with where:
+                loss = torch.empty((), dtype=torch.float32, device=dev)
+                state = torch.empty(n, dtype=torch.uint8, device=dev)
+                b = _lib.PolicyBatch(rows, old.data_ptr(), adv.data_ptr(), ptr(ref), ptr(weights), *self.clip, self.kl, loss.data_ptr(), lp.data_ptr(),
+                                     ratio.data_ptr(), ptr(kl))
+                check(self.lib.qws_policy_loss(C.byref(b), state.data_ptr(), n, ptr(grad), rows.V, stream), "qws_policy_loss")
+            return loss, rows, state, tokens
+
+        return call, (lp, ratio, kl)
+
+
+class PreferenceLoss(_Base):
+    """The loss of pairs of texts by the log ratio of their probabilities, the first of each pair preferred.
+
+        loss_fn = PreferenceLoss("cuda", beta=0.1)
+        out = loss_fn(logits, tokens, starts, ref=ref_logprobs)   # logits [R, V], tokens [R], starts [2 P + 1]
+        out.loss.backward()
+        out, grad = loss_fn.value_and_grad(logits, tokens, starts)   # without autograd, in one call
+
+    Sequence i is rows starts[i] .. starts[i + 1], 2 p the preferred one of pair p and 2 p + 1 the other; s_i is the sum (average:
+    the mean) of its tokens' log probabilities; with u = beta ((s_2p - ref_2p) - (s_2p+1 - ref_2p+1)) - margin a pair's loss is
+    -(1 - smoothing) ln sigmoid(u) - smoothing ln sigmoid(-u), times its weight; without weights the mean over the pairs.
+    logits: fp32 or bf16 [..., V], rows contiguous, the leading dimensions at up to two strides.  tokens: int32 [...]
+    (one outside [0, V), as -1 for a prompt's positions and padding, leaves its row out).  starts: int32 [2 P + 1],
+    ascending; None with logits [2 P, L, V]: a sequence each.  ref (the reference's s) [2 P], weights [P]: fp32, constants."""
+
+    def __init__(self, device="cuda", beta: float = 0.1, margin: float = 0.0, smoothing: float = 0.0, average: bool = False):
+        super().__init__(device)
+        if not (abs(float(beta)) < 1e38 and abs(float(margin)) < 1e38):
+            raise ValidationError("beta and margin must be finite", "beta", beta)
+        if not 0.0 <= float(smoothing) <= 1.0:
+            raise ValidationError("smoothing must be in [0, 1]", "smoothing", smoothing)
+        self.beta, self.margin, self.smoothing, self.average = float(beta), float(margin), float(smoothing), bool(average)
+
+    def __call__(self, logits: torch.Tensor, tokens: torch.Tensor, starts: Optional[torch.Tensor] = None, ref: Optional[torch.Tensor] = None,
+                 weights: Optional[torch.Tensor] = None) -> PreferenceLossResult:
+        call, others = self._prepare(logits, tokens, starts, ref, weights)
+        return PreferenceLossResult(self._forward(logits, call), *others)
+
+    def value_and_grad(self, logits: torch.Tensor, tokens: torch.Tensor, starts: Optional[torch.Tensor] = None, ref: Optional[torch.Tensor] = None,
+                       weights: Optional[torch.Tensor] = None) -> Tuple[PreferenceLossResult, torch.Tensor]:
+        """(the result, the loss's gradient at the logits: their type and shape, contiguous)."""
+        call, others = self._prepare(logits, tokens, starts, ref, weights)
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return PreferenceLossResult(call(grad)[0], *others), grad
+
+    def _prepare(self, logits, tokens, starts, ref, weights):
+        rows = self._rows(logits, tokens)
+        lead, dev = logits.shape[:-1], logits.device
+        if starts is None:
+            if len(lead) != 2 or lead[0] % 2:
+                raise ValidationError("without starts logits must be [2 P, L, V]", "starts")
+            P = lead[0] // 2
+        else:
+            if starts.dim() != 1 or starts.numel() % 2 == 0:
+                raise ValidationError("starts must be [2 P + 1]", "starts")
+            given(starts, starts.shape, torch.int32, dev, "starts")
+            P = starts.numel() // 2
+        for t, size, name in ((ref, 2 * P, "ref"), (weights, P, "weights")):
+            if t is not None:
+                self._number(t, (size,), dev, name)
+        n = self._state(self.lib.qws_preference_state_bytes, rows.dtype, rows.R, rows.V, P)
+        where, stream = on_stream(dev.index)
+        with where:
+            if starts is None:
+                starts = torch.arange(0, 2 * P + 1, dtype=torch.int32, device=dev).mul_(lead[1])
+            sums = torch.empty(2 * P, dtype=torch.float32, device=dev)
+            margins = torch.empty(P, dtype=torch.float32, device=dev)
+            lp = torch.empty(lead, dtype=torch.float32, device=dev)
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+
+        def call(grad):
+            with where:
+                loss = torch.empty((), dtype=torch.float32, device=dev)
+                state = torch.empty(n, dtype=torch.uint8, device=dev)
+                b = _lib.PreferenceBatch(rows, starts.data_ptr(), P, int(self.average), ptr(ref), ptr(weights), self.beta, self.margin, self.smoothing,
+                                         loss.data_ptr(), sums.data_ptr(), margins.data_ptr(), lp.data_ptr())
+                check(self.lib.qws_preference_loss(C.byref(b), state.data_ptr(), n, ptr(grad), rows.V, stream), "qws_preference_loss")
+            return loss, rows, state, tokens
+
+        return call, (sums, margins, lp)

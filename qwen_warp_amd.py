@@ -12,3 +12,4 @@ from qwen_warp_amd.head import HeadSelect  # noqa: E402,F401
 from qwen_warp_amd.logprobs import LogProbs, LogProbsResult  # noqa: E402,F401
 from qwen_warp_amd.fp8 import Fp8Head  # noqa: E402,F401
 from qwen_warp_amd.int4 import Int4Head  # noqa: E402,F401
+from qwen_warp_amd.losses import PolicyLoss, PolicyLossResult, PreferenceLoss, PreferenceLossResult  # noqa: E402,F401
