@@ -107,7 +107,7 @@ EXPORTS = ("qws_sample_ws_bytes", "qws_sample", "qws_sample_noalloc", "qws_verif
            "qws_finish", "qws_finish_rows", "qws_finish_forced", "qws_head_ws_bytes", "qws_head_select_rescore", "qws_head_ws_cand", "qws_head_ws_exact",
            "qws_logprobs_ws_bytes", "qws_logprobs", "qws_fp8_pack_bytes", "qws_fp8_pack", "qws_fp8_head_ws_bytes", "qws_fp8_head", "qws_fp8_score_ws_bytes",
            "qws_fp8_score", "qws_int4_pack_bytes", "qws_int4_pack", "qws_int4_pack_codes", "qws_int4_head_ws_bytes", "qws_int4_head",
-           "qws_policy_state_bytes", "qws_policy_loss", "qws_preference_state_bytes", "qws_preference_loss", "qws_loss_grad", "qws_pld_default_cfg", "qws_pld_bytes", "qws_pld_reset", "qws_pld_append", "qws_pld_propose",
+           "qws_policy_state_bytes", "qws_policy_loss", "qws_preference_state_bytes", "qws_preference_loss", "qws_policy_one_pass", "qws_loss_grad", "qws_pld_default_cfg", "qws_pld_bytes", "qws_pld_reset", "qws_pld_append", "qws_pld_propose",
            "qws_row_init", "qws_row_check", "qws_abi_sizes",
            "qws_timing", "qws_timing_read", "qws_timing_read_verify", "qws_test_philox", "qws_test_proc_logits", "qws_test_dist")
 
@@ -166,7 +166,8 @@ def load(path=None):
     lib.qws_policy_loss.argtypes, lib.qws_policy_loss.restype = [C.POINTER(PolicyBatch), vp, sz, vp, ll, vp], ci
     lib.qws_preference_state_bytes.argtypes, lib.qws_preference_state_bytes.restype = [ci] * 4, sz
     lib.qws_preference_loss.argtypes, lib.qws_preference_loss.restype = [C.POINTER(PreferenceBatch), vp, sz, vp, ll, vp], ci
-    lib.qws_loss_grad.argtypes, lib.qws_loss_grad.restype = [C.POINTER(LossRows), vp, vp, vp, ll, vp], ci
+    lib.qws_policy_one_pass.argtypes, lib.qws_policy_one_pass.restype = [ci] * 3, ci
+    lib.qws_loss_grad.argtypes, lib.qws_loss_grad.restype = [C.POINTER(LossRows), vp, vp, vp, ll, ci, vp], ci
     lib.qws_pld_default_cfg.argtypes, lib.qws_pld_default_cfg.restype = [C.POINTER(PldCfg)], None
     lib.qws_pld_bytes.argtypes, lib.qws_pld_bytes.restype = [ci, ci], sz
     lib.qws_pld_reset.argtypes, lib.qws_pld_reset.restype = [vp, ci, ci, ci, vp, ci, vp], ci

@@ -125,20 +125,15 @@ __device__ __forceinline__ void ls_slow(LsSum& v, const float (&x)[U][E], float 
 }
 
 template <typename T>
-constexpr int ls_stripe() { return LS_NT * lp_e<T>(); }
+constexpr int ls_stripe(int nt = LS_NT) { return nt * lp_e<T>(); }
 
-template <typename T, int U>
-__global__ void __launch_bounds__(LS_NT, 5) k_ls_scan(LsArgs a) {
-  constexpr int E = lp_e<T>(), SE = ls_stripe<T>();
-  __shared__ LsSum s_sum[LS_NW];
-  const int tid = threadIdx.x, lane = lane_id(), wave = wave_id();
-  const int row = blockIdx.x / a.G, ch = blockIdx.x % a.G;
-  if (ls_token(a, row) < 0) return;  // no one reads its parts
-  const T* p = ls_row<T>(a, row);
-  const int lead = (int)((uintptr_t)p / sizeof(T)) & (E - 1), end = lead + a.V;
+// The maximum and sum of stripes s_begin .. s_end of a row by NT threads; lane's own
+template <typename T, int U, int NT>
+__device__ __forceinline__ LsSum ls_scan_part(const T* p, int V, int s_begin, int s_end, float c) {
+  constexpr int E = lp_e<T>(), SE = ls_stripe<T>(NT);
+  const int tid = threadIdx.x, lead = (int)((uintptr_t)p / sizeof(T)) & (E - 1), end = lead + V;
   const T* base = p - lead;
-  const float c = lse_scale(a.temp ? a.temp[row] : 1.0f);
-  const int nstripes = (end + SE - 1) / SE, s_begin = ch * a.per, s_end = min(s_begin + a.per, nstripes);
+  s_end = min(s_end, (end + SE - 1) / SE);
   vu4 r[U];
   auto load = [&](int s) {
     const int first = s * SE;
@@ -167,14 +162,30 @@ __global__ void __launch_bounds__(LS_NT, 5) k_ls_scan(LsArgs a) {
     const Lse q = lse_exact(f.m, f.M, f.s, 0.0f, c);
     v = ls_join(v, {q.m, q.s}, c);
   }
+  return v;
+}
+// joined over the workgroup, in thread 0
+template <int NT>
+__device__ __forceinline__ LsSum ls_join_group(LsSum v, float c, LsSum* s_sum) {
   v = ls_join_wave(v, c);
-  if (lane == 0) s_sum[wave] = v;
+  if (lane_id() == 0) s_sum[wave_id()] = v;
   bar();
-  if (tid == 0) {
+  if (threadIdx.x == 0) {
 #pragma unroll
-    for (int w = 1; w < LS_NW; w++) v = ls_join(v, s_sum[w], c);
-    a.part[(size_t)row * a.G + ch] = make_float2(v.m, v.s);
+    for (int w = 1; w < NT / 64; w++) v = ls_join(v, s_sum[w], c);
   }
+  return v;
+}
+
+template <typename T, int U>
+__global__ void __launch_bounds__(LS_NT, 5) k_ls_scan(LsArgs a) {
+  __shared__ LsSum s_sum[LS_NW];
+  const int row = blockIdx.x / a.G, ch = blockIdx.x % a.G;
+  if (ls_token(a, row) < 0) return;  // no one reads its parts
+  const float c = lse_scale(a.temp ? a.temp[row] : 1.0f);
+  LsSum v = ls_scan_part<T, U, LS_NT>(ls_row<T>(a, row), a.V, ch * a.per, ch * a.per + a.per, c);
+  v = ls_join_group<LS_NT>(v, c, s_sum);
+  if (threadIdx.x == 0) a.part[(size_t)row * a.G + ch] = make_float2(v.m, v.s);
 }
 
 // A row's parts joined by a wave
@@ -264,10 +275,9 @@ __device__ __forceinline__ int ls_sequence(const LsArgs& a, int row) {
   }
   return lo;
 }
+// one wave
 template <typename T>
-__global__ void __launch_bounds__(LS_NT) k_ls_rows(LsArgs a) {
-  const int row = blockIdx.x * LS_NW + wave_id();
-  if (row >= a.R) return;
+__device__ __forceinline__ void ls_preference_row(const LsArgs& a, int row) {
   const int tok = ls_token(a, row), seq = ls_sequence(a, row);
   const float temp = a.temp ? a.temp[row] : 1.0f, c = lse_scale(temp);
   const LsSum v = tok < 0 ? LsSum{-INFINITY, 0.0f} : ls_parts(a, row, c);
@@ -279,6 +289,11 @@ __global__ void __launch_bounds__(LS_NT) k_ls_rows(LsArgs a) {
   a.lp[row] = lp;
   if (a.out_lp) a.out_lp[row] = tok >= 0 ? (float)lp : 0.0f;
 }
+template <typename T>
+__global__ void __launch_bounds__(LS_NT) k_ls_rows(LsArgs a) {
+  const int row = blockIdx.x * LS_NW + wave_id();
+  if (row < a.R) ls_preference_row<T>(a, row);
+}
 
 // One wave: pair i's term; the slopes and results of its sequences
 __device__ __forceinline__ double ls_pair(const LsArgs& a, int i) {
@@ -289,10 +304,17 @@ __device__ __forceinline__ double ls_pair(const LsArgs& a, int i) {
     const int from = ls_start(a, 2 * i + h), to = ls_start(a, 2 * i + h + 1);
     double s = 0.0;
     int n = 0;
-    for (int r = from + lane_id(); r < to; r += 64) {
-      const double p = a.lp[r];
-      if (p > -INFINITY) s += p;
-      if (p == p) n++;
+    constexpr int U = 8;  // loaded together
+    for (int r = from + lane_id(); r < to; r += 64 * U) {
+      double p[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) p[u] = a.lp[min(r + 64 * u, a.R - 1)];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (r + 64 * u < to) {
+          if (p[u] > -INFINITY) s += p[u];
+          if (p[u] == p[u]) n++;
+        }
     }
     sum[h] = wave_sum<double>(s);
     count[h] = a.average ? max(wave_sum<int>(n), 1) : 1;
@@ -321,17 +343,11 @@ __global__ void __launch_bounds__(LS_NT) k_ls_pairs(LsArgs a) {
   if (lane_id() == 0) a.term[i] = term;
 }
 
-// One workgroup: the sum of n terms, in a fixed order.  Without weights it is their mean: over the rows with a token, or the pairs.
-template <bool POLICY>
-__global__ void __launch_bounds__(LS_ONE) k_ls_sum(LsArgs a, int n) {
+// The loss from the threads' sums of terms and counts, in a fixed order.  Without weights it is their mean: over the rows with a
+// token, or the pairs.
+__device__ __forceinline__ void ls_total(const LsArgs& a, double s, int k, int pairs) {
   __shared__ double s_sum[LS_ONE / 64];
   __shared__ int s_count[LS_ONE / 64];
-  double s = 0.0;
-  int k = 0;
-  for (int i = threadIdx.x; i < n; i += LS_ONE) {
-    s += a.term[i];
-    if (POLICY) k += ls_token(a, i) >= 0;
-  }
   s = wave_sum<double>(s);
   k = wave_sum<int>(k);
   if (lane_id() == 0) {
@@ -344,15 +360,48 @@ __global__ void __launch_bounds__(LS_ONE) k_ls_sum(LsArgs a, int n) {
     s += s_sum[w];
     k += s_count[w];
   }
-  if (!POLICY) k = n;
+  if (pairs) k = pairs;
   const double scale = a.weights || k == 0 ? 1.0 : 1.0 / k;
   a.head->loss = s * scale;
   a.head->scale = (float)scale;
   *a.out_loss = (float)(s * scale);
 }
+// One workgroup: the loss of n terms
+template <bool POLICY>
+__global__ void __launch_bounds__(LS_ONE) k_ls_sum(LsArgs a, int n) {
+  double s = 0.0;
+  int k = 0;
+  for (int i = threadIdx.x; i < n; i += LS_ONE) {
+    s += a.term[i];
+    if (POLICY) k += ls_token(a, i) >= 0;
+  }
+  ls_total(a, s, k, POLICY ? 0 : n);
+}
+// One workgroup for a few pairs (and, with ROWS, a few rows): rows, pairs and the loss without launches between them, 3 us of the
+// host's time and as much of the card's each.
+constexpr int LS_FEW = 64;
+template <typename T, bool ROWS>
+__global__ void __launch_bounds__(LS_ONE) k_ls_few(LsArgs a) {
+  if constexpr (ROWS) {
+    for (int row = wave_id(); row < a.R; row += LS_ONE / 64) ls_preference_row<T>(a, row);
+    __syncthreads();  // the rows' log probabilities are other waves' in memory
+  }
+  double s = 0.0;
+  for (int i = wave_id(); i < a.P; i += LS_ONE / 64) {
+    const double term = ls_pair(a, i);
+    if (lane_id() == 0) s += term;
+  }
+  ls_total(a, s, 0, a.P);
+}
 
 // ------------------------------------------------------------------------------------------------ the gradient's rows
 typedef vu4 ls_any __attribute__((aligned(2)));  // 16 bytes at any element: the hardware takes them
+// the vector at place v of `base`, at any element, of which [lead, end) exist: the rest reads -inf
+template <typename T>
+__device__ __forceinline__ vu4 lp_load_any(const T* base, int v, int lead, int end) {
+  if (v >= lead && v + lp_e<T>() <= end) return *(const QWS_G ls_any*)(base + v);
+  return lp_load_edge(base, v, lead, end);
+}
 template <typename T, int E>
 __device__ __forceinline__ vu4 ls_pack(const float* y) {
   vu4 r;
@@ -385,20 +434,45 @@ __device__ __forceinline__ void ls_slopes(const LsRow& q, const float* x, float*
   }
 }
 
-template <typename T, int U>
-__global__ void __launch_bounds__(LS_NT) k_ls_grad(LsArgs a) {
-  constexpr int E = lp_e<T>(), SE = ls_stripe<T>();
-  const int tid = threadIdx.x, row = blockIdx.x / a.G, ch = blockIdx.x % a.G;
-  const LsRow q = a.rows[row];
-  T* out = (T*)a.grad + (long long)row * a.grad_stride;
+// the vector at place j0, of which [lead, end) exist
+template <typename T>
+__device__ __forceinline__ void ls_grad_edge(const LsRow& q, const T* base, T* to, int lead, int end, int j0, int tok, float k, float slope) {
+  constexpr int E = lp_e<T>();
+  const bool zero = slope == 0.0f;
+  if (j0 >= lead && j0 + E <= end) {
+    float x[E], y[E];
+    vu4 w = {0, 0, 0, 0};
+    if (!zero) {
+      const vu4 r = *(const QWS_G ls_any*)(base + j0);
+      lp_unpack<T>(r, x);
+      ls_slopes<E>(q, x, y, k, slope, tok, j0);
+      w = ls_pack<T, E>(y);
+    }
+    *(vu4*)(to + j0) = w;
+    return;
+  }
+  for (int j = max(j0, lead); j < min(j0 + E, end); j++) {
+    float x, y = 0.0f;
+    if constexpr (sizeof(T) == 4)
+      x = *gmem((const float*)base + j);
+    else
+      x = __uint_as_float((uint32_t)*gmem((const uint16_t*)base + j) << 16);
+    if (!zero) ls_slopes<1>(q, &x, &y, k, slope, tok, j);
+    if constexpr (sizeof(T) == 4)
+      *((float*)to + j) = y;
+    else
+      *((__bf16*)to + j) = (__bf16)y;
+  }
+}
+// Stripes s_begin .. s_end of a row's gradient
+template <typename T, int U, int NT>
+__device__ __forceinline__ void ls_grad_part(const LsRow& q, const T* x_row, T* out, int V, int s_begin, int s_end, float slope) {
+  constexpr int E = lp_e<T>(), SE = ls_stripe<T>(NT);
   // aligned to the gradient's vectors; the logits' loads are at any element
-  const int lead = (int)((uintptr_t)out / sizeof(T)) & (E - 1), end = lead + a.V;
-  const T* base = ls_row<T>(a, row) - lead;
+  const int tid = threadIdx.x, lead = (int)((uintptr_t)out / sizeof(T)) & (E - 1), end = lead + V;
+  const T* base = x_row - lead;
   T* to = out - lead;
-  const int nstripes = (end + SE - 1) / SE, s_begin = ch * a.per, s_end = min(s_begin + a.per, nstripes);
-  float slope = 0.0f;
-  if (q.mode) slope = a.slope[q.slot] * a.head->scale * (a.upstream ? *a.upstream : 1.0f) * q.per_t;
-  if (fabsf(slope) > 0.25f * F32_MAX) slope = copysignf(0.25f * F32_MAX, slope);  // no infinity meets a p of 0; NaN stays
+  s_end = min(s_end, (end + SE - 1) / SE);
   const float k = -slope * q.inv;
   const bool zero = slope == 0.0f;
   const int tok = q.tok + lead;
@@ -423,24 +497,159 @@ __global__ void __launch_bounds__(LS_NT) k_ls_grad(LsArgs a) {
         *(vu4*)(to + j0) = w;
       }
     } else {
-      for (int u = 0; u < U && s + u < s_end; u++) {
-        const int j0 = first + u * SE + tid * E;
-        for (int j = j0; j < j0 + E; j++)
-          if (j >= lead && j < end) {
-            float x, y = 0.0f;
-            if constexpr (sizeof(T) == 4)
-              x = *gmem((const float*)base + j);
-            else
-              x = __uint_as_float((uint32_t)*gmem((const uint16_t*)base + j) << 16);
-            if (!zero) ls_slopes<1>(q, &x, &y, k, slope, tok, j);
-            if constexpr (sizeof(T) == 4)
-              *((float*)to + j) = y;
-            else
-              *((__bf16*)to + j) = (__bf16)y;
-          }
-      }
+      for (int u = 0; u < U && s + u < s_end; u++) ls_grad_edge<T>(q, base, to, lead, end, first + u * SE + tid * E, tok, k, slope);
     }
   }
+}
+__device__ __forceinline__ float ls_held(float slope) {  // no infinity meets a p of 0; NaN stays
+  return fabsf(slope) > 0.25f * F32_MAX ? copysignf(0.25f * F32_MAX, slope) : slope;
+}
+
+// written: the gradient is there for an upstream of 1.  Rows from the last on: the logits that k_ls_scan read last may still be in the
+// memory's cache.
+template <typename T, int U>
+__global__ void __launch_bounds__(LS_NT) k_ls_grad(LsArgs a, int written) {
+  const float upstream = a.upstream ? *a.upstream : 1.0f;
+  if (written && upstream == 1.0f) return;
+  const float scale = a.head->scale * upstream;
+  for (unsigned i = blockIdx.x; i < (unsigned)a.R * a.G; i += gridDim.x) {
+    const int row = a.R - 1 - (int)(i / a.G), ch = i % a.G;
+    const LsRow q = a.rows[row];
+    const float slope = q.mode ? ls_held(a.slope[q.slot] * scale * q.per_t) : 0.0f;
+    ls_grad_part<T, U, LS_NT>(q, ls_row<T>(a, row), (T*)a.grad + (long long)row * a.grad_stride, a.V, ch * a.per, ch * a.per + a.per, slope);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the policy loss, a row at a time
+// A workgroup per row: its maximum and sum, its term and slope, its gradient.  Of the row's stripes that lie inside it, NL stay in
+// LDS and NV in registers between the two passes; the others are read again, the last ones first.
+template <typename T, int NT, int NV, int NL>
+__global__ void __launch_bounds__(NT) k_ls_policy(LsArgs a) {
+  constexpr int E = lp_e<T>(), SE = ls_stripe<T>(NT), U = E == 8 ? 2 : 4;
+  static_assert(NV % U == 0 && NL % U == 0 && NV >= 2 * U, "blocks");
+  extern __shared__ __attribute__((aligned(16))) char s_mem[];
+  vu4* held = (vu4*)s_mem + threadIdx.x;  // [NL][NT]: a thread's own
+  __shared__ LsSum s_sum[NT / 64];
+  __shared__ LsRow s_row;
+  __shared__ float s_slope;
+  const int tid = threadIdx.x, row = blockIdx.x, tok = ls_token(a, row);
+  const float temp = a.temp ? a.temp[row] : 1.0f, c = lse_scale(temp);
+  T* out = (T*)a.grad + (long long)row * a.grad_stride;
+  const int lead = (int)((uintptr_t)out / sizeof(T)) & (E - 1), end = lead + a.V;
+  const T* base = ls_row<T>(a, row) - lead;
+  T* to = out - lead;
+  const int stripes = (end + SE - 1) / SE, s0 = lead ? 1 : 0, full = max(end / SE - s0, 0) / U * U;  // whole stripes from s0 on, in blocks
+  const int in_lds = min(full, NL), in_regs = min(full - in_lds, NV), s1 = s0 + in_lds, s2 = s1 + in_regs;
+  vu4 r[NV];
+  LsSum v = {-INFINITY, 0.0f};
+  LsFast f = {-INFINITY, -1e30f, -INFINITY, 0.0f};
+  auto vec = [&](int s) { return *(const QWS_G ls_any*)(base + s * SE + tid * E); };
+  auto add = [&](const vu4* w) {
+    float x[U][E], best = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      lp_unpack<T>(w[u], x[u]);
+      best = fmaxf(best, lp_max<E>(x[u]));
+    }
+    if (!ls_fast(f, x, best, c)) ls_slow(v, x, fminf(best, F32_MAX), c);
+  };
+  if (tok >= 0) {
+    if constexpr (NL > 0) {
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (in_lds) r[u] = vec(s0 + u);
+#pragma unroll
+      for (int i = 0; i < NL; i += U)
+        if (i < in_lds) {
+          vu4* now = r + i / U % 2 * U;
+          vu4* next = r + (i / U + 1) % 2 * U;
+          if (i + U < in_lds) {
+#pragma unroll
+            for (int u = 0; u < U; u++) next[u] = vec(s0 + i + U + u);
+          }
+          add(now);
+#pragma unroll
+          for (int u = 0; u < U; u++) held[(i + u) * NT] = now[u];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+      if (i < in_regs) r[i] = vec(s1 + i);
+#pragma unroll
+    for (int i = 0; i < NV; i += U)
+      if (i < in_regs) add(r + i);
+    // the rest: whole blocks, then what is left of the row's ends
+    vu4 w[U];
+    int s = s2;
+    for (; s < s0 + full; s += U) {
+#pragma unroll
+      for (int u = 0; u < U; u++) w[u] = vec(s + u);
+      add(w);
+    }
+    for (; s < stripes + s0; s += U) {  // stripe 0, where it is not whole, at the end
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int at = s + u < stripes ? s + u : 0;
+        w[u] = lp_load_any(base, at * SE + tid * E, s + u < stripes + s0 ? lead : end, end);
+      }
+      add(w);
+    }
+    if (f.m != -INFINITY) {
+      const Lse q = lse_exact(f.m, f.M, f.s, 0.0f, c);
+      v = ls_join(v, {q.m, q.s}, c);
+    }
+  }
+  v = ls_join_group<NT>(v, c, s_sum);
+  if (tid == 0) {
+    a.term[row] = ls_policy<T>(a, row, tok, v, c, temp);
+    const LsRow q = a.rows[row];  // this thread's own
+    s_row = q;
+    s_slope = q.mode ? ls_held(a.slope[row] * (a.weights ? 1.0f : a.head->scale) * q.per_t) : 0.0f;
+  }
+  bar();
+  const LsRow q = s_row;
+  const float slope = s_slope, k = -slope * q.inv;
+  const bool zero = slope == 0.0f;
+  const int at_tok = q.tok + lead;
+  auto put = [&](int s, vu4 w) {
+    const int j0 = s * SE + tid * E;
+    float x[E], y[E];
+    lp_unpack<T>(w, x);
+    ls_slopes<E>(q, x, y, k, slope, at_tok, j0);
+    *(vu4*)(to + j0) = ls_pack<T, E>(y);
+  };
+  if (zero) {
+    for (int s = 0; s < stripes; s++) ls_grad_edge<T>(q, base, to, lead, end, s * SE + tid * E, at_tok, k, slope);
+    return;
+  }
+  for (int s = stripes + s0 - 1; s >= s0 + full; s--) ls_grad_edge<T>(q, base, to, lead, end, (s < stripes ? s : 0) * SE + tid * E, at_tok, k, slope);
+  for (int s = s0 + full - U; s >= s2; s -= U) {
+    vu4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) w[u] = vec(s + u);
+#pragma unroll
+    for (int u = 0; u < U; u++) put(s + u, w[u]);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; i++)
+    if (i < in_regs) put(s1 + i, r[i]);
+  if constexpr (NL > 0) {
+#pragma unroll 2
+    for (int i = 0; i < NL; i++)
+      if (i < in_lds) put(s0 + i, held[i * NT]);
+  }
+}
+// One workgroup: without weights, the scale of the slopes is known before them: 1 over the rows with a token
+__global__ void __launch_bounds__(LS_ONE) k_ls_count(LsArgs a) {
+  __shared__ int s_count[LS_ONE / 64];
+  int k = 0;
+  for (int i = threadIdx.x; i < a.R; i += LS_ONE) k += ls_token(a, i) >= 0;
+  k = wave_sum<int>(k);
+  if (lane_id() == 0) s_count[wave_id()] = k;
+  bar();
+  if (threadIdx.x) return;
+  for (int w = 1; w < LS_ONE / 64; w++) k += s_count[w];
+  a.head->scale = k ? (float)(1.0 / k) : 1.0f;
 }
 
 // ------------------------------------------------------------------------------------------------ the host's side
@@ -511,13 +720,40 @@ static void ls_scan(const LsArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((k_ls_scan<T, LS_U>), dim3((unsigned)a.R * a.G), dim3(LS_NT), 0, st, a);
 }
 template <typename T>
-static void ls_grad_of(const LsArgs& a, hipStream_t st) {
+static void ls_grad_of(const LsArgs& a, int written, hipStream_t st) {
+  unsigned wgs = (unsigned)a.R * a.G;
+  if (written && wgs > 1024) wgs = 1024;  // most often they find it written
   if (a.per == 1)
-    hipLaunchKernelGGL((k_ls_grad<T, 1>), dim3((unsigned)a.R * a.G), dim3(LS_NT), 0, st, a);
+    hipLaunchKernelGGL((k_ls_grad<T, 1>), dim3(wgs), dim3(LS_NT), 0, st, a, written);
   else
-    hipLaunchKernelGGL((k_ls_grad<T, LS_U>), dim3((unsigned)a.R * a.G), dim3(LS_NT), 0, st, a);
+    hipLaunchKernelGGL((k_ls_grad<T, LS_U>), dim3(wgs), dim3(LS_NT), 0, st, a, written);
 }
-static void ls_grad(const LsArgs& a, int dtype, hipStream_t st) { dtype == QWS_DTYPE_F32 ? ls_grad_of<float>(a, st) : ls_grad_of<uint16_t>(a, st); }
+static void ls_grad(const LsArgs& a, int dtype, int written, hipStream_t st) {
+  dtype == QWS_DTYPE_F32 ? ls_grad_of<float>(a, written, st) : ls_grad_of<uint16_t>(a, written, st);
+}
+// Whether a policy loss with its gradient takes a workgroup per row (k_ls_policy): from 128 rows on, or where the row's workgroup holds
+// all of it (up to 12,288 vectors).  Measured, us a call, k_ls_policy / the three launches: 248,320 bf16 logits, 64 rows 38 / 29, 100 rows 39 /
+// 32, 150 rows 42 / 45, 256 rows 56 / 77, 2,048 rows 417 / 571; fp32, 64 rows 45 / 36, 192 rows 112 / 115, 512 rows 254 / 296;
+// 32,001 bf16 logits, 64 rows 26 / 29, 1,024 rows 32 / 42.
+constexpr int LS_HELD = 512 * 24;
+static int ls_vectors(int dtype, int V) { return V / (dtype == QWS_DTYPE_F32 ? 4 : 8); }
+static bool ls_one_pass(int dtype, int R, int V) { return R >= 128 || ls_vectors(dtype, V) <= LS_HELD; }
+template <typename T, int NT, int NV, int NL>
+static void ls_policy_rows(const LsArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((k_ls_policy<T, NT, NV, NL>), dim3(a.R), dim3(NT), NL * NT * 16, st, a);
+}
+// The least workgroup that holds a row: 2,048 bf16 rows, us with 256 x 16 / 512 x 24 / 1,024 x 24 vectors: of 16,000 logits 33 / 42 / 64,
+// of 32,001 65 / 72 / 95, of 40,000 82 / 81 / 101, of 100,000 221 / 181 / 188, of 130,000 308 / 239 / 244, of 200,000 439 / 376 / 347.
+template <typename T>
+static void ls_policy_one_pass(const LsArgs& a, hipStream_t st) {
+  const int n = a.V / lp_e<T>();
+  if (n <= 256 * 16)
+    ls_policy_rows<T, 256, 16, 0>(a, st);
+  else if (n <= LS_HELD)
+    ls_policy_rows<T, 512, 16, 8>(a, st);
+  else
+    ls_policy_rows<T, 1024, 16, 8>(a, st);
+}
 template <typename T>
 static void ls_policy_run(const LsArgs& a, hipStream_t st) {
   ls_scan<T>(a, st);
@@ -525,8 +761,18 @@ static void ls_policy_run(const LsArgs& a, hipStream_t st) {
 }
 template <typename T>
 static void ls_preference_run(const LsArgs& a, hipStream_t st) {
-  ls_scan<T>(a, st);
-  hipLaunchKernelGGL((k_ls_rows<T>), dim3((a.R + LS_NW - 1) / LS_NW), dim3(LS_NT), 0, st, a);
+  if (a.R) ls_scan<T>(a, st);
+  if (a.P <= LS_FEW && a.R <= LS_FEW) {
+    hipLaunchKernelGGL((k_ls_few<T, true>), dim3(1), dim3(LS_ONE), 0, st, a);
+    return;
+  }
+  if (a.R) hipLaunchKernelGGL((k_ls_rows<T>), dim3((a.R + LS_NW - 1) / LS_NW), dim3(LS_NT), 0, st, a);
+  if (a.P <= LS_FEW) {
+    hipLaunchKernelGGL((k_ls_few<T, false>), dim3(1), dim3(LS_ONE), 0, st, a);
+    return;
+  }
+  hipLaunchKernelGGL(k_ls_pairs, dim3((a.P + LS_NW - 1) / LS_NW), dim3(LS_NT), 0, st, a);
+  hipLaunchKernelGGL((k_ls_sum<false>), dim3(1), dim3(LS_ONE), 0, st, a, a.P);
 }
 static bool ls_aligned(const void* p) { return p && ((uintptr_t)p & 255) == 0; }
 static bool ls_launches(const LsArgs& a) { return (long long)a.R * a.G <= 0xFFFFFF; }  // below 2^32 threads
@@ -568,12 +814,20 @@ extern "C" int qws_policy_loss(const qws_policy_batch* b, void* state, size_t st
   a.out_ratio = b->out_ratio;
   a.out_kl = b->out_kl;
   hipStream_t st = (hipStream_t)stream;
+  if (R && grad && ls_one_pass(b->rows.dtype, R, V)) {
+    a.grad = grad;
+    a.grad_stride = grad_stride;
+    if (!a.weights) hipLaunchKernelGGL(k_ls_count, dim3(1), dim3(LS_ONE), 0, st, a);
+    b->rows.dtype == QWS_DTYPE_F32 ? ls_policy_one_pass<float>(a, st) : ls_policy_one_pass<uint16_t>(a, st);
+    hipLaunchKernelGGL((k_ls_sum<true>), dim3(1), dim3(LS_ONE), 0, st, a, R);
+    return (int)hipGetLastError();
+  }
   if (R) b->rows.dtype == QWS_DTYPE_F32 ? ls_policy_run<float>(a, st) : ls_policy_run<uint16_t>(a, st);
   hipLaunchKernelGGL((k_ls_sum<true>), dim3(1), dim3(LS_ONE), 0, st, a, R);
   if (R && grad) {
     a.grad = grad;
     a.grad_stride = grad_stride;
-    ls_grad(a, b->rows.dtype, st);
+    ls_grad(a, b->rows.dtype, 0, st);
   }
   return (int)hipGetLastError();
 }
@@ -602,18 +856,18 @@ extern "C" int qws_preference_loss(const qws_preference_batch* b, void* state, s
   a.out_sums = b->out_logprobs;
   a.out_margins = b->out_margins;
   hipStream_t st = (hipStream_t)stream;
-  if (R) b->rows.dtype == QWS_DTYPE_F32 ? ls_preference_run<float>(a, st) : ls_preference_run<uint16_t>(a, st);
-  if (P) hipLaunchKernelGGL(k_ls_pairs, dim3((P + LS_NW - 1) / LS_NW), dim3(LS_NT), 0, st, a);
-  hipLaunchKernelGGL((k_ls_sum<false>), dim3(1), dim3(LS_ONE), 0, st, a, P);
+  b->rows.dtype == QWS_DTYPE_F32 ? ls_preference_run<float>(a, st) : ls_preference_run<uint16_t>(a, st);
   if (R && grad) {
     a.grad = grad;
     a.grad_stride = grad_stride;
-    ls_grad(a, b->rows.dtype, st);
+    ls_grad(a, b->rows.dtype, 0, st);
   }
   return (int)hipGetLastError();
 }
 
-extern "C" int qws_loss_grad(const qws_loss_rows* r, const void* state, const float* upstream, void* grad, long long grad_stride, void* stream) {
+extern "C" int qws_policy_one_pass(int dtype, int R, int V) { return R > 0 && V > 0 && qws::ls_one_pass(dtype, R, V); }
+
+extern "C" int qws_loss_grad(const qws_loss_rows* r, const void* state, const float* upstream, void* grad, long long grad_stride, int written, void* stream) {
   using namespace qws;
   if (!r || !ls_rows_ok(*r) || !ls_aligned(state) || (r->R && (!grad || !ls_grad_ok(*r, grad, grad_stride)))) return QWS_ERR_INVALID;
   if (!ls_fits(r->R, r->V)) return QWS_ERR_NOT_SUPPORTED;
@@ -623,6 +877,6 @@ extern "C" int qws_loss_grad(const qws_loss_rows* r, const void* state, const fl
   a.upstream = upstream;
   a.grad = grad;
   a.grad_stride = grad_stride;
-  ls_grad(a, r->dtype, (hipStream_t)stream);
+  ls_grad(a, r->dtype, written && upstream, (hipStream_t)stream);
   return (int)hipGetLastError();
 }

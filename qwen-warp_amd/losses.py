@@ -56,11 +56,14 @@ def blocks_of(x: torch.Tensor, name: str):
 
 
 class _Loss(torch.autograd.Function):
-    """The loss as a function of the logits; `call(None)` runs it and returns (loss, rows, state, what they refer to)."""
+    """The loss as a function of the logits; `call(grad)` runs it and returns (loss, rows, state, what they refer to).  With
+    `ahead` the gradient is written by the forward pass, for an upstream gradient of 1; the first backward pass hands it out, after
+    a launch that writes it anew for any other.  Later ones write their own."""
 
     @staticmethod
-    def forward(ctx, logits, owner, call):
-        loss, ctx.rows, ctx.state, ctx.keep = call(None)
+    def forward(ctx, logits, owner, call, ahead):
+        ctx.grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if ahead else None
+        loss, ctx.rows, ctx.state, ctx.keep = call(ctx.grad)
         ctx.owner = owner
         ctx.save_for_backward(logits)
         return loss
@@ -71,10 +74,14 @@ class _Loss(torch.autograd.Function):
         (logits,) = ctx.saved_tensors
         where, stream = on_stream(logits.device.index)
         with where:
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            grad, ctx.grad = ctx.grad, None
+            written = grad is not None
+            if not written:
+                grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
             upstream = upstream.contiguous()
-            check(ctx.owner.lib.qws_loss_grad(C.byref(ctx.rows), ctx.state.data_ptr(), upstream.data_ptr(), grad.data_ptr(), logits.shape[-1], stream), "qws_loss_grad")
-        return grad, None, None
+            check(ctx.owner.lib.qws_loss_grad(C.byref(ctx.rows), ctx.state.data_ptr(), upstream.data_ptr(), grad.data_ptr(), logits.shape[-1], written, stream),
+                  "qws_loss_grad")
+        return grad, None, None, None
 
 
 class _Base:
@@ -116,13 +123,13 @@ class _Base:
             raise ValidationError("logits: fewer than 2^24 rows of at most 2^24 values", "logits")
         return n
 
-    def _forward(self, logits, call):
+    def _forward(self, logits, call, ahead=False):
         """call(grad), with autograd where the logits ask for it."""
         if not (logits.requires_grad and torch.is_grad_enabled()):
             return call(None)[0]
         if logits.is_leaf and torch.cuda.is_current_stream_capturing():
             raise ValidationError("inside a captured graph the gradient of a leaf is value_and_grad's", "logits")
-        return _Loss.apply(logits, self, call)
+        return _Loss.apply(logits, self, call, ahead)
 
 
 class PolicyLoss(_Base):
@@ -151,7 +158,9 @@ class PolicyLoss(_Base):
     def __call__(self, logits: torch.Tensor, tokens: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor, ref_logprobs: Optional[torch.Tensor] = None,
                  weights: Optional[torch.Tensor] = None, temperature: Optional[torch.Tensor] = None) -> PolicyLossResult:
         call, others = self._prepare(logits, tokens, old_logprobs, advantages, ref_logprobs, weights, temperature)
-        return PolicyLossResult(self._forward(logits, call), *others)
+        # from some size on the gradient comes on the loss's own way over the logits
+        ahead = bool(self.lib.qws_policy_one_pass(_lib.DTYPE_F32 if logits.dtype == torch.float32 else _lib.DTYPE_BF16, others[0].numel(), logits.shape[-1]))
+        return PolicyLossResult(self._forward(logits, call, ahead), *others)
 
     def value_and_grad(self, logits: torch.Tensor, tokens: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor,
                        ref_logprobs: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,

@@ -135,12 +135,12 @@ def test_sizes_and_refusals():
     for kw in (dict(starts=None), dict(P=-1), dict(beta=nan), dict(margin=inf), dict(smoothing=-0.1), dict(smoothing=1.1), dict(smoothing=nan)):
         assert preference(**kw) == _lib.ERR_INVALID, kw
     r = rows()
-    assert lib.qws_loss_grad(None, 256, None, 256, 10, None) == _lib.ERR_INVALID
-    assert lib.qws_loss_grad(C.byref(r), None, None, 256, 10, None) == _lib.ERR_INVALID
-    assert lib.qws_loss_grad(C.byref(r), 256, None, None, 10, None) == _lib.ERR_INVALID
-    assert lib.qws_loss_grad(C.byref(r), 256, None, 256, 9, None) == _lib.ERR_INVALID
+    assert lib.qws_loss_grad(None, 256, None, 256, 10, 0, None) == _lib.ERR_INVALID
+    assert lib.qws_loss_grad(C.byref(r), None, None, 256, 10, 0, None) == _lib.ERR_INVALID
+    assert lib.qws_loss_grad(C.byref(r), 256, None, None, 10, 0, None) == _lib.ERR_INVALID
+    assert lib.qws_loss_grad(C.byref(r), 256, None, 256, 9, 0, None) == _lib.ERR_INVALID
     r = rows(R=0)
-    assert lib.qws_loss_grad(C.byref(r), 256, None, None, 0, None) == _lib.OK
+    assert lib.qws_loss_grad(C.byref(r), 256, None, None, 0, 0, None) == _lib.OK
 
 
 def test_python_refusals():
