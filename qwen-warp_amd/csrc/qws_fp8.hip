@@ -17,6 +17,7 @@
 // rows; the hidden states of a workgroup) lie together for each 64 values of K, so that a workgroup copies runs of several
 // KB.  The exponents (biased by 127) of four consecutive blocks are the bytes of one word per row, a tile's words together.
 // Rows and values beyond N, T and K are 0.
+#include "qws_lds.h"
 #include "qws_lse.h"
 
 #include <type_traits>
@@ -398,26 +399,6 @@ __global__ void __launch_bounds__(256, RAW ? 4 : 1) k_f8_few(F8Args a) {
   }
 }
 
-typedef __attribute__((address_space(3))) void f8_lds;
-// 1 KB of consecutive bytes of memory into LDS, 16 bytes a lane, past the registers; OFFSET (below 4 KB) moves both places.
-// The instruction is written out because the compiler, where it knows of such a copy, waits for all of them before a read of
-// LDS; what has arrived is f8_meet's to say.
-template <int OFFSET>
-__device__ __forceinline__ void f8_copy(const char* from, uint32_t lane_offset, const void* to) {
-  const uint32_t at = (uint32_t)(uintptr_t)(f8_lds*)to;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(at), "v"(lane_offset), "s"(from), "n"(OFFSET) : "memory", "m0");
-}
-__device__ __forceinline__ void f8_copy_words(const char* from, uint32_t lane_offset, const void* to) {  // 64 words
-  const uint32_t at = (uint32_t)(uintptr_t)(f8_lds*)to;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(at), "v"(lane_offset), "s"(from) : "memory", "m0");
-}
-// Waits until at most N of the wave's newest loads are in flight and its LDS reads are done, then for the workgroup.  One
-// statement that no memory access moves across.
-template <int N>
-__device__ __forceinline__ void f8_meet() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
-
 // Many hidden states: the products bound it, below some 200 the weights' bytes.  A tile is WN x WT = 4 waves of 16 FN weight
 // rows x 16 FT hidden states: 2 x 2, one wave to a SIMD, so that each has the registers for up to 128 x 128 sums and an operand
 // read from LDS serves eight products; for up to 64 hidden states 4 x 1, so that only one wave widens a weight (widening and
@@ -467,11 +448,11 @@ __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int t
     constexpr int d = decltype(D)::value, xd = d - GN / 4;
     k = min(k, stages - 1);  // past the end: the last stage again, into a buffer that is not read any more
     if constexpr (d < GN / 4)
-      f8_copy<d * 1024>(pw + (size_t)k * (F8_ROWS / 16 * F8_FRAG), o16, b.w + GN / 4 * wave * 64);
+      lds_copy<d * 1024>(pw + (size_t)k * (F8_ROWS / 16 * F8_FRAG), o16, b.w + GN / 4 * wave * 64);
     else if constexpr (d < NEW - 1)
-      f8_copy<xd % 4 * 1024>(px + (size_t)k * (2 * WT * FT * 1024) + xd / 4 * 4096, o16, b.x + (XW * wave + xd / 4 * 4) * 64);
+      lds_copy<xd % 4 * 1024>(px + (size_t)k * (2 * WT * FT * 1024) + xd / 4 * 4096, o16, b.x + (XW * wave + xd / 4 * 4) * 64);
     else if constexpr (d == NEW - 1)
-      f8_copy_words(pe + (size_t)(k / 8) * (4 * F8_ROWS), o4, b.e + 64 * wave);
+      lds_copy_words(pe + (size_t)(k / 8) * (4 * F8_ROWS), o4, b.e + 64 * wave);
   };
   auto each = [&](auto f) {  // f(0) .. f(FN - 1), as constants
     [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>()), ...); }(std::make_integer_sequence<int, FN>());
@@ -510,7 +491,7 @@ __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int t
       q = qn;
       __builtin_amdgcn_sched_barrier(0);
     });
-    f8_meet<NEW>();
+    lds_meet<NEW>();
     each([&](auto I) {
       constexpr int i = decltype(I)::value;
       f8_b8 qn;
@@ -537,7 +518,7 @@ __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int t
   for (;;) {
     const int tn = row_tile(id), n0 = tn * BN, t0 = (id >> 3) % tiles_t * BT;
     each([&](auto I) { copy_first(2, b2, I); });  // the others follow in the first half
-    f8_meet<NEW + (FN * CP < NEW ? FN * CP : NEW)>();
+    lds_meet<NEW + (FN * CP < NEW ? FN * CP : NEW)>();
 #pragma unroll
     for (int i = 0; i < FN; i++) read_w(b0, i);
 #pragma unroll
@@ -552,7 +533,7 @@ __global__ void __launch_bounds__(256, 1) k_f8_tile(F8Args a, int tiles_n, int t
       if (k + 1 < stages) stage(k + 1, b1, b2, b0);
       if (k + 2 < stages) stage(k + 2, b2, b0, b1);
     }
-    f8_meet<0>();  // the copies past the end
+    lds_meet<0>();  // the copies past the end
     do id += gridDim.x;
     while (id < total && row_tile(id) >= tiles_n);
     if (id < total) {
