@@ -369,11 +369,24 @@ __device__ __forceinline__ void ls_total(const LsArgs& a, double s, int k, int p
 // One workgroup: the loss of n terms
 template <bool POLICY>
 __global__ void __launch_bounds__(LS_ONE) k_ls_sum(LsArgs a, int n) {
+  constexpr int U = 8;  // loaded together
   double s = 0.0;
   int k = 0;
-  for (int i = threadIdx.x; i < n; i += LS_ONE) {
-    s += a.term[i];
-    if (POLICY) k += ls_token(a, i) >= 0;
+  for (int i = threadIdx.x; i < n; i += LS_ONE * U) {
+    double v[U];
+    int t[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int at = min(i + LS_ONE * u, n - 1);
+      v[u] = a.term[at];
+      t[u] = POLICY ? ls_token(a, at) : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (i + LS_ONE * u < n) {
+        s += v[u];
+        if (POLICY) k += t[u] >= 0;
+      }
   }
   ls_total(a, s, k, POLICY ? 0 : n);
 }
@@ -644,8 +657,15 @@ __global__ void __launch_bounds__(NT) k_ls_policy(LsArgs a) {
 // One workgroup: without weights, the scale of the slopes is known before them: 1 over the rows with a token
 __global__ void __launch_bounds__(LS_ONE) k_ls_count(LsArgs a) {
   __shared__ int s_count[LS_ONE / 64];
+  constexpr int U = 8;  // loaded together
   int k = 0;
-  for (int i = threadIdx.x; i < a.R; i += LS_ONE) k += ls_token(a, i) >= 0;
+  for (int i = threadIdx.x; i < a.R; i += LS_ONE * U) {
+    int t[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) t[u] = ls_token(a, min(i + LS_ONE * u, a.R - 1));
+#pragma unroll
+    for (int u = 0; u < U; u++) k += i + LS_ONE * u < a.R && t[u] >= 0;
+  }
   k = wave_sum<int>(k);
   if (lane_id() == 0) s_count[wave_id()] = k;
   bar();

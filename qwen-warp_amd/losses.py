@@ -127,8 +127,8 @@ class _Base:
         """call(grad), with autograd where the logits ask for it."""
         if not (logits.requires_grad and torch.is_grad_enabled()):
             return call(None)[0]
-        if logits.is_leaf and torch.cuda.is_current_stream_capturing():
-            raise ValidationError("inside a captured graph the gradient of a leaf is value_and_grad's", "logits")
+        if torch.cuda.is_current_stream_capturing():  # a backward pass there ends the process where an eager graph of the same leaves lives
+            raise ValidationError("inside a captured graph the gradient is value_and_grad's", "logits")
         return _Loss.apply(logits, self, call, ahead)
 
 

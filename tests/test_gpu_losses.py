@@ -30,7 +30,7 @@ def close(got, want, tol, what):
     tol = np.broadcast_to(tol, want.shape)
     fine = np.isfinite(want)
     assert got.shape == want.shape and (np.isnan(got) == np.isnan(want)).all() and (got[~fine & ~np.isnan(want)] == want[~fine & ~np.isnan(want)]).all(), what
-    off = np.abs(got - want)[fine]
+    off = np.abs(got[fine] - want[fine])
     assert (off <= tol[fine]).all(), f"{what}: off by {off.max()}, {(off / np.maximum(tol[fine], 1e-300)).max()} of the bound"
 
 
@@ -430,7 +430,7 @@ def test_calls_repeat_and_streams():
 
 
 def test_graphs():
-    """Captured calls replay on new inputs, two graphs between each other and eager calls; a leaf's autograd is refused in one."""
+    """Captured calls replay on new inputs, two graphs between each other and eager calls; autograd is refused in one."""
     R, V = 12, 5000
     logits, x, tokens = logits_of(R, V, torch.float32, 11)
     _, old, adv, _, _ = policy_inputs(x, tokens, 11, False)
@@ -446,10 +446,10 @@ def test_graphs():
         oa, ga = fn.value_and_grad(logits, *args)
     with torch.cuda.graph(b):
         ob, gb = pl.value_and_grad(logits, args[0], starts)
-    c = torch.cuda.CUDAGraph()
-    with pytest.raises(q.ValidationError):
-        with torch.cuda.graph(c):
-            fn(eager_leaf, *args)
+    for refused in (lambda: fn(eager_leaf, *args), lambda: pl(eager_leaf * 1.0, args[0], starts)):
+        with pytest.raises(q.ValidationError):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                refused()
     for seed in range(20, 24):
         logits.copy_(logits_of(R, V, torch.float32, seed)[0])
         a.replay()

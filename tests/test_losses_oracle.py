@@ -68,13 +68,13 @@ def test_against_autograd():
     loss = -torch.minimum(r * a, r.clamp(0.8, 1.2) * a).mean()
     loss.backward()
     got = O.policy(x, tokens, old, adv)
-    assert abs(got["loss"] - float(loss)) < 1e-12 and np.abs(got["grad"] - t.grad.numpy()).max() < 1e-12
+    assert abs(got["loss"] - float(loss.detach())) < 1e-12 and np.abs(got["grad"] - t.grad.numpy()).max() < 1e-12
     t.grad = None
     s = torch.log_softmax(t, 1).gather(1, torch.tensor(tokens).view(-1, 1))[:, 0]
     loss = -torch.nn.functional.logsigmoid(0.1 * (s[:3].sum() - s[3:].sum()))
     loss.backward()
     got = O.preference(x, tokens, [0, 3, 7])
-    assert abs(got["loss"] - float(loss)) < 1e-12 and np.abs(got["grad"] - t.grad.numpy()).max() < 1e-12
+    assert abs(got["loss"] - float(loss.detach())) < 1e-12 and np.abs(got["grad"] - t.grad.numpy()).max() < 1e-12
 
 
 def test_rows_left_out():
