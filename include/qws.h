@@ -383,9 +383,10 @@ int qws_fp8_score(const void* packed, int N, int K, const void* x, long long x_s
  * codes q in 0 .. 15 with a scale s and a zero point z for each group of 32, 64 or 128 (the last may be shorter):
  *   y[t][n] = sum over groups of s * (sum_k q x - z * sum_k x), in fp32, the products exact.
  *   qws_int4_pack:       w [N][K] (dtype QWS_DTYPE_*, rows row_stride elements apart) -> packed (device, qws_int4_pack_bytes(N, K,
- *                        group) bytes, 256-byte aligned).  Per group lo = min(0, least), hi = max(0, largest), s = (hi - lo) / 15
- *                        rounded to bf16, z = -lo / s and q = w / s + z, quotients rounded to the nearest (ties to even), both held
- *                        in 0 .. 15.  A group with a value that is not finite makes its row's products NaN.
+ *                        group) bytes, 256-byte aligned).  Per group lo = min(0, least), hi = max(0, largest), s = (hi - lo) times
+ *                        the fp32 number nearest 1/15, in fp32, rounded to bf16; z = -lo / s and q = w / s + z, quotients rounded to
+ *                        the nearest (ties to even), both held in 0 .. 15.  A group with a value that is not finite, or whose
+ *                        hi - lo is not, makes its row's products NaN.
  *   qws_int4_pack_codes: codes [N][K], one in the low four bits of a byte, rows code_stride apart; scales [N][ceil(K / group)] bf16
  *                        (or fp16) rows scale_stride apart; zeros, like scales, in the low four bits, or NULL: 8.
  *   qws_int4_head:       x [T][K] bf16 (rows x_stride elements apart) -> out [T][N] (fp32 or bf16, rows out_stride >= N apart).

@@ -1,9 +1,9 @@
 """CPU definition of the 4-bit head (TEST INFRASTRUCTURE ONLY: see oracle/__init__.py), in 64 bits.
 
 A group of consecutive values of a row (the last may be shorter) is s (q - z): lo = min(0, least), hi = max(0, largest),
-s = (hi - lo) / 15 in fp32, rounded to bf16 (ties to even); z = -lo / s and q = value / s + z, quotients rounded to the nearest whole
-number (ties to even), both held in 0 .. 15.  A group with s = 0 is 0; one with a value that is not finite, or whose range over 15
-passes bf16's largest, is NaN."""
+s = (hi - lo) times the fp32 number nearest 1/15, both steps in fp32, rounded to bf16 (ties to even); z = -lo / s and q = value / s + z,
+quotients rounded to the nearest whole number (ties to even), both held in 0 .. 15.  A group with s = 0 is 0; one with a value
+that is not finite, or whose range hi - lo is not, is NaN."""
 import numpy as np
 
 
@@ -22,7 +22,7 @@ def quantise(w, group):
     b = np.where(bad[:, :, None], np.float32(0), b)
     lo, hi = np.minimum(b.min(2), 0), np.maximum(b.max(2), 0)
     with np.errstate(over="ignore"):
-        s = ((hi - lo) / np.float32(15)).astype(np.float32)
+        s = ((hi - lo) * np.float32(1 / 15)).astype(np.float32)
     bad |= ~np.isfinite(s)
     s = round_bf16(np.where(bad, np.float32(0), s))
     bad |= ~np.isfinite(s)

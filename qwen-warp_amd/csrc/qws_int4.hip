@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(256) k_i4_pack(I4Pack a) {
         hi = fmaxf(hi, __shfl_xor(hi, i));
         bad = __shfl_xor((int)bad, i) || bad;
       }
-      const float range = (hi - lo) / 15.0f;
+      const float range = (hi - lo) * (1.0f / 15.0f);
       bad = bad || !(range <= F32_MAX);
       const uint32_t s = bad ? 0 : i4_nearest_bf16(range);
       bad = bad || s >= 0x7F80u;
