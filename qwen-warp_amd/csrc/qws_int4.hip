@@ -229,16 +229,16 @@ __device__ __forceinline__ void i4_put(O* p, float y) {
     *p = v;
 }
 
-// A workgroup takes 64 weight rows and 16 TF hidden states, its 4 waves a quarter of K each; their sums meet in LDS.
-template <typename O, int GROUP, int TF>
-__global__ void __launch_bounds__(256, TF > 2 ? 2 : 4) k_i4_few(I4Args a) {
+// A workgroup takes 64 weight rows and 16 TF hidden states, its NW waves a part of K each; their sums meet in LDS.
+template <typename O, int GROUP, int TF, int NW>
+__global__ void __launch_bounds__(64 * NW, TF > 2 ? 2 : 4) k_i4_few(I4Args a) {
   constexpr int G = I4_ROWS / 16, C = I4_KB / GROUP, J = GROUP / 32;  // fragments, groups of a block, products of a group
-  __shared__ vf4 s_acc[4][G * TF][64];
+  __shared__ vf4 s_acc[NW][G * TF][64];
   const int lane = lane_id(), wave = wave_id(), quad = lane >> 4;
   // XCD x (workgroups x, x + 8, ..) takes the tiles of weight rows x, x + 8, .., all of their hidden states in a row
   const int tile = (blockIdx.x >> 3) / a.tiles_t * 8 + (blockIdx.x & 7), t0 = (blockIdx.x >> 3) % a.tiles_t * 16 * TF;
   if (tile >= a.l.tiles) return;
-  const int kb = a.l.kb, per = (kb + 3) / 4, lo = wave * per, hi = min(lo + per, kb);
+  const int kb = a.l.kb, per = (kb + NW - 1) / NW, lo = wave * per, hi = min(lo + per, kb);
   const char* pw = a.w + (size_t)tile * kb * (I4_ROWS * I4_KB / 2) + 16 * lane;
   const uint32_t* ps = (const uint32_t*)(a.w + a.l.scales) + (size_t)tile * a.l.kg * I4_ROWS + (lane & 15);
   const uint16_t* px[TF];
@@ -309,9 +309,11 @@ __global__ void __launch_bounds__(256, TF > 2 ? 2 : 4) k_i4_few(I4Args a) {
     for (int j = 0; j < TF; j++) s_acc[wave][g * TF + j][lane] = acc[g][j];
   bar();
   const int n = tile * I4_ROWS + lane;  // a store is 64 consecutive rows of one hidden state
-  for (int t = wave; t < 16 * TF && t0 + t < a.T; t += 4) {
+  for (int t = wave; t < 16 * TF && t0 + t < a.T; t += NW) {
     const int i = (lane >> 4) * TF + (t >> 4), l = (t >> 2 & 3) * 16 + (lane & 15), r = t & 3;
-    const float y = (s_acc[0][i][l][r] + s_acc[1][i][l][r]) + (s_acc[2][i][l][r] + s_acc[3][i][l][r]);
+    float y = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; w += 4) y += (s_acc[w][i][l][r] + s_acc[w + 1][i][l][r]) + (s_acc[w + 2][i][l][r] + s_acc[w + 3][i][l][r]);
     if (n < a.N) i4_put<false>((O*)a.out + (long long)(t0 + t) * a.out_stride + n, y);
   }
 }
@@ -511,9 +513,13 @@ inline bool i4_group(int group) { return group == 32 || group == 64 || group == 
 inline bool i4_shape(int T, int N, int K, int group) { return T >= 1 && N >= 1 && K >= 1 && i4_group(group); }
 inline bool i4_fits(int T, int N, int K) { return N <= I4_NMAX && K <= I4_KMAX && T <= I4_TMAX; }
 inline bool i4_aligned(const void* p) { return p && ((uintptr_t)p & 255) == 0; }
+// Up to so many workgroups of k_i4_few each has eight waves, an eighth of K each, instead of four (K = 5,120, us, four / eight: N = 8,191, 1
+// state 14.6 / 9.4; N = 16,384 15.4 / 10.9; N = 24,000 17.0 / 15.5; N = 64,000 30.6 / 30.1; 30 states at N = 16,384, 512 workgroups, 18.4 / 19.7).
+constexpr int I4_SPARSE = 384;
 // What runs T hidden states against N weight rows: k_i4_tile or k_i4_few, with 16 tf of them to a workgroup: the least estimated time.  A
-// kernel's workgroups take `least` us for 40 blocks of K where each CU has one, and `each` for every one of them where it has several
-// (k_i4_few does not split T for up to 64); k_i4_tile's states are packed by a launch of 3 us.  Measured, us, k_i4_few / k_i4_tile:
+// kernel's workgroups take `least` us for 40 blocks of K where each CU has one, and `each` for every one of them where it has several,
+// between the mean and the largest number of them
+// (k_i4_few's for 16 states: with eight waves); k_i4_tile's states are packed by a launch of 3 us.  Measured, us, k_i4_few / k_i4_tile:
 // K = 5,120, N = 248,320: 1 state 107 / 118, 8 states 125 / 126, 12 139 / 129, 16 153 / 132, 36 272 / 163, 64 346 / 197, 200 1,260 / 620; N =
 // 64,000: 8 states 33 / 34, 16 40 / 35, 64 95 / 59; N = 32,001: 12 states 19 / 30, 40 44 / 38, 64 51 / 39; N = 16,384: 64 states 30 / 36.
 struct I4Plan {
@@ -525,15 +531,21 @@ inline I4Plan i4_plan(int T, int N, int K) {
   struct Cost {
     double least, each;
   };
-  constexpr Cost few[3] = {{16, 10}, {22, 12.5}, {28, 24}}, tile[4] = {{26, 31}, {32, 33}, {37, 37}, {43, 47}};
+  constexpr Cost few[3] = {{11, 10}, {22, 12.5}, {28, 24}}, tile[4] = {{26, 31}, {32, 33}, {37, 37}, {43, 47}};
   const double blocks = i4_up(K, I4_KB) / I4_KB / 40.0;
   auto time = [&](Cost c, int rows, int states) {
-    const double wgs = (double)(i4_up(N, rows) / rows) * (i4_up(T, states) / states), each = c.each * ceil(wgs / 256);
+    const double wgs = (double)(i4_up(N, rows) / rows) * (i4_up(T, states) / states) / 256, each = c.each * (wgs + ceil(wgs)) / 2;
     return blocks * (each > c.least ? each : c.least);
   };
-  const int few_tf = T <= 16 ? 1 : T <= 32 ? 2 : 4;
-  I4Plan p = {false, few_tf};
-  double best = time(few[few_tf / 2], I4_ROWS, 16 * few_tf);
+  I4Plan p = {false, 1};
+  double best = time(few[0], I4_ROWS, 16);
+  for (int tf = 2; tf <= 4; tf += tf) {
+    const double t = time(few[tf / 2], I4_ROWS, 16 * tf);
+    if (t < best) {
+      best = t;
+      p.tf = tf;
+    }
+  }
   for (int tf = 1; tf <= 4; tf++) {
     const double t = 3 + time(tile[tf - 1], 4 * I4_ROWS, 16 * tf);
     if (t < best) {
@@ -589,9 +601,14 @@ static int i4_run(I4Args a, char* ws, hipStream_t st) {
     a.K = width;
   }
   switch (tf) {
-    case 1: hipLaunchKernelGGL((k_i4_few<O, GROUP, 1>), grid, nt, 0, st, a); break;
-    case 2: hipLaunchKernelGGL((k_i4_few<O, GROUP, 2>), grid, nt, 0, st, a); break;
-    default: hipLaunchKernelGGL((k_i4_few<O, GROUP, 4>), grid, nt, 0, st, a); break;
+    case 1:
+      if (wgs <= I4_SPARSE)
+        hipLaunchKernelGGL((k_i4_few<O, GROUP, 1, 8>), grid, dim3(512), 0, st, a);
+      else
+        hipLaunchKernelGGL((k_i4_few<O, GROUP, 1, 4>), grid, nt, 0, st, a);
+      break;
+    case 2: hipLaunchKernelGGL((k_i4_few<O, GROUP, 2, 4>), grid, nt, 0, st, a); break;
+    default: hipLaunchKernelGGL((k_i4_few<O, GROUP, 4, 4>), grid, nt, 0, st, a); break;
   }
   return (int)hipGetLastError();
 }

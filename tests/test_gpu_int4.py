@@ -10,6 +10,7 @@ import torch
 
 import qwen_warp_amd as q
 from oracle import int4 as I
+from qwen_warp_amd import _lib
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -112,6 +113,34 @@ def test_large_head(T):
     want, tol = product(x, codes.numpy(), scales.double().numpy(), z.numpy(), group)
     got = q.Int4Head.from_codes(codes.cuda(), scales.cuda(), z.cuda(), group=group)(x.cuda()).double().cpu().numpy()
     assert (np.abs(got - want) <= tol).all()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("T,frags", [(5, 0), (12, 1), (16, 1), (25, 2), (41, 3), (64, 4), (100, 4), (70, 3)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tiles(T, frags, group, dtype):
+    """Heads of many rows, 16 frags states a tile (0: the rows' own kernel): an odd number of blocks of K, the last tile partly
+    past N; the reference by torch in 64 bits on the GPU.  bf16 logits are the fp32 ones rounded."""
+    N, K, kb = 50001, 2600, 21
+    head_bytes = _lib.load().qws_int4_head_ws_bytes(T, N, K, group)
+    assert head_bytes == (-(-T // (16 * frags)) * (kb + 1) * (4 * frags + 1) * 1024 if frags else (T * kb * 256 + 255) // 256 * 256)
+    g = torch.Generator("cuda").manual_seed(T)
+    codes = torch.randint(0, 16, (N, K), generator=g, dtype=torch.uint8, device="cuda")
+    shape = (N, -(-K // group))
+    scales = (0.001 + 0.01 * torch.rand(shape, generator=g, device="cuda")).to(torch.bfloat16)
+    z = torch.randint(0, 16, shape, generator=g, dtype=torch.uint8, device="cuda")
+    x = states(T, K, T).cuda()
+    head = q.Int4Head.from_codes(codes, scales, z, group=group)
+    got = head(x)
+    spread = lambda t: t.double().repeat_interleave(group, 1)[:, :K]  # noqa: E731
+    want = x.double() @ (spread(scales) * (codes.double() - spread(z))).t()
+    size = x.double().abs() @ (spread(scales) * (32 + codes.double() + spread(z))).t()
+    assert ((got.double() - want).abs() <= (group + K / group + 8) * 2.0 ** -23 * size).all()
+    if dtype == torch.bfloat16:
+        assert torch.equal(head(x, dtype=dtype).view(torch.int16), got.to(dtype).view(torch.int16))
+        buf = torch.full((T, N + 9), 7.0, dtype=dtype, device="cuda")
+        head(x, out=buf[:, 5:5 + N])
+        assert torch.equal(buf[:, 5:5 + N], got.to(dtype)) and (buf[:, :5] == 7).all() and (buf[:, 5 + N:] == 7).all()
 
 
 def test_rows_do_not_depend_on_the_batch():
