@@ -6,12 +6,21 @@
 // one number a row beside what the softmax needs.  A row's maximum m and sum s come from one pass over its logits, the loss and
 // dL/dlog p from a few numbers a row (in 64 bits: they are differences of log probabilities), the gradient from a second pass.
 //
-//   k_ls_scan        R x G workgroups: each lane's running maximum and sum
-//   k_ls_policy_rows a wave per row: joins the row's parts, log p, the row's term and slope
-//   k_ls_rows        the same for the preference loss: log p and the row's sequence
+// The policy loss's slope depends on its row alone, so one workgroup does a row from the first pass to the second and keeps what
+// fits of it in between (k_ls_policy): the logits are read once, the gradient written once.  The preference loss's depends on every
+// row of a pair, so between its passes lies a launch and, past the caches, the logits are read twice.
+//
+//   k_ls_policy      a workgroup per row: the policy loss with its gradient.  Bound by the bytes: 2,048 bf16 rows of 248,320 391 us, 5.2
+//                    TB/s of 2.03 GB, which is what was read and written (a large copy makes 4.97); 512 fp32 rows 210 us, 1.24 GB with
+//                    what a row's workgroup cannot keep, read twice; a few short rows by one row's latency, 13 us for 32,001 logits.
+//   k_ls_scan        R x G workgroups: each lane's running maximum and sum.  Bound by the bytes: 256 fp32 rows 44 us, 5.8 TB/s; 1,200 bf16
+//                    rows 99 us, 5.6 TB/s of those with a token.
+//   k_ls_policy_rows a wave per row: joins the row's parts, log p, the row's term and slope (5.4 us up to 512 rows: latency)
+//   k_ls_rows        the same for the preference loss: log p and the row's sequence (5-6 us)
 //   k_ls_pairs       a wave per pair: the sequences' sums, the pair's term, the two slopes
-//   k_ls_sum         the loss: the sum of the terms
-//   k_ls_grad        R x G workgroups: the gradient's rows
+//   k_ls_sum         the loss: the sum of the terms (4-5 us); k_ls_few: pairs, and a few rows, in the same launch (5-10 us)
+//   k_ls_grad        R x G workgroups: the gradient's rows.  Bound by the bytes: 1,200 bf16 rows 193 us, 5.9 TB/s; where it finds the
+//                    gradient written 4.5 us.
 #include "qws_logits.h"
 
 namespace qws {
@@ -765,11 +774,13 @@ static void ls_policy_rows(const LsArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((k_ls_policy<T, NT, NV, NL>), dim3(a.R), dim3(NT), NL * NT * 16, st, a);
 }
 // The least workgroup that holds a row: 2,048 bf16 rows, us with 256 x 16 / 512 x 24 / 1,024 x 24 vectors: of 16,000 logits 33 / 42 / 64,
-// of 32,001 65 / 72 / 95, of 40,000 82 / 81 / 101, of 100,000 221 / 181 / 188, of 130,000 308 / 239 / 244, of 200,000 439 / 376 / 347.
+// of 32,001 65 / 72 / 95, of 40,000 82 / 81 / 101, of 100,000 221 / 181 / 188, of 130,000 308 / 239 / 244, of 200,000 439 / 376 / 347.  Where
+// there are at most two rows to a CU the larger one is quicker from some 2,000 vectors on: 32,001 bf16 logits, 24 rows 16.2 / 12.9, 400
+// rows 21.0 / 18.1; 16,000 bf16 logits, 100 rows 11.3 / 10.4; 8,000, 4 rows 8.9 / 9.1.
 template <typename T>
 static void ls_policy_one_pass(const LsArgs& a, hipStream_t st) {
   const int n = a.V / lp_e<T>();
-  if (n <= 256 * 16)
+  if (n <= 2048 || (n <= 4096 && a.R > 512))
     ls_policy_rows<T, 256, 16, 0>(a, st);
   else if (n <= LS_HELD)
     ls_policy_rows<T, 512, 16, 8>(a, st);
