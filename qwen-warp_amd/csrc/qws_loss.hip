@@ -11,7 +11,7 @@
 // row of a pair, so between its passes lies a launch and, past the caches, the logits are read twice.
 //
 //   k_ls_policy      a workgroup per row: the policy loss with its gradient.  Bound by the bytes: 2,048 bf16 rows of 248,320 391 us, 5.2
-//                    TB/s of 2.03 GB, which is what was read and written (a large copy makes 4.97); 512 fp32 rows 210 us, 1.24 GB with
+//                    TB/s of 2.03 GB, which is what was read and written (a large copy makes 4.97); 512 fp32 rows 210 us, 1.26 GB with
 //                    what a row's workgroup cannot keep, read twice; a few short rows by one row's latency, 13 us for 32,001 logits.
 //   k_ls_scan        R x G workgroups: each lane's running maximum and sum.  Bound by the bytes: 256 fp32 rows 44 us, 5.8 TB/s; 1,200 bf16
 //                    rows 99 us, 5.6 TB/s of those with a token.
