@@ -12,7 +12,7 @@
 // .. + 7, the second operand of the 16x16x32 product j; value 2 i and 2 i + 1 of a word are bits 4 i .. and 4 i + 16 .., so that one
 // mask takes a pair into the halves of a register.  Four fragments (64 rows) lie together for each 128 values of K, 4 KB that one
 // wave reads at once.  A scale is a word: fp32 (from bf16 or fp16: the low 13 bits are 0) with 16 + z in its low byte; the 64 words of a
-// tile's rows lie together for each group.  Rows and values beyond N and K have scale 0.
+// tile's rows lie together for each group.  Values beyond K are 0, rows beyond N not used.
 #include "qws_lds.h"
 #include "qws_lse.h"
 
