@@ -35,8 +35,10 @@ def blocks_of(x: torch.Tensor, name: str):
     shape, strides = x.shape, x.stride()
     if len(shape) < 2 or (shape[-1] > 1 and strides[-1] != 1):
         raise ValidationError(f"{name} must be [..., n] with contiguous rows", name)
-    if max(shape) > INT_MAX or math.prod(shape[:-1]) > INT_MAX:
+    if max(shape) > INT_MAX or (len(shape) > 2 and math.prod(shape[:-1]) > INT_MAX):
         raise ValidationError(f"{name}: at most 2^31 - 1 rows of as many elements", name)
+    if len(shape) == 2:
+        return shape[0], 0, strides[0] if shape[0] > 1 else 0, 0
     levels = []  # (rows, stride), innermost first
     for size, step in zip(reversed(shape[:-1]), reversed(strides[:-1])):
         if size == 1:
@@ -78,9 +80,9 @@ class _Loss(torch.autograd.Function):
             written = grad is not None
             if not written:
                 grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            upstream = upstream.contiguous()
-            check(ctx.owner.lib.qws_loss_grad(C.byref(ctx.rows), ctx.state.data_ptr(), upstream.data_ptr(), grad.data_ptr(), logits.shape[-1], written, stream),
-                  "qws_loss_grad")
+            err = ctx.owner.lib.qws_loss_grad(C.byref(ctx.rows), ctx.state.data_ptr(), upstream.data_ptr(), grad.data_ptr(), ctx.rows.V, written, stream)
+            if err:
+                check(err, "qws_loss_grad")
         return grad, None, None, None
 
 
@@ -102,25 +104,25 @@ class _Base:
             raise ValidationError("logits must have a value a row", "logits")
         lead = logits.shape[:-1]
         given(tokens, lead, torch.int32, dev, "tokens")
-        if temperature is not None:
-            self._number(temperature, lead, dev, "temperature")
         return _lib.LossRows(logits.data_ptr(), _lib.DTYPE_F32 if dtype == torch.float32 else _lib.DTYPE_BF16, R, logits.shape[-1], block, stride, block_stride,
-                             tokens.data_ptr(), temperature.data_ptr() if temperature is not None else None)
+                             tokens.data_ptr(), self._number(temperature, lead, dev, "temperature") if temperature is not None else None)
 
     @staticmethod
     def _number(t, shape, dev, name):
         if t is None:
             raise ValidationError(f"{name} is needed", name)
-        given(t, shape, torch.float32, dev, name)
+        if t.dtype != torch.float32 or t.device != dev or t.shape != shape or not t.is_contiguous():
+            given(t, shape, torch.float32, dev, name)
         if t.requires_grad:
             raise ValidationError(f"{name} is taken as a constant: detach it", name)
+        return t.data_ptr()
 
     def _state(self, query, *key):
         n = self._bytes.get(key)
-        if n is None:
+        if not n:
             n = self._bytes[key] = query(*key)
-        if n == 0:
-            raise ValidationError("logits: fewer than 2^24 rows of at most 2^24 values", "logits")
+            if n == 0:
+                raise ValidationError("logits: fewer than 2^24 rows of at most 2^24 values", "logits")
         return n
 
     def _forward(self, logits, call, ahead=False):
@@ -172,25 +174,24 @@ class PolicyLoss(_Base):
 
     def _prepare(self, logits, tokens, old, adv, ref, weights, temperature):
         rows = self._rows(logits, tokens, temperature)
-        lead, dev = logits.shape[:-1], logits.device
-        for t, name in ((old, "old_logprobs"), (adv, "advantages"), (ref, "ref_logprobs"), (weights, "weights")):
-            if t is not None or name in ("old_logprobs", "advantages"):
-                self._number(t, lead, dev, name)
+        lead, dev, number = logits.shape[:-1], logits.device, self._number
+        inputs = (number(old, lead, dev, "old_logprobs"), number(adv, lead, dev, "advantages"), number(ref, lead, dev, "ref_logprobs") if ref is not None else None,
+                  number(weights, lead, dev, "weights") if weights is not None else None)
         n = self._state(self.lib.qws_policy_state_bytes, rows.dtype, rows.R, rows.V)
         where, stream = on_stream(dev.index)
         with where:
             lp = torch.empty(lead, dtype=torch.float32, device=dev)
             ratio = torch.empty_like(lp)
             kl = torch.empty_like(lp) if ref is not None else None
-        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
 
         def call(grad):
             with where:
-                loss = torch.empty((), dtype=torch.float32, device=dev)
+                loss = lp.new_empty(())
                 state = torch.empty(n, dtype=torch.uint8, device=dev)
-                b = _lib.PolicyBatch(rows, old.data_ptr(), adv.data_ptr(), ptr(ref), ptr(weights), *self.clip, self.kl, loss.data_ptr(), lp.data_ptr(),
-                                     ratio.data_ptr(), ptr(kl))
-                check(self.lib.qws_policy_loss(C.byref(b), state.data_ptr(), n, ptr(grad), rows.V, stream), "qws_policy_loss")
+                b = _lib.PolicyBatch(rows, *inputs, *self.clip, self.kl, loss.data_ptr(), lp.data_ptr(), ratio.data_ptr(), kl.data_ptr() if kl is not None else None)
+                err = self.lib.qws_policy_loss(C.byref(b), state.data_ptr(), n, grad.data_ptr() if grad is not None else None, rows.V, stream)
+                if err:
+                    check(err, "qws_policy_loss")
             return loss, rows, state, tokens
 
         return call, (lp, ratio, kl)
@@ -243,26 +244,24 @@ class PreferenceLoss(_Base):
                 raise ValidationError("starts must be [2 P + 1]", "starts")
             given(starts, starts.shape, torch.int32, dev, "starts")
             P = starts.numel() // 2
-        for t, size, name in ((ref, 2 * P, "ref"), (weights, P, "weights")):
-            if t is not None:
-                self._number(t, (size,), dev, name)
+        inputs = (self._number(ref, (2 * P,), dev, "ref") if ref is not None else None, self._number(weights, (P,), dev, "weights") if weights is not None else None)
         n = self._state(self.lib.qws_preference_state_bytes, rows.dtype, rows.R, rows.V, P)
         where, stream = on_stream(dev.index)
         with where:
             if starts is None:
                 starts = torch.arange(0, 2 * P + 1, dtype=torch.int32, device=dev).mul_(lead[1])
-            sums = torch.empty(2 * P, dtype=torch.float32, device=dev)
-            margins = torch.empty(P, dtype=torch.float32, device=dev)
             lp = torch.empty(lead, dtype=torch.float32, device=dev)
-        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+            sums, margins = lp.new_empty(2 * P), lp.new_empty(P)
 
         def call(grad):
             with where:
-                loss = torch.empty((), dtype=torch.float32, device=dev)
+                loss = lp.new_empty(())
                 state = torch.empty(n, dtype=torch.uint8, device=dev)
-                b = _lib.PreferenceBatch(rows, starts.data_ptr(), P, int(self.average), ptr(ref), ptr(weights), self.beta, self.margin, self.smoothing,
-                                         loss.data_ptr(), sums.data_ptr(), margins.data_ptr(), lp.data_ptr())
-                check(self.lib.qws_preference_loss(C.byref(b), state.data_ptr(), n, ptr(grad), rows.V, stream), "qws_preference_loss")
+                b = _lib.PreferenceBatch(rows, starts.data_ptr(), P, self.average, *inputs, self.beta, self.margin, self.smoothing, loss.data_ptr(), sums.data_ptr(),
+                                         margins.data_ptr(), lp.data_ptr())
+                err = self.lib.qws_preference_loss(C.byref(b), state.data_ptr(), n, grad.data_ptr() if grad is not None else None, rows.V, stream)
+                if err:
+                    check(err, "qws_preference_loss")
             return loss, rows, state, tokens
 
         return call, (sums, margins, lp)

@@ -154,6 +154,23 @@ def test_rows_do_not_depend_on_the_batch():
         assert torch.equal(got, head(x[:T]))
 
 
+@pytest.mark.parametrize("T,N,K,group", [(1, 1 << 24, 32, 32), (2, 70, 1 << 20, 128), (3000, 200, 96, 64), (40, 300, 70001, 32)])
+def test_largest_sizes(T, N, K, group):
+    """The limits of N and K, many hidden states of a small head, a long K for tiles; the reference by torch in 64 bits on the GPU."""
+    g = torch.Generator("cuda").manual_seed(T)
+    codes = torch.randint(0, 16, (N, K), generator=g, dtype=torch.uint8, device="cuda")
+    scales = (0.001 + 0.01 * torch.rand((N, -(-K // group)), generator=g, device="cuda")).to(torch.bfloat16)
+    x = states(T, K, 3).cuda()
+    got = q.Int4Head.from_codes(codes, scales, group=group)(x)
+    for rows in (slice(0, 1 << 13), slice(max(0, N - (1 << 13)), N)):
+        s = scales[rows].double().repeat_interleave(group, 1)[:, :K]
+        want = x.double() @ (s * (codes[rows].double() - 8)).t()
+        size = x.double().abs() @ (s * (40 + codes[rows].double())).t()
+        assert ((got[:, rows].double() - want).abs() <= (group + K / group + 8) * 2.0 ** -23 * size).all()
+    with pytest.raises(q.ValidationError):
+        q.Int4Head(torch.empty(1, 1, device="cuda").expand(1, (1 << 20) + 1))
+
+
 def test_special_values():
     """Zeros give zeros; a row with NaN or an infinity is NaN, the others are not touched by it."""
     w, x = weights(500, 300, 6), states(20, 300, 7)

@@ -413,6 +413,29 @@ def test_offsets_past_32_bits():
     assert torch.allclose(g[-20:].float(), gw.float(), rtol=2.0 ** -7, atol=1e-9)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R", [2, 140])
+def test_longest_rows(dtype, R):
+    """V at its limit, and a value past it refused; the log probabilities against torch's in 64 bits."""
+    V = 1 << 24 if R == 2 else 1 << 21
+    x = torch.randn(R, V, device="cuda", generator=torch.Generator("cuda").manual_seed(R)).mul_(2).to(dtype)
+    tokens = torch.arange(R, device="cuda", dtype=torch.int32) * 7 + V - 2000
+    old, adv = torch.full((R,), -14.0, device="cuda"), torch.ones(R, device="cuda")
+    fn = q.PolicyLoss("cuda", clip=(1.0, 1e6))
+    out, g = fn.value_and_grad(x, tokens, old, adv)
+    for r in (0, 1, R - 1):
+        lp = torch.log_softmax(x[r].double(), 0)
+        assert abs(float(out.logprobs[r]) - float(lp[int(tokens[r])])) <= delta(V) + U * 20
+        p, slope = lp.exp(), -float(out.ratio[r]) / R
+        want = -slope * p
+        want[int(tokens[r])] += slope
+        off = (g[r].double() - want).abs()
+        # |d| of any logit here: below 40 log2 units
+        assert (off <= (abs(slope) * p * (92 * U + 2 * delta(V)) + 8 * U * abs(slope) * (want.abs() == want.abs().max())) * (1 + HALF[dtype]) + HALF[dtype] * want.abs() + 1e-37).all()
+    with pytest.raises(q.ValidationError):
+        fn(torch.empty(1, 1, device="cuda").expand(1, (1 << 24) + 1).contiguous(), tokens[:1], old[:1], adv[:1])
+
+
 def test_calls_repeat_and_streams():
     logits, x, tokens = logits_of(40, 9001, torch.bfloat16, 10, pad=3)
     _, old, adv, ref, w = policy_inputs(x, tokens, 10, False)
