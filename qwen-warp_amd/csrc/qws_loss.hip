@@ -18,7 +18,7 @@
 //   k_ls_policy_rows a wave per row: joins the row's parts, log p, the row's term and slope (5.4 us up to 512 rows: latency)
 //   k_ls_rows        the same for the preference loss: log p and the row's sequence (5-6 us)
 //   k_ls_pairs       a wave per pair: the sequences' sums, the pair's term, the two slopes
-//   k_ls_sum         the loss: the sum of the terms (4-5 us); k_ls_few: pairs, and a few rows, in the same launch (5-10 us)
+//   k_ls_sum         the loss: the sum of the terms (4-5 us); k_ls_few, k_ls_policy_few: pairs and a few rows in the same launch (5-10 us)
 //   k_ls_grad        R x G workgroups: the gradient's rows.  Bound by the bytes: 1,200 bf16 rows 193 us, 5.9 TB/s; where it finds the
 //                    gradient written 4.5 us.
 #include "qws_logits.h"
@@ -263,14 +263,22 @@ __device__ __forceinline__ double ls_policy(const LsArgs& a, int row, int tok, L
   if (a.out_kl) a.out_kl[row] = (float)kl;
   return term;
 }
+// One wave: a row's parts joined, its term (lane 0's); k counts the rows with a token
+template <typename T>
+__device__ __forceinline__ double ls_policy_row(const LsArgs& a, int row, int& k) {
+  const int tok = ls_token(a, row);
+  const float temp = a.temp ? a.temp[row] : 1.0f, c = lse_scale(temp);
+  const LsSum v = tok < 0 ? LsSum{-INFINITY, 0.0f} : ls_parts(a, row, c);
+  k += tok >= 0;
+  return lane_id() == 0 ? ls_policy<T>(a, row, tok, v, c, temp) : 0.0;
+}
 template <typename T>
 __global__ void __launch_bounds__(LS_NT) k_ls_policy_rows(LsArgs a) {
   const int row = blockIdx.x * LS_NW + wave_id();
   if (row >= a.R) return;
-  const int tok = ls_token(a, row);
-  const float temp = a.temp ? a.temp[row] : 1.0f, c = lse_scale(temp);
-  const LsSum v = tok < 0 ? LsSum{-INFINITY, 0.0f} : ls_parts(a, row, c);
-  if (lane_id() == 0) a.term[row] = ls_policy<T>(a, row, tok, v, c, temp);
+  int k = 0;
+  const double term = ls_policy_row<T>(a, row, k);
+  if (lane_id() == 0) a.term[row] = term;
 }
 
 // ------------------------------------------------------------------------------------------------ the preference loss's rows and pairs
@@ -400,8 +408,9 @@ __global__ void __launch_bounds__(LS_ONE) k_ls_sum(LsArgs a, int n) {
   ls_total(a, s, k, POLICY ? 0 : n);
 }
 // One workgroup for a few pairs (and, with ROWS, a few rows): rows, pairs and the loss without launches between them, 3 us of the
-// host's time and as much of the card's each.
-constexpr int LS_FEW = 64;
+// host's time each.  Rows go to the waves in turn, which the card pays for from some number on: the policy loss of 16 rows of 248,320
+// without gradient 14.2 us in a graph in one launch behind the scan, 14.4 in two, of 40 rows 16.0 and 12.4, of 64 24.3 and 14.6.
+constexpr int LS_FEW = 64, LS_FEW_ROWS = 48, LS_FEW_POLICY = 16;  // pairs; rows of the preference loss; rows of the policy loss, whose exponentials in 64 bits take longer
 template <typename T, bool ROWS>
 __global__ void __launch_bounds__(LS_ONE) k_ls_few(LsArgs a) {
   if constexpr (ROWS) {
@@ -414,6 +423,18 @@ __global__ void __launch_bounds__(LS_ONE) k_ls_few(LsArgs a) {
     if (lane_id() == 0) s += term;
   }
   ls_total(a, s, 0, a.P);
+}
+
+// The same for a few rows of the policy loss
+template <typename T>
+__global__ void __launch_bounds__(LS_ONE) k_ls_policy_few(LsArgs a) {
+  double s = 0.0;
+  int k = 0;
+  for (int row = wave_id(); row < a.R; row += LS_ONE / 64) {
+    const double term = ls_policy_row<T>(a, row, k);
+    if (lane_id() == 0) s += term;
+  }
+  ls_total(a, s, lane_id() ? 0 : k, 0);
 }
 
 // ------------------------------------------------------------------------------------------------ the gradient's rows
@@ -789,13 +810,18 @@ static void ls_policy_one_pass(const LsArgs& a, hipStream_t st) {
 }
 template <typename T>
 static void ls_policy_run(const LsArgs& a, hipStream_t st) {
-  ls_scan<T>(a, st);
+  if (a.R) ls_scan<T>(a, st);
+  if (a.R <= LS_FEW_POLICY) {
+    hipLaunchKernelGGL((k_ls_policy_few<T>), dim3(1), dim3(LS_ONE), 0, st, a);
+    return;
+  }
   hipLaunchKernelGGL((k_ls_policy_rows<T>), dim3((a.R + LS_NW - 1) / LS_NW), dim3(LS_NT), 0, st, a);
+  hipLaunchKernelGGL((k_ls_sum<true>), dim3(1), dim3(LS_ONE), 0, st, a, a.R);
 }
 template <typename T>
 static void ls_preference_run(const LsArgs& a, hipStream_t st) {
   if (a.R) ls_scan<T>(a, st);
-  if (a.P <= LS_FEW && a.R <= LS_FEW) {
+  if (a.P <= LS_FEW && a.R <= LS_FEW_ROWS) {
     hipLaunchKernelGGL((k_ls_few<T, true>), dim3(1), dim3(LS_ONE), 0, st, a);
     return;
   }
@@ -855,8 +881,7 @@ extern "C" int qws_policy_loss(const qws_policy_batch* b, void* state, size_t st
     hipLaunchKernelGGL((k_ls_sum<true>), dim3(1), dim3(LS_ONE), 0, st, a, R);
     return (int)hipGetLastError();
   }
-  if (R) b->rows.dtype == QWS_DTYPE_F32 ? ls_policy_run<float>(a, st) : ls_policy_run<uint16_t>(a, st);
-  hipLaunchKernelGGL((k_ls_sum<true>), dim3(1), dim3(LS_ONE), 0, st, a, R);
+  b->rows.dtype == QWS_DTYPE_F32 ? ls_policy_run<float>(a, st) : ls_policy_run<uint16_t>(a, st);
   if (R && grad) {
     a.grad = grad;
     a.grad_stride = grad_stride;

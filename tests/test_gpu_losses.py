@@ -100,7 +100,7 @@ def policy_tolerances(want, adv, kl, ref, w, V):
     (1, 1, 0, False, 0.0, False, False), (1, 2, 1, True, 0.1, True, False), (3, 7, 0, False, 0.05, False, False), (5, 255, 3, True, 0.0, True, False),
     (17, 1000, 8, False, 0.1, True, True), (64, 4096, 0, True, 0.05, False, False), (9, 32001, 7, False, 0.05, True, True), (70, 3001, 1, True, 0.1, False, True),
     (3, 248320, 0, False, 0.05, True, False), (2, 100003, 5, True, 0.1, False, True), (700, 513, 2, False, 0.05, True, True), (2100, 64, 0, False, 0.0, False, False),
-    (130, 100003, 5, True, 0.1, False, True), (6, 65432, 0, False, 0.05, True, False), (600, 9001, 3, False, 0.0, True, False)])
+    (130, 100003, 5, True, 0.1, False, True), (20, 100003, 1, False, 0.05, False, True), (6, 65432, 0, False, 0.05, True, False), (600, 9001, 3, False, 0.0, True, False)])
 def test_policy(dtype, R, V, pad, temperature, kl, weights, masks):
     logits, x, tokens = logits_of(R, V, dtype, R + V, pad, masks)
     T, old, adv, ref, w = policy_inputs(x, tokens, R, temperature)
