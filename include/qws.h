@@ -424,9 +424,10 @@ int qws_int4_head(const void* packed, int N, int K, int group, const void* x, lo
  *   out_logprobs [2 P] = s, out_margins [P] = u, out_token_logprobs [R]: optional.
  * NaN among what a used row or pair brings makes the loss and the gradient's rows that depend on it NaN.
  *
- * grad (optional): [R][V] of the logits' type, rows grad_stride >= V apart: the loss's derivative, every row written (0 where
- * there is none).  qws_loss_grad writes it later, times *upstream (device, NULL: 1), from the state that the call left; r as in that call;
- * written != 0: grad is what the call wrote, and stays so where *upstream is 1.  qws_policy_one_pass: 1 where qws_policy_loss takes the
+ * grad (optional): [R][V] of the logits' type, rows grad_stride >= V apart, apart from the logits: the loss's derivative times
+ * grad_scale, every row written (0 where there is none).  qws_loss_grad writes it later, times *upstream (device, NULL: 1), from the
+ * state that the call left; r as in that call; written != 0: grad is what the call wrote with that grad_scale, and stays so where
+ * *upstream is the same.  qws_policy_one_pass: 1 where qws_policy_loss takes the
  * gradient on the same way over the logits, so that asking for it there saves a read of them.
  * state: qws_*_state_bytes, 256-byte aligned, no zeroing needed; one for each loss in flight.  R < 2^24, V <= 2^24, P < 2^23
  * (else QWS_ERR_NOT_SUPPORTED); clip_low in [0, 1], clip_high >= 0, smoothing in [0, 1], all finite.  Statistics are fp32, what
@@ -458,11 +459,12 @@ typedef struct qws_preference_batch {
   float *out_logprobs, *out_margins, *out_token_logprobs;
 } qws_preference_batch;
 size_t qws_policy_state_bytes(int dtype, int R, int V);
-int qws_policy_loss(const qws_policy_batch* b, void* state, size_t state_bytes, void* grad, long long grad_stride, void* stream);
+int qws_policy_loss(const qws_policy_batch* b, void* state, size_t state_bytes, void* grad, long long grad_stride, float grad_scale, void* stream);
 size_t qws_preference_state_bytes(int dtype, int R, int V, int P);
-int qws_preference_loss(const qws_preference_batch* b, void* state, size_t state_bytes, void* grad, long long grad_stride, void* stream);
+int qws_preference_loss(const qws_preference_batch* b, void* state, size_t state_bytes, void* grad, long long grad_stride, float grad_scale,
+                        void* stream);
 int qws_policy_one_pass(int dtype, int R, int V);
-int qws_loss_grad(const qws_loss_rows* r, const void* state, const float* upstream, void* grad, long long grad_stride, int written, void* stream);
+int qws_loss_grad(const qws_loss_rows* r, const void* state, const float* upstream, void* grad, long long grad_stride, float written, void* stream);
 
 /* Argmax over fp32 logits [T][N] -> out_tok[t] (lowest index on ties, NaN never wins) and optional
  * out_val[t].  Same signature and contract as the reference's smk_argmax

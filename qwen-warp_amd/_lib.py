@@ -163,11 +163,11 @@ def load(path=None):
     lib.qws_int4_head_ws_bytes.argtypes, lib.qws_int4_head_ws_bytes.restype = [ci] * 4, sz
     lib.qws_int4_head.argtypes, lib.qws_int4_head.restype = [vp, ci, ci, ci, vp, ll, ci, vp, ci, ll, vp, sz, vp], ci
     lib.qws_policy_state_bytes.argtypes, lib.qws_policy_state_bytes.restype = [ci] * 3, sz
-    lib.qws_policy_loss.argtypes, lib.qws_policy_loss.restype = [C.POINTER(PolicyBatch), vp, sz, vp, ll, vp], ci
+    lib.qws_policy_loss.argtypes, lib.qws_policy_loss.restype = [C.POINTER(PolicyBatch), vp, sz, vp, ll, C.c_float, vp], ci
     lib.qws_preference_state_bytes.argtypes, lib.qws_preference_state_bytes.restype = [ci] * 4, sz
-    lib.qws_preference_loss.argtypes, lib.qws_preference_loss.restype = [C.POINTER(PreferenceBatch), vp, sz, vp, ll, vp], ci
+    lib.qws_preference_loss.argtypes, lib.qws_preference_loss.restype = [C.POINTER(PreferenceBatch), vp, sz, vp, ll, C.c_float, vp], ci
     lib.qws_policy_one_pass.argtypes, lib.qws_policy_one_pass.restype = [ci] * 3, ci
-    lib.qws_loss_grad.argtypes, lib.qws_loss_grad.restype = [C.POINTER(LossRows), vp, vp, vp, ll, ci, vp], ci
+    lib.qws_loss_grad.argtypes, lib.qws_loss_grad.restype = [C.POINTER(LossRows), vp, vp, vp, ll, C.c_float, vp], ci
     lib.qws_pld_default_cfg.argtypes, lib.qws_pld_default_cfg.restype = [C.POINTER(PldCfg)], None
     lib.qws_pld_bytes.argtypes, lib.qws_pld_bytes.restype = [ci, ci], sz
     lib.qws_pld_reset.argtypes, lib.qws_pld_reset.restype = [vp, ci, ci, ci, vp, ci, vp], ci

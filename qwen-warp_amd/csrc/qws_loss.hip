@@ -40,7 +40,6 @@ struct LsRow {
   int mode;            // 0: no gradient
 };
 struct LsHead {
-  double loss;
   float scale;  // of every slope
 };
 
@@ -72,7 +71,8 @@ struct LsArgs {
   // gradient
   void* grad;
   long long grad_stride;
-  const float* upstream;
+  const float* upstream;  // the gradient's factor, or null: grad_scale
+  float grad_scale;
 };
 
 template <typename T>
@@ -379,7 +379,6 @@ __device__ __forceinline__ void ls_total(const LsArgs& a, double s, int k, int p
   }
   if (pairs) k = pairs;
   const double scale = a.weights || k == 0 ? 1.0 : 1.0 / k;
-  a.head->loss = s * scale;
   a.head->scale = (float)scale;
   *a.out_loss = (float)(s * scale);
 }
@@ -550,12 +549,12 @@ __device__ __forceinline__ float ls_held(float slope) {  // no infinity meets a 
   return fabsf(slope) > 0.25f * F32_MAX ? copysignf(0.25f * F32_MAX, slope) : slope;
 }
 
-// written: the gradient is there for an upstream of 1.  Rows from the last on: the logits that k_ls_scan read last may still be in the
+// written != 0: the gradient is there, for an upstream of that value.  Rows from the last on: the logits that k_ls_scan read last may still be in the
 // memory's cache.
 template <typename T, int U>
-__global__ void __launch_bounds__(LS_NT) k_ls_grad(LsArgs a, int written) {
-  const float upstream = a.upstream ? *a.upstream : 1.0f;
-  if (written && upstream == 1.0f) return;
+__global__ void __launch_bounds__(LS_NT) k_ls_grad(LsArgs a, float written) {
+  const float upstream = a.upstream ? *a.upstream : a.grad_scale;
+  if (written != 0.0f && upstream == written) return;
   const float scale = a.head->scale * upstream;
   for (unsigned i = blockIdx.x; i < (unsigned)a.R * a.G; i += gridDim.x) {
     const int row = a.R - 1 - (int)(i / a.G), ch = i % a.G;
@@ -649,7 +648,7 @@ __global__ void __launch_bounds__(NT) k_ls_policy(LsArgs a) {
     a.term[row] = ls_policy<T>(a, row, tok, v, c, temp);
     const LsRow q = a.rows[row];  // this thread's own
     s_row = q;
-    s_slope = q.mode ? ls_held(a.slope[row] * (a.weights ? 1.0f : a.head->scale) * q.per_t) : 0.0f;
+    s_slope = q.mode ? ls_held(a.slope[row] * ((a.weights ? 1.0f : a.head->scale) * a.grad_scale) * q.per_t) : 0.0f;
   }
   bar();
   const LsRow q = s_row;
@@ -772,15 +771,15 @@ static void ls_scan(const LsArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((k_ls_scan<T, LS_U>), dim3((unsigned)a.R * a.G), dim3(LS_NT), 0, st, a);
 }
 template <typename T>
-static void ls_grad_of(const LsArgs& a, int written, hipStream_t st) {
+static void ls_grad_of(const LsArgs& a, float written, hipStream_t st) {
   unsigned wgs = (unsigned)a.R * a.G;
-  if (written && wgs > 1024) wgs = 1024;  // most often they find it written
+  if (written != 0.0f && wgs > 4096) wgs = 4096;  // most often they find it written
   if (a.per == 1)
     hipLaunchKernelGGL((k_ls_grad<T, 1>), dim3(wgs), dim3(LS_NT), 0, st, a, written);
   else
     hipLaunchKernelGGL((k_ls_grad<T, LS_U>), dim3(wgs), dim3(LS_NT), 0, st, a, written);
 }
-static void ls_grad(const LsArgs& a, int dtype, int written, hipStream_t st) {
+static void ls_grad(const LsArgs& a, int dtype, float written, hipStream_t st) {
   dtype == QWS_DTYPE_F32 ? ls_grad_of<float>(a, written, st) : ls_grad_of<uint16_t>(a, written, st);
 }
 // Whether a policy loss with its gradient takes a workgroup per row (k_ls_policy): from 128 rows on, or where the row's workgroup holds
@@ -850,8 +849,9 @@ extern "C" size_t qws_preference_state_bytes(int dtype, int R, int V, int P) {
   return ls_state(dtype, R, V, 2ll * P, P).total;
 }
 
-extern "C" int qws_policy_loss(const qws_policy_batch* b, void* state, size_t state_bytes, void* grad, long long grad_stride, void* stream) {
+extern "C" int qws_policy_loss(const qws_policy_batch* b, void* state, size_t state_bytes, void* grad, long long grad_stride, float grad_scale, void* stream) {
   using namespace qws;
+  if (!ls_number(grad_scale)) return QWS_ERR_INVALID;
   if (!b || !ls_rows_ok(b->rows) || !b->out_loss || !ls_aligned(state)) return QWS_ERR_INVALID;
   if (!(b->clip_low >= 0.0f && b->clip_low <= 1.0f) || !(b->clip_high >= 0.0f) || !ls_number(b->clip_high) || !ls_number(b->kl)) return QWS_ERR_INVALID;
   const int R = b->rows.R, V = b->rows.V;
@@ -872,6 +872,7 @@ extern "C" int qws_policy_loss(const qws_policy_batch* b, void* state, size_t st
   a.out_lp = b->out_logprobs;
   a.out_ratio = b->out_ratio;
   a.out_kl = b->out_kl;
+  a.grad_scale = grad_scale;
   hipStream_t st = (hipStream_t)stream;
   if (R && grad && ls_one_pass(b->rows.dtype, R, V)) {
     a.grad = grad;
@@ -890,8 +891,9 @@ extern "C" int qws_policy_loss(const qws_policy_batch* b, void* state, size_t st
   return (int)hipGetLastError();
 }
 
-extern "C" int qws_preference_loss(const qws_preference_batch* b, void* state, size_t state_bytes, void* grad, long long grad_stride, void* stream) {
+extern "C" int qws_preference_loss(const qws_preference_batch* b, void* state, size_t state_bytes, void* grad, long long grad_stride, float grad_scale, void* stream) {
   using namespace qws;
+  if (!ls_number(grad_scale)) return QWS_ERR_INVALID;
   if (!b || !ls_rows_ok(b->rows) || !b->out_loss || !ls_aligned(state) || b->P < 0 || (b->P && !b->starts)) return QWS_ERR_INVALID;
   if (!ls_number(b->beta) || !ls_number(b->margin) || !(b->smoothing >= 0.0f && b->smoothing <= 1.0f)) return QWS_ERR_INVALID;
   const int R = b->rows.R, V = b->rows.V, P = b->P;
@@ -913,6 +915,7 @@ extern "C" int qws_preference_loss(const qws_preference_batch* b, void* state, s
   a.out_lp = b->out_token_logprobs;
   a.out_sums = b->out_logprobs;
   a.out_margins = b->out_margins;
+  a.grad_scale = grad_scale;
   hipStream_t st = (hipStream_t)stream;
   b->rows.dtype == QWS_DTYPE_F32 ? ls_preference_run<float>(a, st) : ls_preference_run<uint16_t>(a, st);
   if (R && grad) {
@@ -925,9 +928,9 @@ extern "C" int qws_preference_loss(const qws_preference_batch* b, void* state, s
 
 extern "C" int qws_policy_one_pass(int dtype, int R, int V) { return R > 0 && V > 0 && qws::ls_one_pass(dtype, R, V); }
 
-extern "C" int qws_loss_grad(const qws_loss_rows* r, const void* state, const float* upstream, void* grad, long long grad_stride, int written, void* stream) {
+extern "C" int qws_loss_grad(const qws_loss_rows* r, const void* state, const float* upstream, void* grad, long long grad_stride, float written, void* stream) {
   using namespace qws;
-  if (!r || !ls_rows_ok(*r) || !ls_aligned(state) || (r->R && (!grad || !ls_grad_ok(*r, grad, grad_stride)))) return QWS_ERR_INVALID;
+  if (!ls_number(written) || !r || !ls_rows_ok(*r) || !ls_aligned(state) || (r->R && (!grad || !ls_grad_ok(*r, grad, grad_stride)))) return QWS_ERR_INVALID;
   if (!ls_fits(r->R, r->V)) return QWS_ERR_NOT_SUPPORTED;
   if (r->R == 0) return QWS_OK;
   LsArgs a = ls_args(*r, (char*)state, ls_state(r->dtype, r->R, r->V, 0, 0));  // the places of the rows and slopes do not depend on the loss
@@ -935,6 +938,7 @@ extern "C" int qws_loss_grad(const qws_loss_rows* r, const void* state, const fl
   a.upstream = upstream;
   a.grad = grad;
   a.grad_stride = grad_stride;
-  ls_grad(a, r->dtype, written && upstream, (hipStream_t)stream);
+  a.grad_scale = 1.0f;
+  ls_grad(a, r->dtype, upstream ? written : 0.0f, (hipStream_t)stream);
   return (int)hipGetLastError();
 }

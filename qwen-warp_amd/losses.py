@@ -58,15 +58,15 @@ def blocks_of(x: torch.Tensor, name: str):
 
 
 class _Loss(torch.autograd.Function):
-    """The loss as a function of the logits; `call(grad)` runs it and returns (loss, rows, state, what they refer to).  With
-    `ahead` the gradient is written by the forward pass, for an upstream gradient of 1; the first backward pass hands it out, after
-    a launch that writes it anew for any other.  Later ones write their own."""
+    """The loss as a function of the logits; `call(grad, scale)` runs it and returns (loss, rows, state, what they refer to).  With
+    `ahead` (not 0) the gradient is written by the forward pass, for an upstream gradient of that value; the first backward pass
+    hands it out, after a launch that writes it anew for any other.  Later ones write their own."""
 
     @staticmethod
     def forward(ctx, logits, owner, call, ahead):
         ctx.grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if ahead else None
-        loss, ctx.rows, ctx.state, ctx.keep = call(ctx.grad)
-        ctx.owner = owner
+        loss, ctx.rows, ctx.state, ctx.keep = call(ctx.grad, ahead)
+        ctx.owner, ctx.ahead = owner, ahead
         ctx.save_for_backward(logits)
         return loss
 
@@ -77,8 +77,9 @@ class _Loss(torch.autograd.Function):
         where, stream = on_stream(logits.device.index)
         with where:
             grad, ctx.grad = ctx.grad, None
-            written = grad is not None
-            if not written:
+            written = ctx.ahead
+            if grad is None:
+                written = 0.0
                 grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
             err = ctx.owner.lib.qws_loss_grad(C.byref(ctx.rows), ctx.state.data_ptr(), upstream.data_ptr(), grad.data_ptr(), ctx.rows.V, written, stream)
             if err:
@@ -125,10 +126,10 @@ class _Base:
                 raise ValidationError("logits: fewer than 2^24 rows of at most 2^24 values", "logits")
         return n
 
-    def _forward(self, logits, call, ahead=False):
-        """call(grad), with autograd where the logits ask for it."""
+    def _forward(self, logits, call, ahead=0.0):
+        """The loss, with autograd where the logits ask for it."""
         if not (logits.requires_grad and torch.is_grad_enabled()):
-            return call(None)[0]
+            return call(None, 1.0)[0]
         if torch.cuda.is_current_stream_capturing():  # a backward pass there ends the process where an eager graph of the same leaves lives
             raise ValidationError("inside a captured graph the gradient is value_and_grad's", "logits")
         return _Loss.apply(logits, self, call, ahead)
@@ -146,22 +147,28 @@ class PolicyLoss(_Base):
     -min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A) + kl (e^d - 1 - d), times its weight; without weights the mean over the rows with a token.
     logits: fp32 or bf16, rows contiguous, the leading dimensions at up to two strides.  tokens: int32 (`Sampler`'s; one
     outside [0, V), as -1, leaves its row out).  old_logprobs (`LogProbs`'), advantages, ref_logprobs, weights,
-    temperature (0, negative or NaN: as 1): fp32, constants.  Calls run on any streams; the workspace is allocated with each call."""
+    temperature (0, negative or NaN: as 1): fp32, constants.  Calls run on any streams; the workspace is allocated with each call.
+    upstream: the upstream gradient that backward passes will most often bring (1 / n for a loss that is divided by n, a loss
+    scaler's factor); it may be set between calls.  Any other is right too, but costs another way over the logits."""
 
-    def __init__(self, device="cuda", clip: Sequence[float] = (0.2, 0.2), kl: float = 0.0):
+    def __init__(self, device="cuda", clip: Sequence[float] = (0.2, 0.2), kl: float = 0.0, upstream: float = 1.0):
         super().__init__(device)
         low, high = (float(c) for c in clip)
         if not (0.0 <= low <= 1.0 and 0.0 <= high < 1e38):
             raise ValidationError("clip must be (in [0, 1], >= 0)", "clip", clip)
         if not abs(float(kl)) < 1e38:
             raise ValidationError("kl must be finite", "kl", kl)
-        self.clip, self.kl = (low, high), float(kl)
+        if not abs(float(upstream)) < 1e38:
+            raise ValidationError("upstream must be finite", "upstream", upstream)
+        self.clip, self.kl, self.upstream = (low, high), float(kl), float(upstream)
 
     def __call__(self, logits: torch.Tensor, tokens: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor, ref_logprobs: Optional[torch.Tensor] = None,
                  weights: Optional[torch.Tensor] = None, temperature: Optional[torch.Tensor] = None) -> PolicyLossResult:
         call, others = self._prepare(logits, tokens, old_logprobs, advantages, ref_logprobs, weights, temperature)
         # from some size on the gradient comes on the loss's own way over the logits
-        ahead = bool(self.lib.qws_policy_one_pass(_lib.DTYPE_F32 if logits.dtype == torch.float32 else _lib.DTYPE_BF16, others[0].numel(), logits.shape[-1]))
+        ahead = 0.0
+        if logits.requires_grad and self.lib.qws_policy_one_pass(_lib.DTYPE_F32 if logits.dtype == torch.float32 else _lib.DTYPE_BF16, others[0].numel(), logits.shape[-1]):
+            ahead = self.upstream
         return PolicyLossResult(self._forward(logits, call, ahead), *others)
 
     def value_and_grad(self, logits: torch.Tensor, tokens: torch.Tensor, old_logprobs: torch.Tensor, advantages: torch.Tensor,
@@ -170,7 +177,7 @@ class PolicyLoss(_Base):
         """(the result, the loss's gradient at the logits: their type and shape, contiguous)."""
         call, others = self._prepare(logits, tokens, old_logprobs, advantages, ref_logprobs, weights, temperature)
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        return PolicyLossResult(call(grad)[0], *others), grad
+        return PolicyLossResult(call(grad, 1.0)[0], *others), grad
 
     def _prepare(self, logits, tokens, old, adv, ref, weights, temperature):
         rows = self._rows(logits, tokens, temperature)
@@ -184,12 +191,12 @@ class PolicyLoss(_Base):
             ratio = torch.empty_like(lp)
             kl = torch.empty_like(lp) if ref is not None else None
 
-        def call(grad):
+        def call(grad, scale):
             with where:
                 loss = lp.new_empty(())
                 state = torch.empty(n, dtype=torch.uint8, device=dev)
                 b = _lib.PolicyBatch(rows, *inputs, *self.clip, self.kl, loss.data_ptr(), lp.data_ptr(), ratio.data_ptr(), kl.data_ptr() if kl is not None else None)
-                err = self.lib.qws_policy_loss(C.byref(b), state.data_ptr(), n, grad.data_ptr() if grad is not None else None, rows.V, stream)
+                err = self.lib.qws_policy_loss(C.byref(b), state.data_ptr(), n, grad.data_ptr() if grad is not None else None, rows.V, scale, stream)
                 if err:
                     check(err, "qws_policy_loss")
             return loss, rows, state, tokens
@@ -230,7 +237,7 @@ class PreferenceLoss(_Base):
         """(the result, the loss's gradient at the logits: their type and shape, contiguous)."""
         call, others = self._prepare(logits, tokens, starts, ref, weights)
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        return PreferenceLossResult(call(grad)[0], *others), grad
+        return PreferenceLossResult(call(grad, 1.0)[0], *others), grad
 
     def _prepare(self, logits, tokens, starts, ref, weights):
         rows = self._rows(logits, tokens)
@@ -253,13 +260,13 @@ class PreferenceLoss(_Base):
             lp = torch.empty(lead, dtype=torch.float32, device=dev)
             sums, margins = lp.new_empty(2 * P), lp.new_empty(P)
 
-        def call(grad):
+        def call(grad, scale):
             with where:
                 loss = lp.new_empty(())
                 state = torch.empty(n, dtype=torch.uint8, device=dev)
                 b = _lib.PreferenceBatch(rows, starts.data_ptr(), P, self.average, *inputs, self.beta, self.margin, self.smoothing, loss.data_ptr(), sums.data_ptr(),
                                          margins.data_ptr(), lp.data_ptr())
-                err = self.lib.qws_preference_loss(C.byref(b), state.data_ptr(), n, grad.data_ptr() if grad is not None else None, rows.V, stream)
+                err = self.lib.qws_preference_loss(C.byref(b), state.data_ptr(), n, grad.data_ptr() if grad is not None else None, rows.V, scale, stream)
                 if err:
                     check(err, "qws_preference_loss")
             return loss, rows, state, tokens

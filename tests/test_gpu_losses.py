@@ -320,6 +320,14 @@ def test_upstream_gradients(loss):
     a = torch.autograd.grad(l, leaf, retain_graph=True)[0]
     b = torch.autograd.grad(l * 0.5, leaf)[0]
     assert torch.equal(a, first) and torch.equal(a, g) and torch.equal(b, 0.5 * g)
+    if loss == "policy":  # an upstream gradient that was named beforehand, met and missed (powers of two: exact)
+        fn.upstream = 0.25
+        l = fn(leaf, *args).loss
+        assert torch.equal(torch.autograd.grad(l * 0.25, leaf, retain_graph=True)[0], 0.25 * g) and torch.equal(torch.autograd.grad(l, leaf)[0], g)
+        assert torch.equal(torch.autograd.grad(fn(leaf, *args).loss, leaf)[0], g) and torch.equal(fn.value_and_grad(logits, *args)[1], g)
+        fn.upstream = 0.0
+        assert (torch.autograd.grad(fn(leaf, *args).loss * 0.0, leaf)[0] == 0).all() and torch.equal(torch.autograd.grad(fn(leaf, *args).loss, leaf)[0], g)
+        fn.upstream = 1.0
     h = torch.randn(R, 32, device="cuda", requires_grad=True)
     w = torch.randn(V, 32, device="cuda", requires_grad=True)
     y = h @ w.t()

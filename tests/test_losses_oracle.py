@@ -109,21 +109,21 @@ def test_sizes_and_refusals():
             setattr(r, k, v)
         return r
 
-    def policy(state=256, size=n, grad=None, stride=10, r=None, **kw):
+    def policy(state=256, size=n, grad=None, stride=10, r=None, scale=1.0, **kw):
         b = _lib.PolicyBatch(r or rows(), 256, 256, None, None, 0.2, 0.2, 0.0, 256, None, None, None)
         for k, v in kw.items():
             setattr(b, k, v)
-        return lib.qws_policy_loss(C.byref(b), state, size, grad, stride, None)
+        return lib.qws_policy_loss(C.byref(b), state, size, grad, stride, scale, None)
 
-    def preference(state=256, size=n, grad=None, stride=10, r=None, **kw):
+    def preference(state=256, size=n, grad=None, stride=10, r=None, scale=1.0, **kw):
         b = _lib.PreferenceBatch(r or rows(), 256, 2, 0, None, None, 0.1, 0.0, 0.0, 256, None, None, None)
         for k, v in kw.items():
             setattr(b, k, v)
-        return lib.qws_preference_loss(C.byref(b), state, size, grad, stride, None)
+        return lib.qws_preference_loss(C.byref(b), state, size, grad, stride, scale, None)
 
     nan, inf = float("nan"), float("inf")
     for f in (policy, preference):
-        for kw in (dict(state=None), dict(state=257), dict(size=100), dict(grad=258), dict(grad=256, stride=9), dict(out_loss=None), dict(r=rows(logits=None)),
+        for kw in (dict(state=None), dict(state=257), dict(size=100), dict(grad=258), dict(grad=256, stride=9), dict(out_loss=None), dict(scale=nan), dict(scale=inf), dict(r=rows(logits=None)),
                    dict(r=rows(logits=258)), dict(r=rows(dtype=5)), dict(r=rows(tokens=None)), dict(r=rows(R=-1)), dict(r=rows(V=0)), dict(r=rows(block=-1)),
                    dict(r=rows(row_stride=-1)), dict(r=rows(block_stride=-1))):
             assert f(**kw) == _lib.ERR_INVALID, kw
@@ -139,12 +139,13 @@ def test_sizes_and_refusals():
     assert lib.qws_loss_grad(C.byref(r), None, None, 256, 10, 0, None) == _lib.ERR_INVALID
     assert lib.qws_loss_grad(C.byref(r), 256, None, None, 10, 0, None) == _lib.ERR_INVALID
     assert lib.qws_loss_grad(C.byref(r), 256, None, 256, 9, 0, None) == _lib.ERR_INVALID
+    assert lib.qws_loss_grad(C.byref(r), 256, None, 256, 10, nan, None) == _lib.ERR_INVALID
     r = rows(R=0)
     assert lib.qws_loss_grad(C.byref(r), 256, None, None, 0, 0, None) == _lib.OK
 
 
 def test_python_refusals():
-    for bad in (dict(clip=(-0.1, 0.2)), dict(clip=(0.2, float("nan"))), dict(kl=float("inf"))):
+    for bad in (dict(clip=(-0.1, 0.2)), dict(clip=(0.2, float("nan"))), dict(kl=float("inf")), dict(upstream=float("nan"))):
         with pytest.raises(q.ValidationError):
             q.PolicyLoss("cuda", **bad)
     for bad in (dict(beta=float("nan")), dict(margin=float("inf")), dict(smoothing=1.5)):
