@@ -2,15 +2,15 @@
 // 128 weights along K (the definitions: include/qws.h qws_int4_*).
 //
 // Products.  y = sum over groups of s (sum_k q x - z sum_k x), q and z in 0 .. 15.  The codes enter the bf16 matrix instruction
-// as 16 + q, which is exact in bf16 and takes one shift and one and-or for two of them: a code's four bits are the top of the
+// as 16 + q, which is exact in bf16 and takes an and-or for two of them, and for three of four pairs a shift: a code's four bits are the top of the
 // fraction of a number in [16, 32).  The hidden states enter as they are, so a group's products are exact and summed in fp32; the
 // 16 is taken off with the zero point, (16 + z) sum_k x, whose sum of hidden states is a product with ones, once for
 // all of a wave's weights.  Then the scale is applied in fp32: nothing is rounded to fewer bits.  The offset makes a group's sum
 // some five times as large as what is left of it, so its error is a few 2^-24 of the group's terms.
 //
 // Layout.  16 weight rows x 128 values are a fragment of 1 KB: lane l's 16 bytes are row l % 16, word j values 32 j + 8 (l / 16)
-// .. + 7, the second operand of the 16x16x32 product j; value 2 i and 2 i + 1 of a word are bits 4 i .. and 4 i + 16 .., so that one
-// mask takes a pair into the halves of a register.  Four fragments (64 rows) lie together for each 128 values of K, 4 KB that one
+// .. + 7, the second operand of the 16x16x32 product j; a word's pairs lie so that one mask takes a pair, turned by a multiple of four,
+// into the halves of a register where the fractions' top bits are (i4_word).  Four fragments (64 rows) lie together for each 128 values of K, 4 KB that one
 // wave reads at once.  A scale is a word: fp32 (from bf16 or fp16: the low 13 bits are 0) with 16 + z in its low byte; the 64 words of a
 // tile's rows lie together for each group.  Values beyond K are 0, rows beyond N not used.
 #include "qws_lds.h"
@@ -59,6 +59,13 @@ __device__ __forceinline__ uint32_t i4_nearest_bf16(float x) {  // a finite x >=
   return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
 }
 
+// Eight codes as a word: pair p = codes 2 p and 2 p + 1 at bits 3 .. 6 and 19 .. 22 of the word turned right by 4 p
+__device__ __forceinline__ uint32_t i4_word(const uint32_t (&code)[8]) {
+  uint32_t f[4];
+#pragma unroll
+  for (int p = 0; p < 4; p++) f[p] = code[2 * p] << 3 | code[2 * p + 1] << 19;
+  return f[0] | f[1] << 4 | f[2] << 8 | (f[3] >> 4 | f[3] << 28);
+}
 // Elements k0 .. k0 + 7 of a row as bits, those from K on as 0
 template <typename T>
 __device__ __forceinline__ void i4_load(const T* row, int k0, int K, uint32_t (&v)[8]) {
@@ -114,12 +121,11 @@ __global__ void __launch_bounds__(256) k_i4_pack(I4Pack a) {
 #pragma unroll
       for (int j = 0; j < J; j++) {
         const int k0 = kb * I4_KB + 32 * (g * J + j) + 8 * quad;
-        uint32_t v = 0;
         uint32_t code[8];
         i4_load(row, k0, a.K, code);
 #pragma unroll
-        for (int e = 0; e < 8; e++) v |= (code[e] & 15u) << (4 * (e >> 1) + 16 * (e & 1));
-        q[g * J + j] = v;
+        for (int e = 0; e < 8; e++) code[e] &= 15u;
+        q[g * J + j] = i4_word(code);
       }
       if (r < a.N && kg * GROUP < a.K) {
         const uint32_t s = *gmem(a.scales + (long long)at * a.scale_stride + kg);
@@ -157,13 +163,10 @@ __global__ void __launch_bounds__(256) k_i4_pack(I4Pack a) {
       const float z = fminf(fmaxf(rintf(-lo / d), 0.0f), 15.0f);
 #pragma unroll
       for (int j = 0; j < J; j++) {
-        uint32_t u = 0;
+        uint32_t code[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float c = fminf(fmaxf(rintf(v[j][e] / d) + z, 0.0f), 15.0f);
-          u |= (bad ? 0u : (uint32_t)c) << (4 * (e >> 1) + 16 * (e & 1));
-        }
-        q[g * J + j] = u;
+        for (int e = 0; e < 8; e++) code[e] = bad ? 0u : (uint32_t)fminf(fmaxf(rintf(v[j][e] / d) + z, 0.0f), 15.0f);
+        q[g * J + j] = i4_word(code);
       }
       if (bad)
         word = 0x7FC00000u | 16;  // a value that is not finite, or a range past fp32: NaN
@@ -195,8 +198,8 @@ struct I4Args {
   long long out_stride;
 };
 
-// The pairs of a word's eight codes as 16 + q in bf16: a shift and an and-or each.  The instruction takes one scalar operand, so one of
-// the two constants is a register that the compiler does not see through (it would take two instructions).
+// The pairs of a word's eight codes as 16 + q in bf16: an and-or each, and a shift for all but the first.  The instruction takes one
+// scalar operand, so one of the two constants is a register that the compiler does not see through (it would take two instructions).
 struct I4Wide {
   uint32_t mask, base;
   __device__ __forceinline__ I4Wide() {
@@ -204,7 +207,7 @@ struct I4Wide {
     asm("v_mov_b32 %0, 0x41804180" : "=v"(base));
   }
   __device__ __forceinline__ i4_b8 operator()(uint32_t w) const {
-    const vu4 u = {(w << 3 & mask) | base, (w >> 1 & mask) | base, (w >> 5 & mask) | base, (w >> 9 & mask) | base};
+    const vu4 u = {(w & mask) | base, (w >> 4 & mask) | base, (w >> 8 & mask) | base, (__builtin_amdgcn_alignbit(w, w, 28) & mask) | base};
     return __builtin_bit_cast(i4_b8, u);
   }
 };
@@ -355,10 +358,10 @@ __global__ void __launch_bounds__(256) k_i4_states_tile(const uint16_t* x, long 
 
 // More hidden states: a workgroup takes 256 weight rows and 16 TF hidden states, a wave 64 of the rows over all of K.  Hidden states and
 // their sums are copied into LDS by the memory system two blocks ahead (three buffers), the weights go straight into registers, two
-// blocks ahead as well: one block ahead left too few bytes in flight (36 states at K = 5,120, N = 248,320 172 us, 163 so).  What bounds it:
-// up to 48 states mostly the bytes (36 states 163 us: 4.3 TB/s of weights and logits); from there on the products and the vector
+// blocks ahead as well: one block ahead left too few bytes in flight (36 states at K = 5,120, N = 248,320 172 us, 163 so; 155 with the later steps).  What bounds it:
+// up to 48 states mostly the bytes (36 states 155 us: 4.6 TB/s of weights and logits); from there on the products and the vector
 // instructions beside them, which take turns on this card: a 16x16x32 product and four others take 25 cycles of a SIMD, alone 17 and 11.
-// So the instructions are what counts: two for two codes, two for each scaled sum.
+// So the instructions are what counts: seven for eight codes (eight, 64 states 191 us, 188 so), two for each scaled sum.
 template <typename O, int GROUP, int TF>
 __global__ void __launch_bounds__(256, 2) k_i4_tile(I4Args a) {
   constexpr int G = I4_ROWS / 16, C = I4_KB / GROUP, J = GROUP / 32, REC = i4_record(TF);
