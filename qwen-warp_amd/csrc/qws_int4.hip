@@ -390,8 +390,8 @@ __global__ void __launch_bounds__(256, 2) k_i4_tile(I4Args a) {
     const char* mine = rec + wave * (TF * 1024);
     lds_copy<0>(mine, 16 * lane, to + wave * (TF * 1024));
     if constexpr (TF > 1) lds_copy<1024>(mine, 16 * lane, to + wave * (TF * 1024));
-    if constexpr (TF > 2) lds_copy<2048>(mine, 16 * lane, to + wave * (TF * 1024));
-    if constexpr (TF > 3) lds_copy<3072>(mine, 16 * lane, to + wave * (TF * 1024));
+    if constexpr (TF > 2) lds_copy<2 * 1024>(mine, 16 * lane, to + wave * (TF * 1024));
+    if constexpr (TF > 3) lds_copy<3 * 1024>(mine, 16 * lane, to + wave * (TF * 1024));
     lds_copy_words(rec + TF * 4096 + wave * 256, 4 * lane, to + TF * 4096 + wave * 256);
   };
   // what is left of fragment g's group c when its products are done
