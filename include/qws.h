@@ -426,7 +426,7 @@ int qws_int4_head(const void* packed, int N, int K, int group, const void* x, lo
  *
  * grad (optional): [R][V] of the logits' type, rows grad_stride >= V apart, apart from the logits: the loss's derivative times
  * grad_scale, every row written (0 where there is none).  qws_loss_grad writes it later, times *upstream (device, NULL: 1), from the
- * state that the call left; r as in that call; written != 0: grad is what the call wrote with that grad_scale, and stays so where
+ * state that the call left; r as in that call (the same logits, which may lie elsewhere and at other strides); written != 0: grad is what the call wrote with that grad_scale, and stays so where
  * *upstream is the same.  qws_policy_one_pass: 1 where qws_policy_loss takes the
  * gradient on the same way over the logits, so that asking for it there saves a read of them.
  * state: qws_*_state_bytes, 256-byte aligned, no zeroing needed; one for each loss in flight.  R < 2^24, V <= 2^24, P < 2^23

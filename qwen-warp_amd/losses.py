@@ -57,16 +57,25 @@ def blocks_of(x: torch.Tensor, name: str):
     raise ValidationError(f"{name}: the leading dimensions must lie at two strides at most (reshape it)", name)
 
 
+def structure(logits, tokens: int, temperature: Optional[int] = None):
+    """The rows of logits fp32 / bf16 [..., V] as the library takes them; tokens, temperature: addresses."""
+    R, block, stride, block_stride = blocks_of(logits, "logits")
+    return _lib.LossRows(logits.data_ptr(), _lib.DTYPE_F32 if logits.dtype == torch.float32 else _lib.DTYPE_BF16, R, logits.shape[-1], block, stride, block_stride,
+                         tokens, temperature)
+
+
 class _Loss(torch.autograd.Function):
     """The loss as a function of the logits; `call(grad, scale)` runs it and returns (loss, rows, state, what they refer to).  With
     `ahead` (not 0) the gradient is written by the forward pass, for an upstream gradient of that value; the first backward pass
-    hands it out, after a launch that writes it anew for any other.  Later ones write their own."""
+    hands it out, after a launch that writes it anew for any other.  Later ones write their own.  The logits of a backward pass are
+    those that autograd hands out: under hooks on saved tensors (an offload to the host, a checkpoint that makes them anew) another
+    tensor than the forward pass read, whose memory may be gone, and in strides of its own."""
 
     @staticmethod
     def forward(ctx, logits, owner, call, ahead):
         ctx.grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if ahead else None
-        loss, ctx.rows, ctx.state, ctx.keep = call(ctx.grad, ahead)
-        ctx.owner, ctx.ahead = owner, ahead
+        loss, rows, ctx.state, ctx.keep = call(ctx.grad, ahead)
+        ctx.owner, ctx.ahead, ctx.tokens, ctx.of = owner, ahead, rows.tokens, (logits.shape, logits.dtype, logits.device)
         ctx.save_for_backward(logits)
         return loss
 
@@ -74,6 +83,8 @@ class _Loss(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, upstream):
         (logits,) = ctx.saved_tensors
+        if (logits.shape, logits.dtype, logits.device) != ctx.of:
+            raise ValidationError(f"the saved logits came back as {logits.dtype} {tuple(logits.shape)} on {logits.device}", "logits")
         where, stream = on_stream(logits.device.index)
         with where:
             grad, ctx.grad = ctx.grad, None
@@ -81,7 +92,12 @@ class _Loss(torch.autograd.Function):
             if grad is None:
                 written = 0.0
                 grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            err = ctx.owner.lib.qws_loss_grad(C.byref(ctx.rows), ctx.state.data_ptr(), upstream.data_ptr(), grad.data_ptr(), ctx.rows.V, written, stream)
+            try:
+                rows = structure(logits, ctx.tokens)
+            except ValidationError:  # strides that the forward pass would have refused
+                logits = logits.contiguous()
+                rows = structure(logits, ctx.tokens)
+            err = ctx.owner.lib.qws_loss_grad(C.byref(rows), ctx.state.data_ptr(), upstream.data_ptr(), grad.data_ptr(), rows.V, written, stream)
             if err:
                 check(err, "qws_loss_grad")
         return grad, None, None, None
@@ -100,13 +116,11 @@ class _Base:
             raise ValidationError("logits must be a CUDA fp32 / bf16 tensor", "logits")
         if dev != self.device and (self.device.type != "cuda" or self.device.index is not None):
             raise ValidationError(f"logits must be on {self.device}", "logits")
-        R, block, stride, block_stride = blocks_of(logits, "logits")
-        if logits.shape[-1] < 1:
+        if logits.dim() and logits.shape[-1] < 1:
             raise ValidationError("logits must have a value a row", "logits")
         lead = logits.shape[:-1]
         given(tokens, lead, torch.int32, dev, "tokens")
-        return _lib.LossRows(logits.data_ptr(), _lib.DTYPE_F32 if dtype == torch.float32 else _lib.DTYPE_BF16, R, logits.shape[-1], block, stride, block_stride,
-                             tokens.data_ptr(), self._number(temperature, lead, dev, "temperature") if temperature is not None else None)
+        return structure(logits, tokens.data_ptr(), self._number(temperature, lead, dev, "temperature") if temperature is not None else None)
 
     @staticmethod
     def _number(t, shape, dev, name):

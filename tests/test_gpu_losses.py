@@ -11,6 +11,7 @@ the logits' type.  What lies below 2^-126 may be 0."""
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import qwen_warp_amd as q
 from oracle import losses as O
@@ -492,3 +493,46 @@ def test_graphs():
         assert torch.equal(oa.loss, wa.loss) and torch.equal(ga, wga) and torch.equal(ob.loss, wb.loss) and torch.equal(gb, wgb)
     eager.backward()
     assert torch.isfinite(eager_leaf.grad).all()
+
+
+@pytest.mark.parametrize("loss,R,V", [("policy", 6, 100003), ("policy", 20, 5000), ("policy", 130, 33003), ("preference", 6, 100003), ("preference", 60, 700)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_saved_tensor_hooks_and_checkpoints(loss, R, V, dtype):
+    """The backward pass reads the logits that autograd hands it: copies in other strides whose original was overwritten, copies
+    brought back from the host, logits that a checkpoint made anew.  Each equals the plain one, with and without a gradient
+    that the forward pass wrote, at another upstream gradient (a power of two: exact) and in a second pass."""
+    logits, x, tokens = logits_of(R, V, dtype, R + 1)
+    _, old, adv, _, _ = policy_inputs(x, tokens, 13, False)
+    if loss == "policy":
+        fn, args = q.PolicyLoss("cuda"), (tokens.cuda(), dev(old), dev(adv))
+    else:
+        fn, args = q.PreferenceLoss("cuda"), (tokens.cuda(), dev(np.array([0, 2, R // 2, R - 1, R], np.int32)))
+    _, g = fn.value_and_grad(logits, *args)
+    _, g2 = fn.value_and_grad(logits * 2, *args)  # of the logits that the model below makes
+
+    def padded(t):
+        buf = torch.full((R, V + 3), NAN, dtype=dtype, device="cuda")[:, 1:V + 1]
+        return buf.copy_(t)
+
+    leaf = logits.detach().requires_grad_()
+    for pack, unpack in ((torch.clone, lambda t: t), (torch.clone, padded), (torch.clone, lambda t: t.t().contiguous().t())):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            y = leaf * 1.0
+            l = fn(y, *args).loss
+        y.detach().fill_(NAN)
+        (a,) = torch.autograd.grad(4 * l, leaf, retain_graph=True)
+        (b,) = torch.autograd.grad(l, leaf)
+        assert torch.equal(a, 4 * g) and torch.equal(b, g)
+    with torch.autograd.graph.save_on_cpu():
+        l = fn(leaf * 1.0, *args).loss
+    junk = [torch.full_like(logits, NAN) for _ in range(3)]  # what was freed is used again
+    (a,) = torch.autograd.grad(4 * l, leaf, retain_graph=True)
+    (b,) = torch.autograd.grad(l, leaf)
+    assert torch.equal(a, 4 * g) and torch.equal(b, g)
+    del junk
+    for factor in (1.0, 4.0):
+        l = torch.utils.checkpoint.checkpoint(lambda t: fn(t * 2, *args).loss, leaf, use_reentrant=False)
+        junk = [torch.full_like(logits, NAN) for _ in range(3)]
+        (a,) = torch.autograd.grad(factor * l, leaf)
+        assert torch.equal(a, 2 * factor * g2)
+        del junk
