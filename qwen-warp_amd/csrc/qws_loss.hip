@@ -545,7 +545,12 @@ __device__ __forceinline__ void ls_grad_part(const LsRow& q, const T* x_row, T* 
     }
   }
 }
-__device__ __forceinline__ float ls_held(float slope) {  // no infinity meets a p of 0; NaN stays
+// A row's slope at its logits.  Held where it passes fp32: no infinity meets a p of 0; NaN stays.  A slope of 0 is one at every
+// temperature, where 1 / T is past fp32 (T below 2^-128) as well.
+__device__ __forceinline__ float ls_slope(float slope, float scale, float per_t) {
+  slope *= scale;
+  if (slope == 0.0f) return 0.0f;
+  slope *= per_t;
   return fabsf(slope) > 0.25f * F32_MAX ? copysignf(0.25f * F32_MAX, slope) : slope;
 }
 
@@ -559,7 +564,7 @@ __global__ void __launch_bounds__(LS_NT) k_ls_grad(LsArgs a, float written) {
   for (unsigned i = blockIdx.x; i < (unsigned)a.R * a.G; i += gridDim.x) {
     const int row = a.R - 1 - (int)(i / a.G), ch = i % a.G;
     const LsRow q = a.rows[row];
-    const float slope = q.mode ? ls_held(a.slope[q.slot] * scale * q.per_t) : 0.0f;
+    const float slope = q.mode ? ls_slope(a.slope[q.slot], scale, q.per_t) : 0.0f;
     ls_grad_part<T, U, LS_NT>(q, ls_row<T>(a, row), (T*)a.grad + (long long)row * a.grad_stride, a.V, ch * a.per, ch * a.per + a.per, slope);
   }
 }
@@ -648,7 +653,7 @@ __global__ void __launch_bounds__(NT) k_ls_policy(LsArgs a) {
     a.term[row] = ls_policy<T>(a, row, tok, v, c, temp);
     const LsRow q = a.rows[row];  // this thread's own
     s_row = q;
-    s_slope = q.mode ? ls_held(a.slope[row] * ((a.weights ? 1.0f : a.head->scale) * a.grad_scale) * q.per_t) : 0.0f;
+    s_slope = q.mode ? ls_slope(a.slope[row], (a.weights ? 1.0f : a.head->scale) * a.grad_scale, q.per_t) : 0.0f;
   }
   bar();
   const LsRow q = s_row;

@@ -536,3 +536,26 @@ def test_saved_tensor_hooks_and_checkpoints(loss, R, V, dtype):
         (a,) = torch.autograd.grad(factor * l, leaf)
         assert torch.equal(a, 2 * factor * g2)
         del junk
+
+
+@pytest.mark.parametrize("R,V", [(6, 100003), (6, 300), (140, 50001)])
+@pytest.mark.parametrize("temperature", [2.0 ** -100, 1e-39, 2.0 ** -149])
+def test_no_slope_at_the_smallest_temperatures(R, V, temperature):
+    """A row without a slope (clipped, no advantage, no weight) has a gradient of zeros at every temperature, where 1 / T
+    is past fp32 as well; the others' stay finite.  At such a temperature the best token's p is 1, and its gradient 0."""
+    logits, x, _ = logits_of(R, V, torch.float32, 21)
+    tokens = logits.argmax(1).to(torch.int32)
+    old, adv, w = torch.zeros(R, device="cuda"), torch.ones(R, device="cuda"), torch.ones(R, device="cuda")
+    old[0] = -1.0  # r = e: clipped
+    adv[1], w[2] = 0.0, 0.0
+    T = torch.full((R,), temperature, device="cuda")
+    fn = q.PolicyLoss("cuda")
+    for weights in (None, w):
+        out, g = fn.value_and_grad(logits, tokens, old, adv, weights=weights, temperature=T)
+        assert torch.isfinite(out.loss) and (out.logprobs == 0).all() and (g[:2] == 0).all() and torch.isfinite(g).all()
+        leaf = logits.detach().requires_grad_()
+        l = fn(leaf, tokens, old, adv, weights=weights, temperature=T).loss
+        (a,) = torch.autograd.grad(l, leaf, retain_graph=True)
+        (b,) = torch.autograd.grad(l * 0.0, leaf)
+        assert (a[:2] == 0).all() and torch.isfinite(a).all() and (b == 0).all()
+    assert (g[2] == 0).all()
