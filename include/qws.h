@@ -422,7 +422,8 @@ int qws_int4_head(const void* packed, int N, int K, int group, const void* x, lo
  *   u = beta ((s_2p - ref_2p) - (s_2p+1 - ref_2p+1)) - margin    (ref [2 P] or NULL: 0)
  *   l = -(1 - smoothing) ln sigmoid(u) - smoothing ln sigmoid(-u);  loss = sum w l, weights [P] or NULL: the mean.
  *   out_logprobs [2 P] = s, out_margins [P] = u, out_token_logprobs [R]: optional.
- * NaN among what a used row or pair brings makes the loss and the gradient's rows that depend on it NaN.
+ * NaN among what a used row or pair brings makes the loss and the gradient's rows that depend on it NaN; an upstream gradient that is
+ * not finite makes no element of a row with a slope finite.
  *
  * grad (optional): [R][V] of the logits' type, rows grad_stride >= V apart, apart from the logits: the loss's derivative times
  * grad_scale, every row written (0 where there is none).  qws_loss_grad writes it later, times *upstream (device, NULL: 1), from the

@@ -545,13 +545,14 @@ __device__ __forceinline__ void ls_grad_part(const LsRow& q, const T* x_row, T* 
     }
   }
 }
-// A row's slope at its logits.  Held where it passes fp32: no infinity meets a p of 0; NaN stays.  A slope of 0 is one at every
-// temperature, where 1 / T is past fp32 (T below 2^-128) as well.
+// A row's slope at its logits.  Held where it passes fp32: no infinity meets a p of 0; NaN stays, and so does what an upstream
+// gradient that is not finite makes of it, which a loss scaler looks for.  A slope of 0 is one at every temperature, where 1 / T is
+// past fp32 (T below 2^-128) as well.
 __device__ __forceinline__ float ls_slope(float slope, float scale, float per_t) {
   slope *= scale;
   if (slope == 0.0f) return 0.0f;
   slope *= per_t;
-  return fabsf(slope) > 0.25f * F32_MAX ? copysignf(0.25f * F32_MAX, slope) : slope;
+  return fabsf(slope) > 0.25f * F32_MAX && fabsf(scale) <= F32_MAX ? copysignf(0.25f * F32_MAX, slope) : slope;
 }
 
 // written != 0: the gradient is there, for an upstream of that value.  Rows from the last on: the logits that k_ls_scan read last may still be in the

@@ -559,3 +559,21 @@ def test_no_slope_at_the_smallest_temperatures(R, V, temperature):
         (b,) = torch.autograd.grad(l * 0.0, leaf)
         assert (a[:2] == 0).all() and torch.isfinite(a).all() and (b == 0).all()
     assert (g[2] == 0).all()
+
+
+@pytest.mark.parametrize("loss", ["policy", "preference"])
+@pytest.mark.parametrize("upstream", [INF, -INF, NAN])
+def test_upstream_gradients_that_are_not_finite(loss, upstream):
+    """They reach the gradient of every row that has a slope (a loss scaler looks for them there); the others stay 0."""
+    R, V = 8, 1003
+    logits, x, tokens = logits_of(R, V, torch.float32, 7)
+    tokens[3] = -1
+    old = np.array([O.log_softmax(r)[max(int(t), 0)] for r, t in zip(x.numpy(), tokens)], np.float32)
+    if loss == "policy":
+        fn, args = q.PolicyLoss("cuda"), (tokens.cuda(), dev(old), torch.ones(R, device="cuda"))
+    else:
+        fn, args = q.PreferenceLoss("cuda"), (tokens.cuda(), dev(np.array([0, 2, 5, 6, 8], np.int32)))
+    leaf = logits.detach().requires_grad_()
+    (g,) = torch.autograd.grad(fn(leaf, *args).loss, leaf, grad_outputs=torch.tensor(upstream, device="cuda"))
+    has = [0, 1, 2, 4, 5, 6, 7]
+    assert not torch.isfinite(g[has]).any() and (g[3] == 0).all()
