@@ -7,6 +7,7 @@ import math
 from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -103,6 +104,12 @@ class _Loss(torch.autograd.Function):
         return grad, None, None, None
 
 
+def no_tangent(t, name):
+    """Forward-mode derivatives are not given: without a refusal a loss would come back as one that does not depend on `t`."""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValidationError(f"{name} carries a tangent: no forward-mode derivatives", name)
+
+
 class _Base:
     def __init__(self, device):
         self.lib = _lib.load()
@@ -112,6 +119,7 @@ class _Base:
     def _rows(self, logits, tokens, temperature=None):
         """The checks of the rows, and their structure."""
         dtype, dev = logits.dtype, logits.device
+        no_tangent(logits, "logits")
         if not logits.is_cuda or (dtype != torch.float32 and dtype != torch.bfloat16):
             raise ValidationError("logits must be a CUDA fp32 / bf16 tensor", "logits")
         if dev != self.device and (self.device.type != "cuda" or self.device.index is not None):
@@ -130,6 +138,7 @@ class _Base:
             given(t, shape, torch.float32, dev, name)
         if t.requires_grad:
             raise ValidationError(f"{name} is taken as a constant: detach it", name)
+        no_tangent(t, name)
         return t.data_ptr()
 
     def _state(self, query, *key):

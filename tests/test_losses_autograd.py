@@ -5,6 +5,7 @@ from types import SimpleNamespace
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.utils.checkpoint import checkpoint
 
 import qwen_warp_amd as q
@@ -99,3 +100,20 @@ def test_backward_refuses_other_logits(lib):
         with pytest.raises(q.ValidationError):
             loss.backward()
     assert not lib.calls
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor does not require a gradient, and a loss without a tangent would read as one that does not depend on it."""
+    x, t, v = torch.zeros(2, 3), torch.zeros(2, dtype=torch.int32), torch.zeros(2)
+    fn, pl = q.PolicyLoss("cuda"), q.PreferenceLoss("cuda")
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones(2, 3))
+        for call in (lambda: fn(d, t, v, v), lambda: fn.value_and_grad(d, t, v, v), lambda: pl(d, t, torch.tensor([0, 1, 2], dtype=torch.int32))):
+            with pytest.raises(q.ValidationError, match="tangent"):
+                call()
+        c = forward_ad.make_dual(v, torch.ones(2))
+        with pytest.raises(q.ValidationError, match="advantages.*tangent"):
+            fn._number(c, (2,), v.device, "advantages")
+        assert fn._number(v, (2,), v.device, "advantages") == v.data_ptr()
+    with pytest.raises(q.ValidationError, match="CUDA"):
+        fn(x, t, v, v)
