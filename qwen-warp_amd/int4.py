@@ -8,7 +8,7 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .logprobs import on_stream, rows_of
+from .logprobs import no_tangent, on_stream, rows_of
 from .sampling import ValidationError
 
 GROUPS = (32, 64, 128)
@@ -65,7 +65,11 @@ class Int4Head:
         self._w = self.packed.data_ptr()
 
     def __call__(self, x: torch.Tensor, dtype=torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """The logits [T, N] of hidden states x [T, K] in fp32 or bf16; out: a tensor of that type to write them into."""
+        """The logits [T, N] of hidden states x [T, K] in fp32 or bf16; out: a tensor of that type to write them into.  They are
+        constants: an x that requires a gradient is taken under torch.no_grad() alone."""
+        if x.requires_grad and torch.is_grad_enabled():
+            raise ValidationError("x requires a gradient, which the head does not give: detach it, or call under torch.no_grad()", "x")
+        no_tangent(x, "x")
         if x.dtype != torch.bfloat16 or x.device != self.device or x.dim() != 2 or x.shape[1] != self.K:
             raise ValidationError(f"x must be a bf16 [T, {self.K}] tensor on {self.device}", "x")
         T, stride = rows_of(x, "x")

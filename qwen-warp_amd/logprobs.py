@@ -8,6 +8,7 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check
@@ -49,6 +50,12 @@ def rows_of(x: torch.Tensor, name: str):
 def given(t: torch.Tensor, shape, dtype, device, name: str):
     if t.dtype != dtype or t.device != device or t.shape != shape or not t.is_contiguous():
         raise ValidationError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}", name)
+
+
+def no_tangent(t, name):
+    """Forward-mode derivatives are not given: without a refusal a result would come back as one that does not depend on `t`."""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValidationError(f"{name} carries a tangent: no forward-mode derivatives", name)
 
 
 def on_stream(index: int):

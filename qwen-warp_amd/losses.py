@@ -7,12 +7,11 @@ import math
 from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
-from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import check
-from .logprobs import INT_MAX, given, on_stream
+from .logprobs import INT_MAX, given, no_tangent, on_stream
 from .sampling import ValidationError
 
 
@@ -102,12 +101,6 @@ class _Loss(torch.autograd.Function):
             if err:
                 check(err, "qws_loss_grad")
         return grad, None, None, None
-
-
-def no_tangent(t, name):
-    """Forward-mode derivatives are not given: without a refusal a loss would come back as one that does not depend on `t`."""
-    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
-        raise ValidationError(f"{name} carries a tangent: no forward-mode derivatives", name)
 
 
 class _Base:

@@ -232,3 +232,15 @@ def test_streams_and_graph():
         assert torch.equal(head(o), y)
         torch.cuda.synchronize()
         assert torch.equal(got, y)
+
+
+def test_hidden_states_of_a_trained_model():
+    """Hidden states that require a gradient: taken under no_grad, and weights that do are packed as they are."""
+    w, x = weights(300, 64, 1).cuda().requires_grad_(), states(3, 64, 2).cuda()
+    head = q.Int4Head(w, group=32)
+    leaf = x.clone().requires_grad_()
+    with pytest.raises(q.ValidationError):
+        head(leaf)
+    with torch.no_grad():
+        got = head(leaf)
+    assert torch.equal(got, head(x)) and torch.equal(head(leaf.detach()), got) and not got.requires_grad

@@ -75,3 +75,15 @@ def test_python_refusals():
         q.Int4Head(torch.zeros(4, 4))  # not on a GPU
     with pytest.raises(q.ValidationError):
         q.Int4Head.from_codes(torch.zeros(4, 4, dtype=torch.uint8), torch.ones(4, 1, dtype=torch.bfloat16))
+
+
+def test_hidden_states_that_want_a_derivative_are_refused():
+    """The head gives none: its logits would come back as constants.  Under no_grad, and detached, they go in."""
+    head = q.Int4Head.__new__(q.Int4Head)
+    head.K, head.device = 4, torch.device("cpu")
+    x = torch.zeros(2, 4, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(q.ValidationError, match="gradient"):
+        head(x)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(q.ValidationError, match="tangent"):
+            head(torch.autograd.forward_ad.make_dual(x.detach(), torch.ones(2, 4, dtype=torch.bfloat16)))
