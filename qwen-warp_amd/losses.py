@@ -64,6 +64,14 @@ def structure(logits, tokens: int, temperature: Optional[int] = None):
                          tokens, temperature)
 
 
+def not_captured():
+    """A backward pass there ends the process where an eager graph of the same leaves lives (a leaf's node belongs to that graph's
+    stream, which is not captured).  Of a loss whose forward pass ran before, replays would read logits and state that were given
+    back since."""
+    if torch.cuda.is_current_stream_capturing():
+        raise ValidationError("inside a captured graph the gradient is value_and_grad's", "logits")
+
+
 class _Loss(torch.autograd.Function):
     """The loss as a function of the logits; `call(grad, scale)` runs it and returns (loss, rows, state, what they refer to).  With
     `ahead` (not 0) the gradient is written by the forward pass, for an upstream gradient of that value; the first backward pass
@@ -82,6 +90,7 @@ class _Loss(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream):
+        not_captured()
         (logits,) = ctx.saved_tensors
         if (logits.shape, logits.dtype, logits.device) != ctx.of:
             raise ValidationError(f"the saved logits came back as {logits.dtype} {tuple(logits.shape)} on {logits.device}", "logits")
@@ -146,8 +155,7 @@ class _Base:
         """The loss, with autograd where the logits ask for it."""
         if not (logits.requires_grad and torch.is_grad_enabled()):
             return call(None, 1.0)[0]
-        if torch.cuda.is_current_stream_capturing():  # a backward pass there ends the process where an eager graph of the same leaves lives
-            raise ValidationError("inside a captured graph the gradient is value_and_grad's", "logits")
+        not_captured()
         return _Loss.apply(logits, self, call, ahead)
 
 

@@ -117,3 +117,18 @@ def test_forward_mode_is_refused():
         assert fn._number(v, (2,), v.device, "advantages") == v.data_ptr()
     with pytest.raises(q.ValidationError, match="CUDA"):
         fn(x, t, v, v)
+
+
+@pytest.mark.parametrize("ahead", [0.0, 1.0])
+def test_backward_in_a_captured_graph_is_refused(lib, monkeypatch, ahead):
+    """Of a loss whose forward pass ran before: a replay would read logits and state that were given back, or find a gradient
+    written that is someone else's by then.  Outside, the same loss still has its gradient."""
+    x = torch.randn(3, 7, requires_grad=True)
+    loss = loss_of(lib, x * 2.0, ahead)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(q.ValidationError, match="captured"):
+        loss.backward(retain_graph=True)
+    assert x.grad is None and not lib.calls
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    loss.backward()
+    assert torch.equal(x.grad, 4.0 * x.detach()) and lib.calls[-1].written == ahead
