@@ -244,3 +244,28 @@ def test_hidden_states_of_a_trained_model():
     with torch.no_grad():
         got = head(leaf)
     assert torch.equal(got, head(x)) and torch.equal(head(leaf.detach()), got) and not got.requires_grad
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("T,N,K,frags", [(1, 8191, 5120, 0), (5, 50001, 5120, 0), (30, 8191, 5120, 0), (30, 32001, 5120, 0), (50, 16001, 5120, 0), (100, 39589, 256, 0), (3, 8191, 1000, 0),
+                                         (16, 50001, 5120, 1), (30, 50001, 5120, 2), (48, 50001, 5120, 3), (64, 50001, 5120, 4), (129, 32001, 5120, 3), (100, 32001, 5120, 4), (48, 50001, 2600, 3)])
+def test_sums_are_fp32(T, N, K, frags, group):
+    """The logits' error as a whole, at the sizes where the bound of each (above) is a percent of a logit.  With codes and zero points
+    uniform over 0 .. 15 and independent hidden states of size 1, a sum of i terms (16 + q) x or (16 + z) x is about 24 sqrt(i).  Were
+    each of a group's g additions rounded, independently and by at most 2^-24 of the sum, a group's two sums would be off by
+    24 sqrt(2 g^2 / 2) 2^-24, and its result is about 6.5 sqrt(g) (q - z has variance 2 (16^2 - 1) / 12): 3.7 sqrt(g) 2^-24 of it.  The
+    K / g scaled ones add less than sqrt(K / g) 2^-24, the last steps a few.  Group sums in fp16 put the logits off by 1e-3, in 16 bits by 3e-5."""
+    if frags:
+        kb = -(-K // 128)
+        assert _lib.load().qws_int4_head_ws_bytes(T, N, K, group) == -(-T // (16 * frags)) * (kb + kb % 2) * (4 * frags + 1) * 1024
+    g = torch.Generator("cuda").manual_seed(T + N)
+    codes = torch.randint(0, 16, (N, K), generator=g, dtype=torch.uint8, device="cuda")
+    shape = (N, -(-K // group))
+    z = torch.randint(0, 16, shape, generator=g, dtype=torch.uint8, device="cuda")
+    scales = (0.004 + 0.004 * torch.rand(shape, generator=g, device="cuda")).to(torch.bfloat16)
+    x = torch.randn(T, K, generator=g, device="cuda").to(torch.bfloat16)
+    got = q.Int4Head.from_codes(codes, scales, z, group=group)(x)
+    spread = lambda t: t.double().repeat_interleave(group, 1)[:, :K]  # noqa: E731
+    want = x.double() @ (spread(scales) * (codes.double() - spread(z))).t()
+    off = float((got.double() - want).norm() / want.norm())
+    assert off <= (4 * group ** 0.5 + (K / group) ** 0.5 + 4) * 2.0 ** -24
