@@ -391,8 +391,9 @@ int qws_fp8_score(const void* packed, int N, int K, const void* x, long long x_s
  *                        (or fp16) rows scale_stride apart; zeros, like scales, in the low four bits, or NULL: 8.
  *   qws_int4_head:       x [T][K] bf16 (rows x_stride elements apart) -> out [T][N] (fp32 or bf16, rows out_stride >= N apart).
  * A hidden state that is not finite makes its logits NaN; finite ones are to stay below 2^115, so that a group's sum of 31 * 128
- * of them stays in fp32.  Any N <= 2^24, K <= 2^20, T <= 2^22 (else QWS_ERR_NOT_SUPPORTED), any stride and alignment of the
- * element's size; T = 0 does nothing.  ws: qws_int4_head_ws_bytes(T, N, K, group) bytes, 256-byte aligned, no zeroing needed; calls that
+ * of them stays in fp32.  Any N <= 2^24, K <= 2^20, T <= 2^22 (else QWS_ERR_NOT_SUPPORTED, as for a product
+ * of more than 2^24 - 1 workgroups: there are at most N / 64, rounded up to a multiple of 8, times T / 16, rounded up), any stride and
+ * alignment of the element's size; T = 0 does nothing.  ws: qws_int4_head_ws_bytes(T, N, K, group) bytes, 256-byte aligned, no zeroing needed; calls that
  * share one must be ordered.  Stream-ordered, allocate nothing, deterministic. */
 size_t qws_int4_pack_bytes(int N, int K, int group);
 int qws_int4_pack(const void* w, int dtype, int N, int K, long long row_stride, int group, void* packed, void* stream);

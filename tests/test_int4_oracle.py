@@ -87,3 +87,12 @@ def test_hidden_states_that_want_a_derivative_are_refused():
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(q.ValidationError, match="tangent"):
             head(torch.autograd.forward_ad.make_dual(x.detach(), torch.ones(2, 4, dtype=torch.bfloat16)))
+
+
+def test_products_of_too_many_workgroups():
+    """Refused before anything is launched; N / 64 times T / 16 says which."""
+    lib = _lib.load()
+    p = C.c_void_p(256)
+    for N, T in ((1 << 24, 1 << 22), (1 << 24, 1 << 14), (1 << 20, 1 << 21)):
+        n = lib.qws_int4_head_ws_bytes(T, N, 128, 128)
+        assert n > 0 and lib.qws_int4_head(p, N, 128, 128, p, 128, T, p, 0, N, p, n, None) == _lib.ERR_NOT_SUPPORTED
