@@ -13,13 +13,13 @@
 //   k_ls_policy      a workgroup per row: the policy loss with its gradient.  Bound by the bytes: 2,048 bf16 rows of 248,320 391 us, 5.2
 //                    TB/s of 2.03 GB, which is what was read and written (a large copy makes 4.97); 512 fp32 rows 210 us, 1.26 GB with
 //                    what a row's workgroup cannot keep, read twice; a few short rows by one row's latency, 13 us for 32,001 logits.
-//   k_ls_scan        R x G workgroups: each lane's running maximum and sum.  Bound by the bytes: 256 fp32 rows 44 us, 5.8 TB/s; 1,200 bf16
-//                    rows 99 us, 5.6 TB/s of those with a token.
+//   k_ls_scan        R x G workgroups: each lane's running maximum and sum.  Bound by the bytes of the rows with a token: 240 of 256
+//                    fp32 rows 44 us, 5.4 TB/s; 1,125 of 1,200 bf16 rows 99 us, 5.6 TB/s.
 //   k_ls_policy_rows a wave per row: joins the row's parts, log p, the row's term and slope (5.4 us up to 512 rows: latency)
 //   k_ls_rows        the same for the preference loss: log p and the row's sequence (5-6 us)
 //   k_ls_pairs       a wave per pair: the sequences' sums, the pair's term, the two slopes
 //   k_ls_sum         the loss: the sum of the terms (4-5 us); k_ls_few, k_ls_policy_few: pairs and a few rows in the same launch (5-10 us)
-//   k_ls_grad        R x G workgroups: the gradient's rows.  Bound by the bytes: 1,200 bf16 rows 193 us, 5.9 TB/s; where it finds the
+//   k_ls_grad        R x G workgroups: the gradient's rows.  Bound by the bytes: 1,200 bf16 rows 193 us, 6.0 TB/s; where it finds the
 //                    gradient written 4.5 us.
 #include "qws_logits.h"
 
@@ -408,7 +408,10 @@ __global__ void __launch_bounds__(LS_ONE) k_ls_sum(LsArgs a, int n) {
 }
 // One workgroup for a few pairs (and, with ROWS, a few rows): rows, pairs and the loss without launches between them, 3 us of the
 // host's time each.  Rows go to the waves in turn, which the card pays for from some number on: the policy loss of 16 rows of 248,320
-// without gradient 14.2 us in a graph in one launch behind the scan, 14.4 in two, of 40 rows 16.0 and 12.4, of 64 24.3 and 14.6.
+// without gradient 14.2 us in a graph in one launch behind the scan, 14.4 in two, of 40 rows 16.0 and 12.4, of 64 24.3 and 14.6.  The
+// preference loss of 16, 32, 48 and 64 rows of 248,320 takes 12.2, 16.8, 18.0 and 21.9 us in a graph in one launch, 12.6, 15.1, 14.1 and
+// 16.1 in two, but called one by one, where the host's time counts, 20.4, 19.9, 20.1 and 22.9 against 22.4, 22.4, 22.7 and 23.2; of 96 rows
+// of 32,001 25.3 against 22.6.
 constexpr int LS_FEW = 64, LS_FEW_ROWS = 48, LS_FEW_POLICY = 16;  // pairs; rows of the preference loss; rows of the policy loss, whose exponentials in 64 bits take longer
 template <typename T, bool ROWS>
 __global__ void __launch_bounds__(LS_ONE) k_ls_few(LsArgs a) {
@@ -789,9 +792,9 @@ static void ls_grad(const LsArgs& a, int dtype, float written, hipStream_t st) {
   dtype == QWS_DTYPE_F32 ? ls_grad_of<float>(a, written, st) : ls_grad_of<uint16_t>(a, written, st);
 }
 // Whether a policy loss with its gradient takes a workgroup per row (k_ls_policy): from 128 rows on, or where the row's workgroup holds
-// all of it (up to 12,288 vectors).  Measured, us a call, k_ls_policy / the three launches: 248,320 bf16 logits, 64 rows 38 / 29, 100 rows 39 /
-// 32, 150 rows 42 / 45, 256 rows 56 / 77, 2,048 rows 417 / 571; fp32, 64 rows 45 / 36, 192 rows 112 / 115, 512 rows 254 / 296;
-// 32,001 bf16 logits, 64 rows 26 / 29, 1,024 rows 32 / 42.
+// all of it (up to 12,288 vectors).  Measured, us a call, k_ls_policy / the launches of ls_policy_run and k_ls_grad: 248,320 bf16 logits, 16 rows
+// 35 / 26, 64 rows 37 / 28, 100 rows 38 / 36, 128 rows 38 / 42, 150 rows 39 / 45, 256 rows 58 / 68, 2,048 rows 396 / 528; fp32, 64 rows 43 / 40,
+// 100 rows 55 / 57, 128 rows 64 / 68, 192 rows 91 / 97, 512 rows 215 / 250; 32,001 bf16 logits, 64 rows 26 / 27, 1,024 rows 36 / 48.
 constexpr int LS_HELD = 512 * 24;
 static int ls_vectors(int dtype, int V) { return V / (dtype == QWS_DTYPE_F32 ? 4 : 8); }
 static bool ls_one_pass(int dtype, int R, int V) { return R >= 128 || ls_vectors(dtype, V) <= LS_HELD; }
@@ -801,8 +804,9 @@ static void ls_policy_rows(const LsArgs& a, hipStream_t st) {
 }
 // The least workgroup that holds a row: 2,048 bf16 rows, us with 256 x 16 / 512 x 24 / 1,024 x 24 vectors: of 16,000 logits 33 / 42 / 64,
 // of 32,001 65 / 72 / 95, of 40,000 82 / 81 / 101, of 100,000 221 / 181 / 188, of 130,000 308 / 239 / 244, of 200,000 439 / 376 / 347.  Where
-// there are at most two rows to a CU the larger one is quicker from some 2,000 vectors on: 32,001 bf16 logits, 24 rows 16.2 / 12.9, 400
-// rows 21.0 / 18.1; 16,000 bf16 logits, 100 rows 11.3 / 10.4; 8,000, 4 rows 8.9 / 9.1.
+// there are at most two rows to a CU the larger one is quicker from some 2,000 vectors on (in a graph): 32,001 bf16 logits, 24 rows 16.9 /
+// 14.4, 400 rows 21.4 / 19.0; 16,000 (2,000 vectors: the border), 100 rows 12.8 / 12.0, 400 rows 15.1 / 14.7; 12,000, 100 rows 11.9 /
+// 11.8; 8,000, 4 and 100 rows 10.9 / 11.0.
 template <typename T>
 static void ls_policy_one_pass(const LsArgs& a, hipStream_t st) {
   const int n = a.V / lp_e<T>();
